@@ -55,6 +55,15 @@ SIGNATURES = {
     "ldm_conv_create": (_i, [C.POINTER(_vp), _i, _i, _i, _i, _i, _vp, _vp]),
     "ldm_conv_forward": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "ldm_conv_destroy": (None, [_vp]),
+    "ldm_layer_norm": (_i, [_i, _vp, _l, _vp, _vp, C.c_float, _vp, _l, _vp, _vp, _l, _i, _vp]),
+    "ldm_layer_norm_ws_floats": (_l, [_i, _l, _i]),
+    "ldm_layer_norm_backward": (_i, [_i, _vp, _l, _vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _l, _vp, _vp, _vp, _l, _i, _vp]),
+    "ldm_rope": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "ldm_linear_ws_floats": (_l, [_i, _l, _l, _l, _i]),
+    "ldm_linear": (_i, [_i, _vp, _l, _vp, _l, _i, _vp, _vp, _l, _i, _vp, _l, _vp, _l, _l, _l, _l, _vp, _vp]),
+    "ldm_linear_backward_ws_floats": (_l, [_i, _l, _l, _l, _i]),
+    "ldm_linear_backward": (_i, [_i, _vp, _l, _vp, _l, _vp, _l, _i, _vp, _l, _i, _vp, _l, _vp, _l, _vp, _l, _vp, _vp, _l, _l,
+                                 _l, _vp]),
     "ldm_sched_step": (_i, [_vp, _vp, _vp, _l, _fp, _i, _i, _vp]),
     "ldm_sampler_create": (_i, [C.POINTER(_vp), _vp, _i, _i, _i, _i]),
     "ldm_sampler_run": (_i, [_vp, _i, _i, _vp, _vp, _u64, _u32, _vp, _vp, _vp, _i, _vp]),

@@ -1,0 +1,475 @@
+// Layer norm over the last axis, forward and backward (no counterpart in the reference, whose blocks use batch norm):
+//   y  = (x - mu) r w + b,   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps)
+//   dx = r (g - mean(g) - xh mean(g xh)) + add,   xh = (x - mu) r, g = dy w;   dw = sum_rows dy xh, db = sum_rows dy
+// Both passes are bound by HBM: one read of each input and one write of the output.  A row lives in the registers of its
+// LPR lanes (a part of a wave, a wave, or a workgroup), so the mean, the centred sum of squares and the output come from
+// one read.  Statistics and all sums are f32; the variance is the sum of squares around the mean that was just found
+// (E[x^2] - mu^2 would lose it for rows far from zero).
+// Rows need no alignment: 16-byte vector accesses at element alignment, which this target's global memory serves.
+#include "blocks.h"
+
+namespace ldm {
+
+namespace {
+
+struct LnFwdArgs {
+    const char* x;
+    char* y;
+    const float *w, *b;
+    float *mean, *rstd;
+    long xs, ys;       // row strides in elements
+    long rows;
+    int C;
+    float eps;
+};
+struct LnBwdArgs {
+    const char *dy, *x, *add;
+    char* dx;
+    const float *mean, *rstd, *w;
+    float* part;       // [2][gridDim.x][C] partial sums of dw and db, or null
+    long dys, xs, as, dxs;
+    long rows;
+    int C;
+};
+
+template <typename T> struct LnVec;
+template <> struct LnVec<float> {
+    static constexpr int N = 4;
+    typedef float V __attribute__((ext_vector_type(4), aligned(4)));
+    static __device__ __forceinline__ float get(const float* p) { return *p; }
+    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+    static __device__ __forceinline__ void load(const float* p, float* o) {
+        const V v = *(const V*)p;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = v[e];
+    }
+    static __device__ __forceinline__ void store(float* p, const float* o) {
+        V v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = o[e];
+        *(V*)p = v;
+    }
+};
+template <> struct LnVec<__bf16> {
+    static constexpr int N = 8;
+    typedef __bf16 V __attribute__((ext_vector_type(8), aligned(2)));
+    typedef float F __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ float get(const __bf16* p) { return (float)*p; }
+    static __device__ __forceinline__ void put(__bf16* p, float v) { *p = (__bf16)v; }
+    static __device__ __forceinline__ void load(const __bf16* p, float* o) {
+        const F v = __builtin_convertvector(*(const V*)p, F);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = v[e];
+    }
+    static __device__ __forceinline__ void store(__bf16* p, const float* o) {
+        F v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = o[e];
+        *(V*)p = __builtin_convertvector(v, V);
+    }
+};
+
+// VEC elements at column c of a row of C (zero behind its end)
+template <typename T>
+__device__ __forceinline__ void ln_load(const T* row, int c, int C, float* o) {
+    constexpr int N = LnVec<T>::N;
+    if (c + N <= C) {
+        LnVec<T>::load(row + c, o);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = c + e < C ? LnVec<T>::get(row + c + e) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void ln_store(T* row, int c, int C, const float* o) {
+    constexpr int N = LnVec<T>::N;
+    if (c + N <= C) {
+        LnVec<T>::store(row + c, o);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (c + e < C) LnVec<T>::put(row + c + e, o[e]);
+    }
+}
+// NE f32 parameters of the columns c .. c + NE - 1
+template <int NE>
+__device__ __forceinline__ void ln_param(const float* p, int c, int C, float dflt, float* o) {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) o[e] = p && c + e < C ? p[c + e] : dflt;
+}
+
+// sums over the LPR lanes of a row, the same bits in every lane; LPR = 256: the whole workgroup, through `sm` (8 floats)
+template <int LPR>
+__device__ __forceinline__ void ln_sum2(float& a, float& b, float* sm) {
+#pragma unroll
+    for (int m = 1; m < (LPR < 64 ? LPR : 64); m <<= 1) {
+        a += __shfl_xor(a, m);
+        b += __shfl_xor(b, m);
+    }
+    if constexpr (LPR > 64) {
+        __syncthreads();                 // the previous sums have been read
+        if ((threadIdx.x & 63) == 0) {
+            sm[(threadIdx.x >> 6) * 2] = a;
+            sm[(threadIdx.x >> 6) * 2 + 1] = b;
+        }
+        __syncthreads();
+        a = (sm[0] + sm[2]) + (sm[4] + sm[6]);
+        b = (sm[1] + sm[3]) + (sm[5] + sm[7]);
+    }
+}
+template <int LPR>
+__device__ __forceinline__ float ln_sum(float a, float* sm) {
+    float b = 0.f;
+    ln_sum2<LPR>(a, b, sm);
+    return a;
+}
+
+template <typename T, int NV, int LPR>
+__global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
+    constexpr int N = LnVec<T>::N, RPB = 256 / LPR;
+    __shared__ float sm[8];
+    const int l = threadIdx.x % LPR;
+    float w[NV][N], b[NV][N];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        ln_param<N>(a.w, (v * LPR + l) * N, a.C, 1.f, w[v]);
+        ln_param<N>(a.b, (v * LPR + l) * N, a.C, 0.f, b[v]);
+    }
+    const float n = (float)a.C;      // divided by, not multiplied with 1 / C: the mean of a constant row is exact
+    for (long row = (long)blockIdx.x * RPB + threadIdx.x / LPR; row < a.rows; row += (long)gridDim.x * RPB) {
+        const T* xr = (const T*)a.x + row * a.xs;
+        float x[NV][N];
+        float s = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            ln_load<T>(xr, (v * LPR + l) * N, a.C, x[v]);
+#pragma unroll
+            for (int e = 0; e < N; ++e) s += x[v][e];
+        }
+        const float mu = ln_sum<LPR>(s, sm) / n;
+        float q = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                x[v][e] -= mu;
+                if ((v * LPR + l) * N + e < a.C) q += x[v][e] * x[v][e];
+            }
+        const float r = 1.0f / sqrtf(ln_sum<LPR>(q, sm) / n + a.eps);
+        T* yr = (T*)a.y + row * a.ys;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            float o[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) o[e] = x[v][e] * r * w[v][e] + b[v][e];
+            ln_store<T>(yr, (v * LPR + l) * N, a.C, o);
+        }
+        if (l == 0) {
+            if (a.mean) a.mean[row] = mu;
+            if (a.rstd) a.rstd[row] = r;
+        }
+    }
+}
+
+// Rows that do not fit the registers of a workgroup: one workgroup per row, which it reads three times (the second and
+// third time from the caches).
+template <typename T>
+__global__ __launch_bounds__(256) void ln_fwd_wide_kernel(LnFwdArgs a) {
+    constexpr int N = LnVec<T>::N;
+    __shared__ float sm[8];
+    const float n = (float)a.C;
+    for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* xr = (const T*)a.x + row * a.xs;
+        float s = 0.f;
+        for (int c = threadIdx.x * N; c < a.C; c += 256 * N) {
+            float x[N];
+            ln_load<T>(xr, c, a.C, x);
+#pragma unroll
+            for (int e = 0; e < N; ++e) s += x[e];
+        }
+        const float mu = ln_sum<256>(s, sm) / n;
+        float q = 0.f;
+        for (int c = threadIdx.x * N; c < a.C; c += 256 * N) {
+            float x[N];
+            ln_load<T>(xr, c, a.C, x);
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (c + e < a.C) q += (x[e] - mu) * (x[e] - mu);
+        }
+        const float r = 1.0f / sqrtf(ln_sum<256>(q, sm) / n + a.eps);
+        T* yr = (T*)a.y + row * a.ys;
+        for (int c = threadIdx.x * N; c < a.C; c += 256 * N) {
+            float x[N], w[N], b[N];
+            ln_load<T>(xr, c, a.C, x);
+            ln_param<N>(a.w, c, a.C, 1.f, w);
+            ln_param<N>(a.b, c, a.C, 0.f, b);
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = (x[e] - mu) * r * w[e] + b[e];
+            ln_store<T>(yr, c, a.C, x);
+        }
+        if (threadIdx.x == 0) {
+            if (a.mean) a.mean[row] = mu;
+            if (a.rstd) a.rstd[row] = r;
+        }
+    }
+}
+
+// Backward.  Every workgroup walks over rows and keeps its columns' sums of dy xh and dy in registers; at the end its row
+// groups are joined through LDS in a fixed order and written as one partial row, which colsum_kernel adds up.
+template <typename T, int NV, int LPR>
+__global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
+    constexpr int N = LnVec<T>::N, RPB = 256 / LPR;
+    __shared__ float sm[8];
+    __shared__ float join[256 * N];
+    const int l = threadIdx.x % LPR;
+    float w[NV][N], aw[NV][N], ab[NV][N];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        ln_param<N>(a.w, (v * LPR + l) * N, a.C, 1.f, w[v]);
+#pragma unroll
+        for (int e = 0; e < N; ++e) aw[v][e] = ab[v][e] = 0.f;
+    }
+    const float inv = 1.0f / (float)a.C;
+    for (long row = (long)blockIdx.x * RPB + threadIdx.x / LPR; row < a.rows; row += (long)gridDim.x * RPB) {
+        const T* xr = (const T*)a.x + row * a.xs;
+        const T* dr = (const T*)a.dy + row * a.dys;
+        float xh[NV][N], g[NV][N];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            ln_load<T>(xr, (v * LPR + l) * N, a.C, xh[v]);
+            ln_load<T>(dr, (v * LPR + l) * N, a.C, g[v]);
+        }
+        const float mu = a.mean[row], r = a.rstd[row];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if ((v * LPR + l) * N + e < a.C) xh[v][e] = (xh[v][e] - mu) * r;
+                aw[v][e] += g[v][e] * xh[v][e];
+                ab[v][e] += g[v][e];
+                g[v][e] *= w[v][e];
+                s1 += g[v][e];
+                s2 += g[v][e] * xh[v][e];
+            }
+        ln_sum2<LPR>(s1, s2, sm);
+        s1 *= inv;
+        s2 *= inv;
+        T* or_ = (T*)a.dx + row * a.dxs;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            float o[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) o[e] = r * (g[v][e] - s1 - xh[v][e] * s2);
+            if (a.add) {
+                float p[N];
+                ln_load<T>((const T*)a.add + row * a.as, (v * LPR + l) * N, a.C, p);
+#pragma unroll
+                for (int e = 0; e < N; ++e) o[e] += p[e];
+            }
+            ln_store<T>(or_, (v * LPR + l) * N, a.C, o);
+        }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float* dst = a.part + ((long)k * gridDim.x + blockIdx.x) * a.C;
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < N; ++e) join[threadIdx.x * N + e] = k ? ab[v][e] : aw[v][e];
+            __syncthreads();
+            for (int i = threadIdx.x; i < LPR * N; i += 256) {
+                float s = 0.f;
+#pragma unroll
+                for (int j = 0; j < RPB; ++j) s += join[j * LPR * N + i];
+                const int c = v * LPR * N + i;
+                if (c < a.C) dst[c] = s;
+            }
+        }
+}
+
+// Rows too long for the registers: dx by re-reading the row, and the columns' sums by a kernel of their own.
+template <typename T>
+__global__ __launch_bounds__(256) void ln_bwd_wide_dx_kernel(LnBwdArgs a) {
+    constexpr int N = LnVec<T>::N;
+    __shared__ float sm[8];
+    const float inv = 1.0f / (float)a.C;
+    for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* xr = (const T*)a.x + row * a.xs;
+        const T* dr = (const T*)a.dy + row * a.dys;
+        const float mu = a.mean[row], r = a.rstd[row];
+        float s1 = 0.f, s2 = 0.f;
+        for (int c = threadIdx.x * N; c < a.C; c += 256 * N) {
+            float x[N], d[N], w[N];
+            ln_load<T>(xr, c, a.C, x);
+            ln_load<T>(dr, c, a.C, d);
+            ln_param<N>(a.w, c, a.C, 1.f, w);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float g = d[e] * w[e];
+                s1 += g;
+                if (c + e < a.C) s2 += g * ((x[e] - mu) * r);
+            }
+        }
+        ln_sum2<256>(s1, s2, sm);
+        s1 *= inv;
+        s2 *= inv;
+        for (int c = threadIdx.x * N; c < a.C; c += 256 * N) {
+            float x[N], d[N], w[N], p[N];
+            ln_load<T>(xr, c, a.C, x);
+            ln_load<T>(dr, c, a.C, d);
+            ln_param<N>(a.w, c, a.C, 1.f, w);
+            if (a.add) ln_load<T>((const T*)a.add + row * a.as, c, a.C, p);
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                x[e] = r * (d[e] * w[e] - s1 - (x[e] - mu) * r * s2) + (a.add ? p[e] : 0.f);
+            ln_store<T>((T*)a.dx + row * a.dxs, c, a.C, x);
+        }
+    }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void ln_bwd_wide_dw_kernel(LnBwdArgs a) {
+    constexpr int N = LnVec<T>::N;
+    const int c = (blockIdx.y * 256 + threadIdx.x) * N;
+    if (c >= a.C) return;
+    float aw[N] = {}, ab[N] = {};
+    for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        float x[N], d[N];
+        ln_load<T>((const T*)a.x + row * a.xs, c, a.C, x);
+        ln_load<T>((const T*)a.dy + row * a.dys, c, a.C, d);
+        const float mu = a.mean[row], r = a.rstd[row];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            aw[e] += d[e] * ((x[e] - mu) * r);
+            ab[e] += d[e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+        if (c + e < a.C) {
+            a.part[(long)blockIdx.x * a.C + c + e] = aw[e];
+            a.part[((long)gridDim.x + blockIdx.x) * a.C + c + e] = ab[e];
+        }
+}
+
+// out[k][c] = sum over g of part[k][g][c], in a fixed order: sixteen threads per column take every sixteenth row
+__global__ __launch_bounds__(1024) void colsum_kernel(const float* part, int G, int C, float* o0, float* o1) {
+    __shared__ float sm[16][64];
+    const int cl = threadIdx.x & 63, sl = threadIdx.x >> 6;
+    const int c = blockIdx.x * 64 + cl;
+    const int k = blockIdx.y;
+    float s = 0.f;
+    if (c < C)
+        for (int g = sl; g < G; g += 16) s += part[((long)k * G + g) * C + c];
+    sm[sl][cl] = s;
+    __syncthreads();
+    if (sl == 0 && c < C) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += sm[i][cl];
+        (k ? o1 : o0)[c] = t;
+    }
+}
+
+// lanes per row and vectors per lane for nvec 16-byte vectors a row; LPR = 0: does not fit
+struct LnShape { int lpr, nv; };
+LnShape ln_shape(long C, int es) {
+    const long nvec = (C * es + 15) / 16;
+    if (nvec <= 8) return {8, 1};
+    if (nvec <= 16) return {16, 1};
+    if (nvec <= 32) return {32, 1};
+    if (nvec <= 64) return {64, 1};
+    if (nvec <= 128) return {64, 2};
+    if (nvec <= 256) return {64, 4};
+    if (nvec <= 512) return {256, 2};
+    if (nvec <= 1024) return {256, 4};
+    if (nvec <= 2048) return {256, 8};
+    return {0, 0};
+}
+constexpr int kLnMaxGroups = 1024;      // workgroups that walk over the rows: four per CU
+
+// workgroups of the backward pass = rows of its partial sums
+long ln_bwd_groups(int es, long rows, long C) {
+    const LnShape sh = ln_shape(C, es);
+    if (sh.lpr == 0) return rows < 64 ? rows : 64;
+    const long rpb = 256 / sh.lpr, n = (rows + rpb - 1) / rpb;
+    return n < kLnMaxGroups ? n : kLnMaxGroups;
+}
+
+#define LN_DISPATCH(KERNEL, T, sh, grid, s, a)                                                        \
+    do {                                                                                              \
+        if (sh.lpr == 8) KERNEL<T, 1, 8><<<grid, 256, 0, s>>>(a);                                     \
+        else if (sh.lpr == 16) KERNEL<T, 1, 16><<<grid, 256, 0, s>>>(a);                              \
+        else if (sh.lpr == 32) KERNEL<T, 1, 32><<<grid, 256, 0, s>>>(a);                              \
+        else if (sh.lpr == 64 && sh.nv == 1) KERNEL<T, 1, 64><<<grid, 256, 0, s>>>(a);                \
+        else if (sh.lpr == 64 && sh.nv == 2) KERNEL<T, 2, 64><<<grid, 256, 0, s>>>(a);                \
+        else if (sh.lpr == 64) KERNEL<T, 4, 64><<<grid, 256, 0, s>>>(a);                              \
+        else if (sh.nv == 2) KERNEL<T, 2, 256><<<grid, 256, 0, s>>>(a);                               \
+        else if (sh.nv == 4) KERNEL<T, 4, 256><<<grid, 256, 0, s>>>(a);                               \
+        else KERNEL<T, 8, 256><<<grid, 256, 0, s>>>(a);                                               \
+    } while (0)
+
+template <typename T>
+int ln_fwd(const LnFwdArgs& a, hipStream_t s) {
+    const LnShape sh = ln_shape(a.C, sizeof(T));
+    if (sh.lpr == 0) {
+        ln_fwd_wide_kernel<T><<<(unsigned)(a.rows < 2048 ? a.rows : 2048), 256, 0, s>>>(a);
+    } else {
+        const long rpb = 256 / sh.lpr, n = (a.rows + rpb - 1) / rpb;
+        const unsigned grid = (unsigned)(n < 2 * kLnMaxGroups ? n : 2 * kLnMaxGroups);
+        LN_DISPATCH(ln_fwd_kernel, T, sh, grid, s, a);
+    }
+    LDM_HIP(hipGetLastError());
+    return LDM_OK;
+}
+
+template <typename T>
+int ln_bwd(const LnBwdArgs& a, hipStream_t s) {
+    const LnShape sh = ln_shape(a.C, sizeof(T));
+    const unsigned G = (unsigned)ln_bwd_groups(sizeof(T), a.rows, a.C);
+    if (sh.lpr == 0) {
+        ln_bwd_wide_dx_kernel<T><<<(unsigned)(a.rows < 2048 ? a.rows : 2048), 256, 0, s>>>(a);
+        LDM_HIP(hipGetLastError());
+        if (a.part) {
+            const unsigned cb = (unsigned)((a.C + 256 * LnVec<T>::N - 1) / (256 * LnVec<T>::N));
+            ln_bwd_wide_dw_kernel<T><<<dim3(G, cb), 256, 0, s>>>(a);
+        }
+    } else {
+        LN_DISPATCH(ln_bwd_kernel, T, sh, G, s, a);
+    }
+    LDM_HIP(hipGetLastError());
+    return LDM_OK;
+}
+
+}  // namespace
+
+int launch_colsum(const float* part, int G, int C, int nsums, float* out0, float* out1, hipStream_t s) {
+    colsum_kernel<<<dim3((unsigned)((C + 63) / 64), (unsigned)nsums), 1024, 0, s>>>(part, G, C, out0, out1);
+    LDM_HIP(hipGetLastError());
+    return LDM_OK;
+}
+
+int launch_layer_norm(int dtype, const void* x, long xs, const float* w, const float* b, float eps, void* y, long ys,
+                      float* mean, float* rstd, long rows, int C, hipStream_t s) {
+    if (rows == 0) return LDM_OK;
+    LnFwdArgs a{(const char*)x, (char*)y, w, b, mean, rstd, xs, ys, rows, C, eps};
+    return dtype == LDM_BF16 ? ln_fwd<__bf16>(a, s) : ln_fwd<float>(a, s);
+}
+
+long ln_ws_floats(int dtype, long rows, long C) {
+    return 2 * ln_bwd_groups(dtype == LDM_BF16 ? 2 : 4, rows, C) * C;
+}
+
+int launch_layer_norm_backward(int dtype, const void* dy, long dys, const void* x, long xs, const void* add, long as,
+                               const float* mean, const float* rstd, const float* w, void* dx, long dxs, float* dw,
+                               float* db, float* ws, long rows, int C, hipStream_t s) {
+    LnBwdArgs a{(const char*)dy, (const char*)x, (const char*)add, (char*)dx, mean, rstd, w, dw ? ws : nullptr,
+                dys, xs, as, dxs, rows, C};
+    if (rows > 0) LDM_TRY(dtype == LDM_BF16 ? ln_bwd<__bf16>(a, s) : ln_bwd<float>(a, s));
+    if (!dw) return LDM_OK;
+    return launch_colsum(ws, (int)ln_bwd_groups(dtype == LDM_BF16 ? 2 : 4, rows, C), C, 2, dw, db, s);
+}
+
+}  // namespace ldm

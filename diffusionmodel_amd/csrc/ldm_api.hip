@@ -10,7 +10,7 @@
 #include <memory>
 #include <vector>
 
-#include "common.h"
+#include "blocks.h"
 
 namespace ldm {
 
@@ -1451,6 +1451,126 @@ int ldm_batchnorm_act(int dtype, const void* h, const void* res, void* out, int 
     LDM_TRY(launch_bn_stats(dtype, h, B, HW, C, gamma, beta, eps, ws, mean_out, var_out, st));
     if (!out) return LDM_OK;    // statistics only
     return launch_bn_apply(dtype, h, res, out, B, HW, C, ws, act, tvec, C, 1.0f - dropout_p, seed, st);
+}
+
+int ldm_layer_norm(int dtype, const void* x, long xs, const float* w, const float* b, float eps, void* y, long ys, float* mean,
+                   float* rstd, long rows, int C, void* stream) {
+    LDM_REQUIRE(dtype == LDM_F32 || dtype == LDM_BF16, "unknown dtype");
+    LDM_REQUIRE(rows >= 0 && C > 0 && C <= (1 << 24), "needs rows >= 0 and 1 <= C <= 2^24");
+    LDM_REQUIRE(eps >= 0.f, "eps must not be negative");
+    LDM_REQUIRE(rows == 0 || (x && y), "bad arguments");
+    LDM_REQUIRE(xs >= 0 && (ys >= C || rows <= 1), "output rows overlap");
+    return launch_layer_norm(dtype, x, xs, w, b, eps, y, ys, mean, rstd, rows, C, (hipStream_t)stream);
+}
+long ldm_layer_norm_ws_floats(int dtype, long rows, int C) {
+    if ((dtype != LDM_F32 && dtype != LDM_BF16) || rows < 0 || C <= 0) return -1;
+    return ln_ws_floats(dtype, rows, C);
+}
+int ldm_layer_norm_backward(int dtype, const void* dy, long dys, const void* x, long xs, const void* add, long as,
+                            const float* mean, const float* rstd, const float* w, void* dx, long dxs, float* dw, float* db,
+                            float* ws, long rows, int C, void* stream) {
+    LDM_REQUIRE(dtype == LDM_F32 || dtype == LDM_BF16, "unknown dtype");
+    LDM_REQUIRE(rows >= 0 && C > 0 && C <= (1 << 24), "needs rows >= 0 and 1 <= C <= 2^24");
+    LDM_REQUIRE(rows == 0 || (dy && x && mean && rstd && dx), "bad arguments");
+    LDM_REQUIRE((dw != nullptr) == (db != nullptr), "dweight and dbias go together");
+    LDM_REQUIRE(!dw || ws || rows == 0, "the parameters' gradients need a workspace");
+    LDM_REQUIRE(dys >= 0 && xs >= 0 && as >= 0 && (dxs >= C || rows <= 1), "output rows overlap");
+    return launch_layer_norm_backward(dtype, dy, dys, x, xs, add, as, mean, rstd, w, dx, dxs, dw, db, ws, rows, C,
+                                      (hipStream_t)stream);
+}
+
+int ldm_rope(int dtype, const void* q, const void* k, void* oq, void* ok, const long* st, int B, int N, int Hq, int Hk, int D,
+             const void* pos, int pos_type, const long* pst, const float* inv_freq, const int* sections, int axes,
+             int interleaved, int inverse, void* stream) {
+    LDM_REQUIRE(dtype == LDM_F32 || dtype == LDM_BF16, "unknown dtype");
+    LDM_REQUIRE(B >= 0 && N >= 0 && Hq > 0 && Hk >= 0 && D > 0 && D <= 2048, "needs Hq >= 1 and 1 <= D <= 2048");
+    LDM_REQUIRE((long)B * N < (1L << 31) && (long)Hq + Hk <= 65535, "too many tokens or heads for one launch");
+    LDM_REQUIRE(axes >= 1 && axes <= 4 && sections && st && pst, "needs 1 to 4 axes");
+    LDM_REQUIRE(pos_type >= 0 && pos_type <= 2, "unknown position type");
+    RopeArgs a = {};
+    long P = 0;
+    for (int i = 0; i < 4; ++i) {
+        LDM_REQUIRE(i >= axes || sections[i] >= 0, "sections must not be negative");
+        if (i < axes) P += sections[i];
+        a.sec_end[i] = i < axes - 1 ? (int)(P < D ? P : D) : D;      // the last axis takes what is left
+    }
+    LDM_REQUIRE(P >= 1 && 2 * P <= D, "the sections must cover between one pair and D / 2 pairs");
+    if ((long)B * N == 0) return LDM_OK;
+    LDM_REQUIRE(q && oq && pos && inv_freq && (Hk == 0 || (k && ok)), "bad arguments");
+    a.in[0] = q; a.in[1] = k; a.out[0] = oq; a.out[1] = ok;
+    for (int w = 0; w < 2; ++w) {
+        a.isb[w] = st[w * 3]; a.isn[w] = st[w * 3 + 1]; a.ish[w] = st[w * 3 + 2];
+        a.osb[w] = st[6 + w * 3]; a.osn[w] = st[7 + w * 3]; a.osh[w] = st[8 + w * 3];
+    }
+    a.H[0] = Hq; a.H[1] = Hk;
+    a.N = N; a.D = D; a.P = (int)P;
+    a.tokens = (long)B * N;
+    a.pos = pos; a.pos_dtype = pos_type;
+    a.pos_sb = pst[0]; a.pos_sa = pst[1]; a.pos_sn = pst[2];
+    a.inv_freq = inv_freq;
+    a.inverse = inverse != 0;
+    return launch_rope(dtype, interleaved, a, (hipStream_t)stream);
+}
+
+static int check_linear(int dtype, long M, long K, long N, int w_order, int act) {
+    LDM_REQUIRE(dtype == LDM_F32 || dtype == LDM_BF16, "unknown dtype");
+    LDM_REQUIRE(M >= 0 && M < (1L << 40) && K >= 1 && K < (1L << 30) && N >= 1 && N < (1L << 30),
+                "needs M >= 0 and 1 <= K, N < 2^30");
+    LDM_REQUIRE(w_order == 0 || w_order == 1, "unknown weight order");
+    LDM_REQUIRE(act >= LIN_NONE && act <= LIN_GELU, "unknown activation");
+    return LDM_OK;
+}
+long ldm_linear_ws_floats(int dtype, long M, long K, long N, int w_order) {
+    if (check_linear(dtype, M, K, N, w_order, 0) != LDM_OK) return -1;
+    return 0;
+}
+int ldm_linear(int dtype, const void* x, long ldx, const void* w, long ldw, int w_order, const float* bias, const void* res,
+               long ldres, int act, void* out, long ldo, void* pre, long ldpre, long M, long K, long N, float* ws,
+               void* stream) {
+    LDM_TRY(check_linear(dtype, M, K, N, w_order, act));
+    if (M == 0) return LDM_OK;
+    LDM_REQUIRE(x && w && out, "bad arguments");
+    LDM_REQUIRE(ldx >= 0 && ldw >= 0 && ldres >= 0, "strides must not be negative");
+    LDM_REQUIRE(M == 1 || (ldo >= N && (!pre || ldpre >= N)), "output rows overlap");
+    GemmArgs a = {};
+    a.A = x; a.lda = ldx; a.B = w; a.ldb = ldw;
+    a.bias = bias; a.res = res; a.ldr = ldres;
+    a.pre = pre; a.ldp = ldpre; a.C = out; a.ldc = ldo;
+    a.M = M; a.N = N; a.K = K; a.act = act;
+    return launch_gemm(dtype, a, true, w_order == 1, (hipStream_t)stream);
+}
+long ldm_linear_backward_ws_floats(int dtype, long M, long K, long N, int w_order) {
+    if (check_linear(dtype, M, K, N, w_order, 0) != LDM_OK) return -1;
+    return linear_dz_ws_floats(M, N);
+}
+int ldm_linear_backward(int dtype, const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, int w_order,
+                        const void* pre, long ldpre, int act, void* dz, long lddz, void* dx, long lddx, void* dw, long lddw,
+                        float* db, float* ws, long M, long K, long N, void* stream) {
+    LDM_TRY(check_linear(dtype, M, K, N, w_order, act));
+    LDM_REQUIRE(M == 0 || dy, "bad arguments");
+    LDM_REQUIRE(M == 0 || act == LIN_NONE || (pre && dz), "an activation's gradient needs pre and dz");
+    LDM_REQUIRE(M == 0 || ((!dx || w) && (!dw || x)), "dx needs the weight and dw the input");
+    LDM_REQUIRE(lddy >= 0 && ldx >= 0 && ldw >= 0 && ldpre >= 0, "strides must not be negative");
+    LDM_REQUIRE(M <= 1 || ((act == LIN_NONE || lddz >= N) && (!dx || lddx >= K)), "output rows overlap");
+    LDM_REQUIRE(!dw || (w_order == 0 ? (K == 1 || lddw >= N) : (N == 1 || lddw >= K)), "rows of dw overlap");
+    LDM_REQUIRE(!db || ws || M == 0, "dbias needs a workspace");
+    hipStream_t st = (hipStream_t)stream;
+    LDM_TRY(launch_linear_dz(dtype, dy, lddy, pre, ldpre, dz, lddz, db, ws, M, N, act, st));
+    if (act == LIN_NONE) { dz = (void*)dy; lddz = lddy; }
+    if (dx) {
+        GemmArgs a = {};
+        a.A = dz; a.lda = lddz; a.B = w; a.ldb = ldw; a.C = dx; a.ldc = lddx;
+        a.M = M; a.N = K; a.K = N;
+        LDM_TRY(launch_gemm(dtype, a, true, w_order == 0, st));
+    }
+    if (dw) {
+        GemmArgs a = {};
+        a.C = dw; a.ldc = lddw; a.K = M;
+        if (w_order == 0) { a.A = x; a.lda = ldx; a.M = K; a.B = dz; a.ldb = lddz; a.N = N; }
+        else { a.A = dz; a.lda = lddz; a.M = N; a.B = x; a.ldb = ldx; a.N = K; }
+        LDM_TRY(launch_gemm(dtype, a, false, false, st));
+    }
+    return LDM_OK;
 }
 
 int ldm_resblock_forward(ldm_module* m, const float* x, const float* t_emb, float* out, int B, int H, int W, void* stream) {

@@ -198,6 +198,53 @@ void ldm_conv_destroy(ldm_conv* c);
  * pick the hardware-counter record that belongs to the kernel it timed. */
 const char* ldm_last_kernel(void);
 
+/* ---- operators of transformer blocks over latent tokens (no counterpart in the reference) ---- */
+/* Layer norm, rotary positions and the linear layer, each with its backward pass: what a block of tokens needs around the
+ * attention.  `dtype` is the element type of the tensors (LDM_F32 / LDM_BF16); statistics, biases, norm parameters and
+ * their gradients are f32, sums are f32 whatever the type.  Strides are in elements and tensors need no alignment beyond
+ * their element's.  Workspaces belong to one call at a time: calls that may overlap take different ones.  Nothing is
+ * allocated, nothing synchronises; every call can be captured into a graph.  Sums are taken in a fixed order: the same
+ * call gives the same bits. */
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis of x [rows, C] (biased variance); weight / bias [C]
+ * or NULL.  mean_dev / rstd_dev [rows] f32, optional: what the backward pass needs.  y may be x (same stride). */
+int ldm_layer_norm(int dtype, const void* x_dev, long x_stride, const float* weight_dev, const float* bias_dev, float eps,
+                   void* y_dev, long y_stride, float* mean_dev, float* rstd_dev, long rows, int C, void* stream);
+/* dx = rstd (g - mean(g) - xh mean(g xh)) + add, xh = (x - mean) rstd, g = dy weight; dweight = sum over rows of dy xh,
+ * dbias = sum over rows of dy (both [C] f32, both NULL for a frozen norm).  add [rows, C] or NULL: the gradient that
+ * reaches x by the residual branch.  ws_dev: ldm_layer_norm_ws_floats(dtype, rows, C) floats (unused without dweight). */
+long ldm_layer_norm_ws_floats(int dtype, long rows, int C);
+int ldm_layer_norm_backward(int dtype, const void* dy_dev, long dy_stride, const void* x_dev, long x_stride,
+                            const void* add_dev, long add_stride, const float* mean_dev, const float* rstd_dev,
+                            const float* weight_dev, void* dx_dev, long dx_stride, float* dweight_dev, float* dbias_dev,
+                            float* ws_dev, long rows, int C, void* stream);
+/* Rotary positions over `axes` (1..4) axes.  The P = sections_host[0] + ... rotated pairs of a head's D elements are
+ * (j, P + j) or, interleaved, (2j, 2j + 1); elements behind 2P pass through.  Pair j belongs to the axis in whose section
+ * it falls and turns by position[axis] * inv_freq[j] (the angle in f64; `inverse`: by the opposite angle, which is the
+ * backward pass).  q [B, N, Hq, D] and k [B, N, Hk, D] (Hk = 0: none) with the strides
+ *   strides_host[12] = { q batch, token, head, k batch, token, head, oq ..., ok ... },
+ * elements of a head contiguous.  positions: int32 (pos_type 0), int64 (1) or f32 (2) at
+ * b * pos_strides_host[0] + axis * pos_strides_host[1] + token * pos_strides_host[2].  An output may be its input. */
+int ldm_rope(int dtype, const void* q_dev, const void* k_dev, void* oq_dev, void* ok_dev, const long* strides_host, int B,
+             int N, int Hq, int Hk, int D, const void* pos_dev, int pos_type, const long* pos_strides_host,
+             const float* inv_freq_dev, const int* sections_host, int axes, int interleaved, int inverse, void* stream);
+/* out = act(z), z = x W + bias + res:  x [M, K], W [K, N] (w_order 0: W[k, n] at k * ldw + n; 1: at n * ldw + k, a
+ * transposed weight), bias [N] or NULL, res [M, N] or NULL (may be out, same stride), pre [M, N] or NULL: z, for the
+ * backward pass.  act: 0 none, 1 SiLU, 2 ReLU, 3 GELU (erf).  Products accumulate in f32 and are rounded once, at the end.
+ * ws_dev: ldm_linear_ws_floats(...) floats (may be 0). */
+long ldm_linear_ws_floats(int dtype, long M, long K, long N, int w_order);
+int ldm_linear(int dtype, const void* x_dev, long ldx, const void* w_dev, long ldw, int w_order, const float* bias_dev,
+               const void* res_dev, long ldres, int act, void* out_dev, long ldo, void* pre_dev, long ldpre, long M, long K,
+               long N, float* ws_dev, void* stream);
+/* dz = dy act'(pre) (the gradient of res; written to dz_dev [M, N], which only an activation needs: without one dz is dy),
+ * dx = dz W^T [M, K], dw = x^T dz in W's order (lddw its leading stride), dbias = column sums of dz [N] f32.  dx, dw and
+ * dbias may each be NULL.  dz is rounded to the element type before the products (the matrix cores' operand type); dbias
+ * sums it unrounded.  ws_dev: ldm_linear_backward_ws_floats(...) floats. */
+long ldm_linear_backward_ws_floats(int dtype, long M, long K, long N, int w_order);
+int ldm_linear_backward(int dtype, const void* dy_dev, long lddy, const void* x_dev, long ldx, const void* w_dev, long ldw,
+                        int w_order, const void* pre_dev, long ldpre, int act, void* dz_dev, long lddz, void* dx_dev,
+                        long lddx, void* dw_dev, long lddw, float* dbias_dev, float* ws_dev, long M, long K, long N,
+                        void* stream);
+
 /* ---- one scheduler update on flat f32 arrays, src/main.rs:712-756,765 --------------------- */
 /* coef5 = one row of ldm_ddpm_coefficients / ldm_ddim_coefficients.  DDPM: z <- (x0*c1 + z*c2) +
  * sigma*noise, or x0 when `last`; DDIM: z <- x0*c1 + eps*c2; x0 = (z - eps*s1m)/sa.  noise_dev may be

@@ -1,0 +1,642 @@
+"""Operators of transformer blocks on the GPU: layer norm, rotary positions and the linear layer, forward and backward,
+against plain statements in 64 bits.
+
+Tolerances are bounds, element by element: half a step of the output's type on the value itself, plus the f32 error of the
+sums, (number of additions in a row) * 2^-24 * (sum of the magnitudes added)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+E32 = 2.0 ** -24                                       # half a step of f32
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: E32}
+DT = {"bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from diffusionmodel_amd import ops
+    return ops
+
+
+def _rn(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def _within(got, ref, tol, what):
+    got = got.double()
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    if got.numel() == 0:
+        return
+    bad = ~((got - ref).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), float((got - ref).abs().max()),
+                           float(((got - ref).abs() / tol.clamp_min(1e-300)).max()))
+
+
+# ---- layer norm -------------------------------------------------------------------------------------------------------
+LN_SHAPES = [(1, 1), (3, 1), (1, 7), (4, 8), (5, 64), (4, 256), (70, 100), (33, 255), (17, 513), (9, 1031), (6, 2048),
+             (5, 2052), (3, 4099), (3, 9000), (2, 17001), (2, 40000), (9000, 8), (5000, 200), (1, 1024)]
+
+
+def _ln_ref(x, w, b, eps):
+    x = x.double()
+    mu = x.mean(-1, keepdim=True)
+    r = 1.0 / torch.sqrt(((x - mu) ** 2).mean(-1, keepdim=True) + eps)
+    xh = (x - mu) * r
+    y = xh * (1.0 if w is None else w.double()) + (0.0 if b is None else b.double())
+    return y, mu, r, xh
+
+
+def _adds(C):
+    """Additions in a row of one lane's sum over C columns, and of its tree."""
+    return 80 + C // 256
+
+
+def _ln_tol(y, x, mu, r, xh, w, b, eps, dt):
+    C = x.shape[-1]
+    n = _adds(C)
+    aw = 1.0 if w is None else w.double().abs()
+    ab = 0.0 if b is None else b.double().abs()
+    mean_abs = x.double().abs().mean(-1, keepdim=True)
+    # the mean is off by n E32 mean|x|; that shifts x - mu, and the variance by the square of it (rows without variance:
+    # r = eps^-1/2 multiplies what is left)
+    dmu = (n + 2) * E32 * mean_abs
+    shift = dmu * r
+    return HALF[dt] * y.abs() + aw * (shift + xh.abs() * ((n + 8) * E32 + shift * shift)) + 2 * E32 * (ab + y.abs())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,C", LN_SHAPES)
+def test_layer_norm(ops, rows, C, dtype):
+    dt = DT[dtype]
+    x = (_rn(rows + C, rows, C) * (0.5 + _rn(3, C).abs()) + 4.0 * _rn(4, C)).to(dt)
+    w, b = 1.0 + 0.2 * _rn(1, C), 0.3 * _rn(2, C)
+    print("layer_norm", dtype, rows, C, flush=True)
+    for ww, bb, eps in ((w, b, 1e-5), (w, None, 1e-3), (None, b, 1e-5), (None, None, 1e-5)):
+        y, mean, rstd = ops.layer_norm(x, ww, bb, eps=eps, stats=True)
+        ref, mu, r, xh = _ln_ref(x, ww, bb, eps)
+        _within(y, ref, _ln_tol(ref, x, mu, r, xh, ww, bb, eps, dt), "y")
+        n = _adds(C)
+        dmu = (n + 2) * E32 * x.double().abs().mean(-1)
+        _within(mean, mu[:, 0], dmu + 1e-45, "mean")
+        _within(rstd, r[:, 0], r[:, 0] * ((n + 8) * E32 + (dmu * r[:, 0]) ** 2), "rstd")
+        assert torch.equal(y, ops.layer_norm(x, ww, bb, eps=eps))          # the same bits again, and without statistics
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,C", LN_SHAPES)
+def test_layer_norm_backward(ops, rows, C, dtype):
+    dt = DT[dtype]
+    x = (_rn(rows + C, rows, C) * (0.5 + _rn(3, C).abs()) + _rn(4, C)).to(dt)
+    dy, add = _rn(5, rows, C).to(dt), _rn(6, rows, C).to(dt)
+    w = 1.0 + 0.2 * _rn(1, C)
+    _, mean, rstd = ops.layer_norm(x, w, None, stats=True)
+    print("layer_norm_backward", dtype, rows, C, flush=True)
+    xh = (x.double() - mean.double()[:, None]) * rstd.double()[:, None]
+    n = _adds(C)
+    for ww, aa in ((w, add), (w, None), (None, None)):
+        dx, dw, db = ops.layer_norm_backward(dy, x, mean, rstd, ww, add=aa)
+        g = dy.double() * (1.0 if ww is None else ww.double())
+        r = rstd.double()[:, None]
+        ref = r * (g - g.mean(-1, keepdim=True) - xh * (g * xh).mean(-1, keepdim=True))
+        size = r * (g.abs() + g.abs().mean(-1, keepdim=True) + xh.abs() * (g * xh).abs().mean(-1, keepdim=True))
+        if aa is not None:
+            ref = ref + aa.double()
+            size = size + aa.double().abs()
+        _within(dx, ref, HALF[dt] * ref.abs() + (n + 10) * E32 * size, "dx")
+        if ww is None:
+            assert dw is None and db is None
+            continue
+        m = rows // 64 + 128                          # rows of one lane, row groups, partial rows
+        _within(dw, (dy.double() * xh).sum(0), (m + 4) * E32 * (dy.double() * xh).abs().sum(0) + 1e-45, "dw")
+        _within(db, dy.double().sum(0), m * E32 * dy.double().abs().sum(0) + 1e-45, "db")
+        dx2, dw2, db2 = ops.layer_norm_backward(dy, x, mean, rstd, ww, add=aa)
+        assert torch.equal(dx, dx2) and torch.equal(dw, dw2) and torch.equal(db, db2)
+        dx3, dw3, db3 = ops.layer_norm_backward(dy, x, mean, rstd, ww, add=aa, param_grads=False)
+        assert torch.equal(dx, dx3) and dw3 is None and db3 is None
+    # parameter gradients of a norm whose weight is all ones, not given
+    _, dw, db = ops.layer_norm_backward(dy, x, mean, rstd, None, param_grads=True)
+    _within(db, dy.double().sum(0), (rows // 64 + 128) * E32 * dy.double().abs().sum(0) + 1e-45, "db without weight")
+
+
+def test_layer_norm_gradient_against_differences(ops):
+    rows, C = 6, 96
+    x, w, b, c = _rn(1, rows, C), 1.0 + 0.2 * _rn(2, C), 0.1 * _rn(3, C), _rn(4, rows, C)
+    vx, vw, vb = _rn(5, rows, C), _rn(6, C), _rn(7, C)
+    _, mean, rstd = ops.layer_norm(x, w, b, stats=True)
+    dx, dw, db = ops.layer_norm_backward(c, x, mean, rstd, w)
+    h = 2.0 ** -8
+
+    def loss(t):
+        return (ops.layer_norm(x + t * vx, w + t * vw, b + t * vb).double() * c.double()).sum()
+    diff = (loss(h) - loss(-h)) / (2 * h)
+    want = (dx.double() * vx.double()).sum() + (dw.double() * vw.double()).sum() + (db.double() * vb.double()).sum()
+    # rounding: 576 outputs of size up to 4 and c up to 4, each off by some 20 E32, over 2h; the error of central
+    # differences is h^2 / 6 times a third derivative of at most some hundred per row
+    tol = 576 * 4 * 20 * E32 * 4 / (2 * h) + h * h / 6 * 100 * rows
+    assert abs(float(diff - want)) < tol, (float(diff), float(want), tol)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_layer_norm_strides_rows_and_inplace(ops, dtype):
+    dt = DT[dtype]
+    big = _rn(1, 6, 5, 300).to(dt)
+    w, b = 1.0 + 0.2 * _rn(2, 77), 0.3 * _rn(3, 77)
+    x = big[..., 101:178]                              # odd offset, wide rows: one run of rows with a stride of 300
+    want, wm, wr = ops.layer_norm(x.contiguous(), w, b, stats=True)
+    got, gm, gr = ops.layer_norm(x, w, b, stats=True)
+    assert torch.equal(got, want) and gm.shape == (6, 5) and torch.equal(gm, wm) and torch.equal(gr, wr)
+    out = torch.full((6, 5, 90), 7.0, dtype=dt, device="cuda")
+    ops.layer_norm(x, w, b, out=out[..., 3:80])
+    assert torch.equal(out[..., 3:80], want)
+    assert bool((out[..., :3] == 7).all()) and bool((out[..., 80:] == 7).all())
+    same = big.clone()[..., 101:178]
+    assert ops.layer_norm(same, w, b, out=same).data_ptr() == same.data_ptr() and torch.equal(same, want)
+    wide = (_rn(4, 3, 20001) + 1.0).to(dt)
+    ref = ops.layer_norm(wide)
+    assert torch.equal(ops.layer_norm(wide, out=wide), ref)
+    # a gradient that is one row for all, and a transposed one that is refused
+    dy1 = _rn(5, 77).to(dt)
+    dx, dw, db = ops.layer_norm_backward(dy1.expand(6, 5, 77), x, gm, gr, w)
+    dx2, dw2, db2 = ops.layer_norm_backward(dy1.expand(6, 5, 77).contiguous(), x.contiguous(), gm, gr, w)
+    assert torch.equal(dx, dx2) and torch.equal(dw, dw2) and torch.equal(db, db2)
+    # no rows
+    y, m, r = ops.layer_norm(big[:0, :, :77], w, b, stats=True)
+    assert y.shape == (0, 5, 77) and m.shape == r.shape == (0, 5)
+    dx, dw, db = ops.layer_norm_backward(y, y, m, r, w)
+    assert dx.shape == (0, 5, 77) and not dw.any() and not db.any()
+
+
+def test_layer_norm_keeps_bad_rows_to_themselves(ops):
+    x = _rn(1, 8, 200)
+    want = ops.layer_norm(x)
+    y = x.clone()
+    y[2, 5], y[4, 0], y[6, 199] = float("nan"), float("inf"), float("-inf")
+    got = ops.layer_norm(y)
+    for i in range(8):
+        if i in (2, 4, 6):
+            assert bool(torch.isnan(got[i]).all())
+        else:
+            assert torch.equal(got[i], want[i])
+    const = torch.full((3, 200), 5.0, device="cuda")
+    assert not ops.layer_norm(const).any()
+
+
+def test_layer_norm_past_32_bit_offsets(ops):
+    C, rows = 8192, 2 ** 31 // 8192 + 3
+    x = torch.zeros(rows, C, dtype=torch.bfloat16, device="cuda")
+    tail = _rn(1, 5, C).to(torch.bfloat16)
+    x[-5:] = tail
+    y, mean, rstd = ops.layer_norm(x, stats=True)
+    assert torch.equal(y[-5:], ops.layer_norm(tail))
+    dx, dw, db = ops.layer_norm_backward(x, x, mean, rstd, None, add=y, param_grads=True)
+    _, tm, tr = ops.layer_norm(tail, stats=True)
+    assert torch.equal(dx[-5:], ops.layer_norm_backward(tail, tail, tm, tr, None, add=y[-5:].clone())[0])
+    assert bool(torch.isfinite(dw).all())
+
+
+# ---- rotary positions -------------------------------------------------------------------------------------------------
+def _rope_ref(x, pos, inv, sec, layout, sign):
+    """x [B, N, H, D], pos [B or 1, axes, N]; each pair as a complex number."""
+    x = x.double().clone()
+    P = inv.numel()
+    ax = torch.tensor([a for a, n in enumerate(sec) for _ in range(n)], device=x.device)
+    ang = pos.double()[:, ax].transpose(1, 2) * inv.double()                    # [B, N, P]
+    c, s = torch.cos(ang)[:, :, None], sign * torch.sin(ang)[:, :, None]
+    a, b = (x[..., :P], x[..., P:2 * P]) if layout == "half" else (x[..., 0:2 * P:2], x[..., 1:2 * P:2])
+    u, v = a * c - b * s, a * s + b * c
+    size = torch.zeros_like(x)
+    m = a.abs() + b.abs()
+    if layout == "half":
+        x[..., :P], x[..., P:2 * P] = u, v
+        size[..., :P], size[..., P:2 * P] = m, m
+    else:
+        x[..., 0:2 * P:2], x[..., 1:2 * P:2] = u, v
+        size[..., 0:2 * P:2], size[..., 1:2 * P:2] = m, m
+    return x, size
+
+
+def _rope_within(got, ref, size, dt, what):
+    # the fraction of a turn is rounded to f32 (2^-26 of a turn: 1.6 E32 of angle), the sine to 2 steps, three roundings
+    _within(got, ref, HALF[dt] * ref.abs() + 8 * E32 * size, what)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("B,N,Hq,Hk,D,sec", [(1, 1, 1, 0, 2, (1,)), (1, 1, 4, 4, 64, (16, 16)), (2, 7, 3, 1, 10, (2, 3)),
+                                             (3, 33, 8, 2, 72, (12, 12, 12)), (2, 300, 16, 4, 128, (16, 24, 24)),
+                                             (1, 17, 2, 2, 96, (9, 7)), (2, 5, 1, 1, 40, (4, 0, 3, 3)),
+                                             (1, 9, 11, 5, 256, (128,)), (4, 64, 4, 4, 64, (3, 5)), (1, 3, 1, 1, 2048, (1024,)),
+                                             (5, 13, 2, 1, 33, (16,))])
+def test_rope(ops, B, N, Hq, Hk, D, sec, dtype, layout):
+    dt = DT[dtype]
+    qkv = _rn(B * N + D, B, N, Hq + 2 * Hk + 1, D).to(dt)
+    q, k = qkv[:, :, :Hq], (qkv[:, :, Hq:Hq + Hk] if Hk else None)
+    inv = ops.rope_frequencies(sec, shared=(N % 2 == 0), device="cuda")
+    g = torch.Generator().manual_seed(N)
+    print("rope", layout, dtype, B, N, Hq, Hk, D, sec, flush=True)
+    shared = torch.randint(0, 5000, (len(sec), N), generator=g).cuda()
+    per_image = torch.randint(-200000, 2000000, (B, len(sec), N), generator=g).cuda()
+    for pos in (shared.int(), shared, per_image.int(), per_image, shared.float() * 0.37,
+                per_image.int().transpose(1, 2).contiguous().transpose(1, 2)):
+        for inverse in (False, True):
+            got = ops.rope(q, k, pos, inv, sections=sec, layout=layout, inverse=inverse)
+            pos3 = pos if pos.dim() == 3 else pos[None]
+            for t, o, name in ((q, got if k is None else got[0], "q"),) + (() if k is None else ((k, got[1], "k"),)):
+                ref, size = _rope_ref(t, pos3, inv, sec, layout, -1.0 if inverse else 1.0)
+                assert o.dtype == dt and o.is_contiguous()
+                _rope_within(o, ref, size, dt, name)
+                P2 = 2 * sum(sec)
+                assert torch.equal(o[..., P2:], t[..., P2:])
+    # position zero leaves everything as it is
+    got = ops.rope(q, k, torch.zeros_like(shared), inv, sections=sec, layout=layout)
+    assert torch.equal(got if k is None else got[0], q)
+
+
+def test_rope_in_place_strides_and_untouched_neighbours(ops):
+    B, N, H, D, sec = 2, 19, 3, 48, (8, 8, 8)
+    inv = ops.rope_frequencies(sec, device="cuda")
+    pos = torch.randint(0, 64, (3, N), generator=torch.Generator().manual_seed(1)).cuda()
+    for dt in (torch.bfloat16, torch.float32):
+        qkv = _rn(7, B, N, 3 * H, D).to(dt)
+        q, k, v = (qkv[:, :, i * H:(i + 1) * H] for i in range(3))
+        wq, wk = ops.rope(q, k, pos, inv, sections=sec)
+        keep = v.clone()
+        oq, ok = ops.rope(q, k, pos, inv, sections=sec, out=(q, k))            # slices of one buffer, in place
+        assert torch.equal(q, wq) and torch.equal(k, wk) and torch.equal(v, keep) and oq is q and ok is k
+        # heads before tokens, as attention kernels mostly want them
+        qt = wq.transpose(1, 2).contiguous().transpose(1, 2)
+        out = torch.full((B, H, N, D + 3), 5.0, dtype=dt, device="cuda")
+        got = ops.rope(qt, None, pos, inv, sections=sec, inverse=True, out=out[..., 1:D + 1].transpose(1, 2))
+        assert torch.equal(got, ops.rope(wq, None, pos, inv, sections=sec, inverse=True))
+        assert bool((out[..., 0] == 5).all()) and bool((out[..., D + 1:] == 5).all())
+    empty = torch.empty(0, N, H, D, device="cuda")
+    assert ops.rope(empty, empty, pos, inv, sections=sec)[0].shape == empty.shape
+    none = torch.empty(2, 0, H, D, device="cuda")
+    assert ops.rope(none, None, pos[:, :0], inv, sections=sec).shape == none.shape
+
+
+def test_rope_gradient_is_the_transposed_map(ops):
+    """<dq, v> = <c, rope(v)> for any v: the map is linear in q, so this is its gradient, differences included."""
+    sec = (8, 12, 12)
+    inv = ops.rope_frequencies(sec, device="cuda")
+    pos = torch.randint(0, 100, (3, 21), generator=torch.Generator().manual_seed(1)).cuda()
+    for layout in ("half", "interleaved"):
+        c, v = _rn(1, 2, 21, 4, 70), _rn(2, 2, 21, 4, 70)
+        dq = ops.rope(c, None, pos, inv, sections=sec, layout=layout, inverse=True)
+        a = (dq.double() * v.double()).sum()
+        y = ops.rope(v, None, pos, inv, sections=sec, layout=layout)
+        b = (c.double() * y.double()).sum()
+        # every output off by 8 E32 (|a| + |b|) and a rounding
+        tol = 9 * E32 * 4 * float((c.double().abs() * (v.double().abs() + 1.0)).sum())
+        assert abs(float(a - b)) < tol
+        # a difference along v is the map of v
+        h = 0.5
+        d = (ops.rope(c + h * v, None, pos, inv, sections=sec, layout=layout).double()
+             - ops.rope(c - h * v, None, pos, inv, sections=sec, layout=layout).double()) / (2 * h)
+        assert float((d - y.double()).abs().max()) < 9 * E32 * 8 * 12
+
+
+# ---- linear -----------------------------------------------------------------------------------------------------------
+LIN_SHAPES = [(1, 1, 1), (1, 256, 2048), (4, 256, 2048), (2, 17, 33), (5, 8, 8), (16, 100, 64), (31, 64, 128), (64, 33, 7),
+              (130, 70, 66), (257, 129, 255), (300, 1024, 512), (1000, 321, 643), (128, 64, 64), (129, 2048, 1),
+              (1, 4100, 5), (700, 1, 300), (512, 512, 512), (2050, 256, 264)]
+
+
+def _act_ref(z, act):
+    return {None: lambda v: v, "relu": torch.relu, "silu": torch.nn.functional.silu, "gelu": torch.nn.functional.gelu}[act](z)
+
+
+def _dact_ref(z, act):
+    if act == "relu":
+        return (z > 0).double()
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return s + z * s * (1 - s)
+    if act == "gelu":
+        return 0.5 * torch.erfc(-z / math.sqrt(2)) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    return torch.ones_like(z)
+
+
+def _weights(seed, K, N, dt, order):
+    w = (_rn(seed, K, N) * K ** -0.5).to(dt)
+    return w if order == "kn" else w.t().contiguous().t()
+
+
+@pytest.mark.parametrize("order", ["kn", "nk"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("M,K,N", LIN_SHAPES)
+def test_linear(ops, M, K, N, dtype, order):
+    dt = DT[dtype]
+    x, w = _rn(M + K, M, K).to(dt), _weights(N, K, N, dt, order)
+    b, res = 0.5 * _rn(1, N), _rn(2, M, N).to(dt)
+    print("linear", dtype, order, M, K, N, flush=True)
+    z0 = x.double() @ w.double()
+    size = x.double().abs() @ w.double().abs()
+    for bias, r, act, save in ((None, None, None, False), (b, None, "gelu", True), (b, res, "silu", True),
+                               (None, res, "relu", False), (b, res, None, True)):
+        got = ops.linear(x, w, bias, act=act, res=r, save_pre=save)
+        out, pre = got if save else (got, None)
+        z = z0 + (0 if bias is None else bias.double()) + (0 if r is None else r.double())
+        sz = size + (0 if bias is None else bias.double().abs()) + (0 if r is None else r.double().abs())
+        tz = (K + 8) * E32 * sz
+        if save:
+            _within(pre, z, HALF[dt] * z.abs() + tz, "pre")
+        ref = _act_ref(z, act)
+        # |act'| <= 1.13; exp and erf to a few steps of f32, erf's against 1 + erf
+        _within(out, ref, HALF[dt] * ref.abs() + 1.13 * tz + 8 * E32 * z.abs(), ("out", act))
+        again = ops.linear(x, w, bias, act=act, res=r, save_pre=save)
+        assert torch.equal(out, again[0] if save else again)
+
+
+@pytest.mark.parametrize("order", ["kn", "nk"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("M,K,N", LIN_SHAPES)
+def test_linear_backward(ops, M, K, N, dtype, order):
+    dt = DT[dtype]
+    x, w = _rn(M + K, M, K).to(dt), _weights(N, K, N, dt, order)
+    dy, pre = _rn(5, M, N).to(dt), _rn(6, M, N).to(dt)
+    print("linear_backward", dtype, order, M, K, N, flush=True)
+    for act in (None, "silu", "relu", "gelu"):
+        dx, dw, db, dz = ops.linear_backward(dy, x, w, pre=pre if act else None, act=act)
+        rz = dy.double() * _dact_ref(pre.double(), act)
+        ez = 16 * E32 * dy.double().abs() * (1 + pre.double().abs()) if act else torch.zeros_like(rz)   # act' in f32
+        if act is None:
+            assert dz is dy
+        else:
+            _within(dz, rz, HALF[dt] * rz.abs() + ez, ("dz", act))
+        rdz = (HALF[dt] * rz.abs() + ez) if act else ez
+        ref = rz @ w.double().t()
+        aw, ax = w.double().abs(), x.double().abs()
+        _within(dx, ref, HALF[dt] * ref.abs() + rdz @ aw.t() + (N + 8) * E32 * (rz.abs() @ aw.t()), ("dx", act))
+        ref = x.double().t() @ rz
+        _within(dw, ref, HALF[dt] * ref.abs() + ax.t() @ rdz + (M + 8) * E32 * (ax.t() @ rz.abs()) + 1e-45, ("dw", act))
+        assert dw.stride() == w.stride() or min(K, N) == 1
+        _within(db, rz.sum(0), ez.sum(0) + (M + 8) * E32 * rz.abs().sum(0) + 1e-45, ("db", act))
+        again = ops.linear_backward(dy, x, w, pre=pre if act else None, act=act)
+        assert all(torch.equal(a, b) for a, b in zip((dx, dw, db, dz), again))
+        part = ops.linear_backward(dy, x, w, pre=pre if act else None, act=act, dx=False, dbias=False)
+        assert part[0] is None and part[2] is None and torch.equal(part[1], dw)
+
+
+def test_linear_gradient_against_differences(ops):
+    M, K, N = 12, 40, 56
+    x, w, b, r, c = _rn(1, M, K), _rn(2, K, N) * K ** -0.5, _rn(3, N), _rn(4, M, N), _rn(5, M, N)
+    vx, vw, vb, vr = _rn(6, M, K), _rn(7, K, N) * K ** -0.5, _rn(8, N), _rn(9, M, N)
+    for act in (None, "silu", "gelu"):
+        _, pre = ops.linear(x, w, b, act=act, res=r, save_pre=True)
+        dx, dw, db, dz = ops.linear_backward(c, x, w, pre=pre, act=act)
+        h = 2.0 ** -7
+
+        def loss(t):
+            return (ops.linear(x + t * vx, w + t * vw, b + t * vb, act=act, res=r + t * vr).double() * c.double()).sum()
+        diff = float((loss(h) - loss(-h)) / (2 * h))
+        want = float(sum((p.double() * q.double()).sum() for p, q in ((dx, vx), (dw, vw), (db, vb), (dz, vr))))
+        # rounding: M N = 672 outputs of size up to 8, (K + 8) E32 each, weighted by c up to 4; central differences:
+        # h^2 / 6 times the third derivative along v, |act'''| < 2 and |dz/dt| < 10, plus the product term's
+        tol = 672 * 8 * 48 * E32 * 4 / (2 * h) + h * h / 6 * 672 * 2 * 60
+        assert abs(diff - want) < tol, (act, diff, want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_linear_strides_in_place_and_rows(ops, dtype):
+    dt = DT[dtype]
+    for K, N in ((96, 80), (45, 77)):
+        big = _rn(1, 3, 7, 2 * K + 5).to(dt)
+        x = big[..., 3:3 + K]
+        wbig = (_rn(2, K, N + 9) * K ** -0.5).to(dt)
+        w = wbig[:, 5:5 + N]
+        b, res = _rn(3, N), _rn(4, 3, 7, N).to(dt)
+        want = ops.linear(x.contiguous(), w.contiguous(), b, act="silu", res=res)
+        assert torch.equal(ops.linear(x, w, b, act="silu", res=res), want) and want.shape == (3, 7, N)
+        out = torch.full((3, 7, N + 6), 9.0, dtype=dt, device="cuda")
+        ops.linear(x, w, b, act="silu", res=res, out=out[..., 1:N + 1])
+        assert torch.equal(out[..., 1:N + 1], want)
+        assert bool((out[..., 0] == 9).all()) and bool((out[..., N + 1:] == 9).all())
+        stream = res.clone()
+        ops.linear(x, w, b, act="silu", res=stream, out=stream)              # the residual stream, updated in place
+        assert torch.equal(stream, want)
+        one = big[:1, :1, 3:3 + K].expand(3, 7, K)                           # one row for all
+        assert torch.equal(ops.linear(one, w, b), ops.linear(one.contiguous(), w, b))
+        dy = _rn(5, 3, 7, 2 * N).to(dt)[..., N:]
+        g1 = ops.linear_backward(dy, x, w)
+        g2 = ops.linear_backward(dy.contiguous(), x.contiguous(), w.contiguous())
+        assert all(torch.equal(p, q) for p, q in zip(g1[:3], g2[:3]))
+    x0 = torch.empty(0, 64, dtype=dt, device="cuda")
+    w = _weights(1, 64, 32, dt, "kn")
+    assert ops.linear(x0, w).shape == (0, 32)
+    dx, dw, db, _ = ops.linear_backward(torch.empty(0, 32, dtype=dt, device="cuda"), x0, w)
+    assert dx.shape == (0, 64) and not dw.any() and not db.any()
+
+
+def test_linear_keeps_bad_rows_to_themselves(ops):
+    for dt in (torch.bfloat16, torch.float32):
+        for M, K, N in ((300, 128, 256), (9, 70, 33)):
+            x, w = _rn(1, M, K).to(dt), _weights(2, K, N, dt, "kn")
+            want = ops.linear(x, w, act="relu")
+            y = x.clone()
+            y[5, K - 1] = float("nan")
+            y[7] = float("inf")
+            got = ops.linear(y, w, act="relu")
+            keep = [i for i in range(M) if i not in (5, 7)]
+            assert torch.equal(got[keep], want[keep]) and bool(torch.isnan(got[5]).all())
+
+
+# ---- streams, graphs, the operators together --------------------------------------------------------------------------
+def _block_args(dt, B=2, N=30, H=4, D=24, seed=0):
+    C = H * D
+    g = lambda i, *s: _rn(seed + i, *s)                 # noqa: E731
+    p = {"w1": 1 + 0.1 * g(1, C), "b1": 0.1 * g(2, C), "wqkv": (g(3, C, 3 * C) * C ** -0.5).to(dt), "bqkv": 0.1 * g(4, 3 * C),
+         "wo": (g(5, C, C) * C ** -0.5).to(dt), "bo": 0.1 * g(6, C), "w2": 1 + 0.1 * g(7, C), "b2": 0.1 * g(8, C),
+         "wu": (g(9, C, 4 * C) * C ** -0.5).to(dt), "bu": 0.1 * g(10, 4 * C), "wd": (g(11, 4 * C, C) * (4 * C) ** -0.5).to(dt),
+         "bd": 0.1 * g(12, C)}
+    return g(20, B, N, C).to(dt), p, H, D
+
+
+def _attend(q, k, v):
+    """softmax(q k^T / sqrt(D)) v on [B, N, H, D] by elementary operations."""
+    s = (q[:, :, None] * k[:, None]).sum(-1) * q.shape[-1] ** -0.5            # [B, N, M, H]
+    p = torch.softmax(s, 2)
+    return (p[..., None] * v[:, None]).sum(2)
+
+
+def _block(ops, x, p, H, D, pos, inv, sec):
+    """One pre-norm transformer block through the operators; returns the output and what the backward pass needs."""
+    B, N, C = x.shape
+    s = {"x": x}
+    s["n1"], s["m1"], s["r1"] = ops.layer_norm(x, p["w1"], p["b1"], stats=True)
+    qkv = ops.linear(s["n1"], p["wqkv"], p["bqkv"]).view(B, N, 3, H, D)
+    s["q"], s["k"] = ops.rope(qkv[:, :, 0], qkv[:, :, 1], pos, inv, sections=sec, out=(qkv[:, :, 0], qkv[:, :, 1]))
+    s["v"] = qkv[:, :, 2]
+    s["a"] = _attend(s["q"].float(), s["k"].float(), s["v"].float()).reshape(B, N, C).to(x.dtype)
+    s["h"] = ops.linear(s["a"], p["wo"], p["bo"], res=x)
+    s["n2"], s["m2"], s["r2"] = ops.layer_norm(s["h"], p["w2"], p["b2"], stats=True)
+    s["u"], s["pre"] = ops.linear(s["n2"], p["wu"], p["bu"], act="gelu", save_pre=True)
+    return ops.linear(s["u"], p["wd"], p["bd"], res=s["h"]), s
+
+
+def _block_ref(x, p, H, D, pos, inv, sec):
+    B, N, C = x.shape
+    ln = torch.nn.functional.layer_norm
+    n1 = ln(x, (C,), p["w1"], p["b1"])
+    qkv = (n1 @ p["wqkv"] + p["bqkv"]).view(B, N, 3, H, D)
+    ax = torch.tensor([a for a, n in enumerate(sec) for _ in range(n)], device=x.device)
+    ang = (pos.double()[ax].t() * inv.double())[None, :, None]
+    P = inv.numel()
+
+    def turn(t):
+        a, b = t[..., :P], t[..., P:2 * P]
+        return torch.cat([a * ang.cos() - b * ang.sin(), a * ang.sin() + b * ang.cos(), t[..., 2 * P:]], -1)
+    a = _attend(turn(qkv[:, :, 0]), turn(qkv[:, :, 1]), qkv[:, :, 2]).reshape(B, N, C)
+    h = x + a @ p["wo"] + p["bo"]
+    u = torch.nn.functional.gelu(ln(h, (C,), p["w2"], p["b2"]) @ p["wu"] + p["bu"])
+    return h + u @ p["wd"] + p["bd"]
+
+
+def test_a_transformer_block_forward_and_backward(ops):
+    x, p, H, D = _block_args(torch.float32)
+    B, N, C = x.shape
+    sec = (4, 4, 4)
+    inv = ops.rope_frequencies(sec, device="cuda")
+    t = torch.arange(N, device="cuda")
+    pos = torch.stack([t // 10, t // 5 % 2, t % 5]).int()
+    out, s = _block(ops, x, p, H, D, pos, inv, sec)
+    ref_in = {k: v.double().requires_grad_() for k, v in p.items()}
+    xr = x.double().requires_grad_()
+    ref = _block_ref(xr, ref_in, H, D, pos, inv, sec)
+    dy = _rn(99, B, N, C)
+    ref.backward(dy.double())
+    g = {}
+    du, g["wd"], g["bd"], dh = ops.linear_backward(dy, s["u"], p["wd"])
+    dn2, g["wu"], g["bu"], _ = ops.linear_backward(du, s["n2"], p["wu"], pre=s["pre"], act="gelu")
+    dh, g["w2"], g["b2"] = ops.layer_norm_backward(dn2, s["h"], s["m2"], s["r2"], p["w2"], add=dh)
+    da, g["wo"], g["bo"], _ = ops.linear_backward(dh, s["a"], p["wo"])
+    q, k, v = (s[i].detach().clone().requires_grad_() for i in "qkv")
+    _attend(q, k, v).backward(da.view(B, N, H, D))
+    dqkv = torch.stack([q.grad, k.grad, v.grad], 2)
+    ops.rope(dqkv[:, :, 0], dqkv[:, :, 1], pos, inv, sections=sec, inverse=True, out=(dqkv[:, :, 0], dqkv[:, :, 1]))
+    dn1, g["wqkv"], g["bqkv"], _ = ops.linear_backward(dqkv.view(B, N, 3 * C), s["n1"], p["wqkv"])
+    dx, g["w1"], g["b1"] = ops.layer_norm_backward(dn1, x, s["m1"], s["r1"], p["w1"], add=dh)
+    # some twenty operators of f32 in a row, each off by at most (384 + 8) E32 = 2.3e-5 of its magnitudes, in norm by
+    # about its root: 20 * sqrt(392) * E32 = 2.4e-5
+    rel = lambda a, b: float((a.double() - b).norm() / b.norm())              # noqa: E731
+    assert rel(out, ref.detach()) < 2.4e-5
+    assert rel(dx, xr.grad) < 2.4e-5
+    for name in p:
+        assert rel(g[name], ref_in[name].grad) < 4.8e-5, name
+
+
+def test_captured_block_replays_and_shares_no_workspace(ops):
+    """Two captured graphs of the same operators, replayed in turn on two streams with eager work between: every replay
+    gives the eager bits for the inputs it finds."""
+    sec = (6, 6)
+    inv = ops.rope_frequencies(sec, device="cuda")
+    x0, p, H, D = _block_args(torch.bfloat16, seed=5)
+    N = x0.shape[1]
+    t = torch.arange(N, device="cuda")
+    pos = torch.stack([t // 6, t % 6]).int()
+
+    def step(x, dy):
+        n1, m, r = ops.layer_norm(x, p["w1"], p["b1"], stats=True)
+        u, pre = ops.linear(n1, p["wu"], p["bu"], act="gelu", save_pre=True)
+        q = ops.rope(u.view(*u.shape[:2], 4 * H, D), None, pos, inv, sections=sec)
+        dn, dw, db, _ = ops.linear_backward(ops.rope(q, None, pos, inv, sections=sec, inverse=True).flatten(2), n1, p["wu"],
+                                            pre=pre, act="gelu")
+        return (q, dw, db) + ops.layer_norm_backward(dn, x, m, r, p["w1"], add=dy)
+    ins = [(x0 * (i + 1), _rn(50 + i, *x0.shape).to(x0.dtype)) for i in range(2)]
+    step(*ins[0])
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x, dy in ins:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(step(x, dy))
+        graphs.append(gr)
+    streams = [torch.cuda.Stream() for _ in ins]
+    for rep in range(3):
+        for i, (x, dy) in enumerate(ins):
+            x.copy_(x0 * (i + 1 + rep))
+            dy.copy_(_rn(60 + 10 * rep + i, *x0.shape))
+        torch.cuda.synchronize()
+        for st, gr in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        for i, (x, dy) in enumerate(ins):
+            want = step(x, dy)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], want)), (rep, i)
+
+
+def test_operators_follow_the_current_stream(ops):
+    """Two streams at once, each with its own inputs and outputs."""
+    sec = (32,)
+    inv = ops.rope_frequencies(sec, device="cuda")
+    pos = torch.arange(256, device="cuda").int()[None]
+    w = _weights(1, 256, 512, torch.bfloat16, "kn")
+    xs = [_rn(i, 4096, 256).to(torch.bfloat16) for i in range(2)]
+
+    def work(x):
+        y, m, r = ops.layer_norm(x, stats=True)
+        z, pre = ops.linear(y, w, act="silu", save_pre=True)
+        q = ops.rope(z.view(16, 256, 8, 64), None, pos, inv)
+        return (q,) + ops.linear_backward(z, y, w, pre=pre, act="silu")[:3] + ops.layer_norm_backward(y, x, m, r, None)[:1]
+    want = [work(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [None, None]
+    for _ in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = work(xs[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want[i]))
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------------
+def test_refusals(ops):
+    x, w = _rn(1, 6, 32), _rn(2, 32, 16)
+    _, m, r = ops.layer_norm(x, stats=True)
+    q = _rn(3, 2, 5, 4, 16)
+    inv = ops.rope_frequencies((4, 4), device="cuda")
+    pos = torch.zeros(2, 5, dtype=torch.int32, device="cuda")
+    bad = [
+        lambda: ops.layer_norm(x.half()), lambda: ops.layer_norm(x.cpu()), lambda: ops.layer_norm(x, w[0]),
+        lambda: ops.layer_norm(x.t()), lambda: ops.layer_norm(x, eps=-1.0), lambda: ops.layer_norm(x, eps=float("nan")),
+        lambda: ops.layer_norm(x[:, :0]), lambda: ops.layer_norm(x, x[0].cpu()),
+        lambda: ops.layer_norm(_rn(1, 4, 6, 8)[:, :3]), lambda: ops.layer_norm(x, out=x[:5]),
+        lambda: ops.layer_norm(x[:4], out=x[1:5]), lambda: ops.layer_norm(x, out=x.bfloat16()),
+        lambda: ops.layer_norm(x, out=x[:1].expand(6, 32)), lambda: ops.layer_norm(x.clone().requires_grad_()),
+        lambda: ops.layer_norm(x, out=torch.empty(32, 6, device="cuda").t()),
+        lambda: ops.layer_norm_backward(x[:5], x, m, r), lambda: ops.layer_norm_backward(x, x, m[:5], r),
+        lambda: ops.layer_norm_backward(x, x, m.double(), r), lambda: ops.layer_norm_backward(x, x, m, r, add=x.bfloat16()),
+        lambda: ops.layer_norm_backward(x.t().contiguous().t(), x, m, r),
+        lambda: ops.rope(q, None, pos, inv), lambda: ops.rope(q, None, pos, inv, sections=(4, 3)),
+        lambda: ops.rope(q, None, pos, inv, sections=(5, 4)), lambda: ops.rope(q, None, pos, inv, sections=(9, -1)),
+        lambda: ops.rope(q, None, pos[:, :4], inv, sections=(4, 4)), lambda: ops.rope(q[0], None, pos, inv, sections=(4, 4)),
+        lambda: ops.rope(q, q[:, :4], pos, inv, sections=(4, 4)), lambda: ops.rope(q, q.bfloat16(), pos, inv, sections=(4, 4)),
+        lambda: ops.rope(q, None, pos.double(), inv, sections=(4, 4)), lambda: ops.rope(q, None, pos, inv.double(), sections=(4, 4)),
+        lambda: ops.rope(q, None, pos, inv, sections=(4, 4), layout="pairs"),
+        lambda: ops.rope(q.transpose(2, 3), None, pos, inv, sections=(1, 1)),
+        lambda: ops.rope(q, q[:, :, :2], pos, inv, sections=(4, 4), out=(q[:, :, 1:3].repeat(1, 1, 2, 1), q[:, :, 1:3])),
+        lambda: ops.rope(q, None, pos[None].expand(3, 2, 5), inv, sections=(4, 4)),
+        lambda: ops.rope(q[..., :6], None, pos, inv, sections=(4, 4)),
+        lambda: ops.linear(x, w[:31]), lambda: ops.linear(x, w.bfloat16()), lambda: ops.linear(x, w, _rn(1, 15)),
+        lambda: ops.linear(x, w, act="tanh"), lambda: ops.linear(x, w, res=x), lambda: ops.linear(x, w[:, ::2]),
+        lambda: ops.linear(x, _rn(1, 32, 32), out=x), lambda: ops.linear(x, _rn(1, 32, 32), res=x, out=x),
+        lambda: ops.linear(x.double(), w.double()), lambda: ops.linear(x, w.clone().requires_grad_()),
+        lambda: ops.linear(x.t(), w), lambda: ops.linear(x, w[None]),
+        lambda: ops.linear_backward(x, x, w), lambda: ops.linear_backward(_rn(1, 6, 16), x, w, act="silu"),
+        lambda: ops.linear_backward(_rn(1, 6, 16).bfloat16(), x, w),
+        lambda: ops.linear_backward(_rn(1, 6, 16), x, w, pre=_rn(1, 5, 16), act="silu"),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            print("not refused:", i, flush=True)
+    with torch.no_grad():
+        ops.layer_norm(x.clone().requires_grad_())                            # nothing is recorded, nothing is lost
+    torch.cuda.synchronize()
