@@ -44,8 +44,11 @@ struct GemmArgs {
     long lda, ldb, ldr, ldp, ldc;
     long M, N, K;
     int act;
+    float* part;                   // set by launch_gemm: partial sums [parts][M][N rounded up to 8] of a split contraction
+    int kper;                      // set by launch_gemm: steps of the contraction per part
 };
-int launch_gemm(int dtype, const GemmArgs& a, bool akc, bool bkc, hipStream_t s);
+long gemm_ws_floats(int dtype, long M, long N, long K);
+int launch_gemm(int dtype, const GemmArgs& a, bool akc, bool bkc, float* ws, hipStream_t s);
 // dz = dy act'(pre) (not written without an activation: dz is dy) and db = column sums of dz (db null: not taken)
 long linear_dz_ws_floats(long M, long N);
 int launch_linear_dz(int dtype, const void* dy, long lddy, const void* pre, long ldp, void* dz, long lddz, float* db, float* ws,

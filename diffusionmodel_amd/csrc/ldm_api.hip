@@ -1522,7 +1522,7 @@ static int check_linear(int dtype, long M, long K, long N, int w_order, int act)
 }
 long ldm_linear_ws_floats(int dtype, long M, long K, long N, int w_order) {
     if (check_linear(dtype, M, K, N, w_order, 0) != LDM_OK) return -1;
-    return 0;
+    return gemm_ws_floats(dtype, M, N, K);
 }
 int ldm_linear(int dtype, const void* x, long ldx, const void* w, long ldw, int w_order, const float* bias, const void* res,
                long ldres, int act, void* out, long ldo, void* pre, long ldpre, long M, long K, long N, float* ws,
@@ -1537,11 +1537,16 @@ int ldm_linear(int dtype, const void* x, long ldx, const void* w, long ldw, int 
     a.bias = bias; a.res = res; a.ldr = ldres;
     a.pre = pre; a.ldp = ldpre; a.C = out; a.ldc = ldo;
     a.M = M; a.N = N; a.K = K; a.act = act;
-    return launch_gemm(dtype, a, true, w_order == 1, (hipStream_t)stream);
+    return launch_gemm(dtype, a, true, w_order == 1, ws, (hipStream_t)stream);
 }
 long ldm_linear_backward_ws_floats(int dtype, long M, long K, long N, int w_order) {
     if (check_linear(dtype, M, K, N, w_order, 0) != LDM_OK) return -1;
-    return linear_dz_ws_floats(M, N);
+    // one after the other: the column sums of dz, dx, dw
+    long n = linear_dz_ws_floats(M, N);
+    const long nx = gemm_ws_floats(dtype, M, K, N);
+    const long nw = w_order == 0 ? gemm_ws_floats(dtype, K, N, M) : gemm_ws_floats(dtype, N, K, M);
+    n = nx > n ? nx : n;
+    return nw > n ? nw : n;
 }
 int ldm_linear_backward(int dtype, const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, int w_order,
                         const void* pre, long ldpre, int act, void* dz, long lddz, void* dx, long lddx, void* dw, long lddw,
@@ -1561,14 +1566,14 @@ int ldm_linear_backward(int dtype, const void* dy, long lddy, const void* x, lon
         GemmArgs a = {};
         a.A = dz; a.lda = lddz; a.B = w; a.ldb = ldw; a.C = dx; a.ldc = lddx;
         a.M = M; a.N = K; a.K = N;
-        LDM_TRY(launch_gemm(dtype, a, true, w_order == 0, st));
+        LDM_TRY(launch_gemm(dtype, a, true, w_order == 0, ws, st));
     }
     if (dw) {
         GemmArgs a = {};
         a.C = dw; a.ldc = lddw; a.K = M;
         if (w_order == 0) { a.A = x; a.lda = ldx; a.M = K; a.B = dz; a.ldb = lddz; a.N = N; }
         else { a.A = dz; a.lda = lddz; a.M = N; a.B = x; a.ldb = ldx; a.N = K; }
-        LDM_TRY(launch_gemm(dtype, a, false, false, st));
+        LDM_TRY(launch_gemm(dtype, a, false, false, ws, st));
     }
     return LDM_OK;
 }

@@ -3,105 +3,423 @@
 // All three products are C[m, n] = sum_k A(m, k) B(k, n) on one kernel family; an operand is either contiguous along the
 // contraction (KC) or along its other index.
 #include "blocks.h"
+#include <type_traits>
 
 namespace ldm {
 
 namespace {
 
-typedef u32x4 u32x4_u2 __attribute__((aligned(2)));
-typedef u32x4 u32x4_u4 __attribute__((aligned(4)));
-
+// exp and the reciprocal by the hardware's instructions (one step of f32 each)
+__device__ __forceinline__ float lin_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and e = exp(-z^2 / 2): Abramowitz and Stegun 7.1.26, erfc(x) = poly(t) exp(-x^2) with
+// t = 1 / (1 + 0.3275911 x), off by at most 1.5e-7; the negative side takes erfc itself, without 1 - ...  A tile's epilogue
+// has few cycles for this: 12 instructions, where the library's erff would cost as much as a tile of 256 products.
+__device__ __forceinline__ float lin_phi(float z, float& e) {
+    const float x = __builtin_fabsf(z) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
+    float p = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
+    p = __builtin_fmaf(t, p, 1.421413741f);
+    p = __builtin_fmaf(t, p, -0.284496736f);
+    p = __builtin_fmaf(t, p, 0.254829592f);
+    e = lin_exp(-x * x);
+    const float tail = 0.5f * t * p * e;
+    return z >= 0.f ? 1.0f - tail : tail;
+}
 __device__ __forceinline__ float lin_act(float v, int act) {
-    if (act == LIN_SILU) return v / (1.0f + expf(-v));
+    if (act == LIN_SILU) return v * __builtin_amdgcn_rcpf(1.0f + lin_exp(-v));
     if (act == LIN_RELU) return v < 0.f ? 0.f : v;
-    if (act == LIN_GELU) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+    if (act == LIN_GELU) {
+        float e;
+        return v * lin_phi(v, e);
+    }
     return v;
 }
 __device__ __forceinline__ float lin_dact(float z, int act) {
     if (act == LIN_SILU) {
-        const float s = 1.0f / (1.0f + expf(-z));
+        const float s = __builtin_amdgcn_rcpf(1.0f + lin_exp(-z));
         return s * (1.0f + z * (1.0f - s));
     }
     if (act == LIN_RELU) return z > 0.f ? 1.f : 0.f;
-    if (act == LIN_GELU)
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+    if (act == LIN_GELU) {
+        float e;
+        const float phi = lin_phi(z, e);
+        return __builtin_fmaf(z * 0.39894228040143268f, e, phi);
+    }
     return 1.f;
 }
 
-template <typename T> __device__ __forceinline__ T lin_zero() { return (T)0.f; }
+// ---- the matrix kernel ---------------------------------------------------------------------------------------------
+// A workgroup of four waves (2 x 2) computes a tile of TILE x TILE outputs (TILE = 32 F), each wave F x F fragments of
+// 16 x 16.  A step of the contraction is 128 bytes of it (64 bf16, 32 f32); two steps are staged in LDS, one being read
+// while the other arrives.  Both operands keep their memory order in LDS: KC operands as rows of 128 bytes, read by
+// ds_read_b128; the others as rows along their contiguous index, read by transposing loads (bf16) or single words (f32).
+// 16-byte pieces are XOR-swizzled so that each group of lanes that the LDS serves at once touches every bank once.
+//
+// The products are taken transposed (first operand = B's columns, second = A's rows), so that a lane's four accumulators
+// of a fragment are four consecutive columns of one row.
+//
+// Per step a wave first multiplies the fragments of the step's first half while it reads those of the second, then waits
+// for the next step's data, meets the other waves, and multiplies the second half while it reads the next step's first
+// fragments and asks for the step after it.  One barrier per step; nothing in front of a product is read later than one
+// half step before it.
+// Fragment reads that the compiler does not wait for: GemmFrag::landed() behind an explicit wait makes the values usable.
+template <typename T, bool KC> struct GemmFrag;
+template <typename T> struct GemmFrag<T, true> {
+    u32x4 v;
+    template <int OFF> __device__ __forceinline__ void read(unsigned a) {
+        asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(a), "n"(OFF));
+    }
+    __device__ __forceinline__ void landed() { asm volatile("" : "+v"(v)); }
+    __device__ __forceinline__ u32x4 bits() const { return v; }
+    __device__ __forceinline__ float f32(int q) const { return __builtin_bit_cast(f32x4, v)[q]; }
+};
+template <> struct GemmFrag<__bf16, false> {
+    uint2 lo, hi;
+    template <int OFF, int NEXT> __device__ __forceinline__ void read(unsigned a) {
+        asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(lo) : "v"(a), "n"(OFF));
+        asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(hi) : "v"(a), "n"(OFF + NEXT));
+    }
+    __device__ __forceinline__ void landed() { asm volatile("" : "+v"(lo), "+v"(hi)); }
+    __device__ __forceinline__ u32x4 bits() const { return u32x4{lo.x, lo.y, hi.x, hi.y}; }
+};
+template <> struct GemmFrag<float, false> {
+    float q0, q1, q2, q3;
+    template <int OFF, int NEXT> __device__ __forceinline__ void read(unsigned a) {
+        asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(q0) : "v"(a), "n"(OFF));
+        asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(q1) : "v"(a), "n"(OFF + NEXT));
+        asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(q2) : "v"(a), "n"(OFF + 2 * NEXT));
+        asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(q3) : "v"(a), "n"(OFF + 3 * NEXT));
+    }
+    __device__ __forceinline__ void landed() { asm volatile("" : "+v"(q0), "+v"(q1), "+v"(q2), "+v"(q3)); }
+    __device__ __forceinline__ float f32(int q) const { return q == 0 ? q0 : q == 1 ? q1 : q == 2 ? q2 : q3; }
+};
 
-// 64 x 64 outputs per workgroup, 64 bytes of the contraction per step, staged through registers with every access
-// guarded: serves every size, stride and alignment.
-constexpr int GT = 64, GROW = 64 + 16;      // bytes of an LDS row: 64 of data, padded against bank conflicts
-template <typename T, bool AKC, bool BKC>
-__global__ __launch_bounds__(256) void gemm_any_kernel(GemmArgs a) {
-    constexpr int ES = sizeof(T), KB = 64 / ES;
-    __shared__ __attribute__((aligned(16))) char As[GT * GROW];
-    __shared__ __attribute__((aligned(16))) char Bs[GT * GROW];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int g = lane >> 4, l15 = lane & 15;
-    const unsigned nt = (unsigned)((a.N + GT - 1) / GT);
-    const long m0 = (long)(blockIdx.x / nt) * GT, n0 = (long)(blockIdx.x % nt) * GT;
-    const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-    f32x4 acc[2][2] = {};      // [n][m]
-    for (long k0 = 0; k0 < a.K; k0 += KB) {
-        __syncthreads();
-        for (int i = tid; i < GT * KB; i += 256) {
-            int r, k;
-            if (AKC) { r = i / KB; k = i % KB; } else { k = i / GT; r = i % GT; }
-            T v = lin_zero<T>();
-            if (m0 + r < a.M && k0 + k < a.K)
-                v = ((const T*)a.A)[AKC ? (m0 + r) * a.lda + k0 + k : (k0 + k) * a.lda + m0 + r];
-            *(T*)(As + r * GROW + k * ES) = v;
+// One operand's tile: where its pieces lie in memory and LDS.
+//   KC:   LDS row r (of TILE) holds 128 bytes of the contraction, piece p at slot p ^ ((r >> 1) & 7)
+//   else: LDS row k (of BK) holds TILE elements; bf16: 32-byte chunk c at c ^ ((k & 3) + 4 ((k >> 3) & 1)),
+//         f32: 64-byte chunk c at c ^ ((k >> 2) & 3)
+template <typename T, bool KC, int F> struct GemmOperand {
+    static constexpr int ES = sizeof(T), TILE = 32 * F, BK = 128 / ES, BYTES = TILE * 128;
+    static constexpr int RB = KC ? 128 : TILE * ES;          // bytes of an LDS row
+    static constexpr int NP = BYTES / 4096;                  // pieces per lane and step
+
+    // fragment f (16 rows / columns from w0 + 16 f) of half step s: the address without the parts that are immediate
+    static __device__ __forceinline__ unsigned base(int lane, int w0, int s) {
+        const int l15 = lane & 15, g = lane >> 4;
+        if constexpr (KC) {
+            return (w0 + l15) * 128 + (((s * 4 + g) ^ (l15 >> 1)) << 4);
+        } else if constexpr (ES == 2) {
+            const int row = g * 8 + (l15 >> 2), f = (l15 >> 2) | ((g & 1) << 2);
+            return row * RB + (((w0 >> 4) ^ f) << 5) + (l15 & 3) * 8;
+        } else {
+            return (g * 4) * RB + (((w0 >> 4) ^ g) << 6) + l15 * 4;
         }
-        for (int i = tid; i < GT * KB; i += 256) {
-            int r, k;
-            if (BKC) { r = i / KB; k = i % KB; } else { k = i / GT; r = i % GT; }
-            T v = lin_zero<T>();
-            if (n0 + r < a.N && k0 + k < a.K)
-                v = ((const T*)a.B)[BKC ? (n0 + r) * a.ldb + k0 + k : (k0 + k) * a.ldb + n0 + r];
-            *(T*)(Bs + r * GROW + k * ES) = v;
+    }
+    template <int f, int s> static __device__ __forceinline__ void read(GemmFrag<T, KC>& fr, unsigned b) {
+        if constexpr (KC) fr.template read<f * 2048>(b);
+        else if constexpr (ES == 2) fr.template read<s * 32 * RB, 4 * RB>(b ^ (f << 5));
+        else fr.template read<s * 16 * RB, RB>(b ^ (f << 6));
+    }
+    // the piece of memory that goes to 16-byte slot `slot` of the tile: row of the tile and element within the row
+    static __device__ __forceinline__ void piece(int slot, int& row, int& el) {
+        row = slot / (RB / 16);
+        const int p = slot % (RB / 16);
+        int q;
+        if constexpr (KC) q = p ^ ((row >> 1) & 7);
+        else if constexpr (ES == 2) q = p ^ (((row & 3) | (((row >> 3) & 1) << 2)) << 1);
+        else q = p ^ (((row >> 2) & 3) << 2);
+        el = q * (16 / ES);
+    }
+};
+
+// the first n of 16 / sizeof(T) elements at p (element aligned), zeros for the rest; n may be zero or less, or more than all
+typedef u32x4 gemm_u16_a2 __attribute__((aligned(2)));
+typedef u32x4 gemm_u16_a4 __attribute__((aligned(4)));
+template <typename T> __device__ __forceinline__ u32x4 gemm_guarded(const T* p, int n) {
+    constexpr int N = 16 / sizeof(T);
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (n >= N) {
+        if constexpr (sizeof(T) == 2) v = *(const gemm_u16_a2*)p;
+        else v = *(const gemm_u16_a4*)p;
+    } else if (n > 0) {
+#pragma unroll
+        for (int e = 0; e < N - 1; ++e)
+            if (e < n) {
+                if constexpr (sizeof(T) == 2) v[e >> 1] |= (unsigned)((const unsigned short*)p)[e] << ((e & 1) * 16);
+                else v[e] = ((const unsigned*)p)[e];
+            }
+    }
+    return v;
+}
+
+// 8 outputs of row m from column n on: bias, residual, the value before the activation, the activation
+template <typename T>
+__device__ __forceinline__ void gemm_finish(const GemmArgs& a, long m, long n, float (&v)[8], const float (&bias)[8]) {
+    typedef T VT __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    typedef float VF __attribute__((ext_vector_type(8)));
+    const bool full = n + 8 <= a.N;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += bias[e];
+    if (a.res) {
+        const T* r = (const T*)a.res + m * a.ldr + n;
+        if (full) {
+            const VF f = __builtin_convertvector(*(const VT*)r, VF);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += f[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (n + e < a.N) v[e] += (float)r[e];
         }
-        __syncthreads();
-        u32x4 fa[2], fb[2];
+    }
+    VF o;
+    if (a.pre) {
+        T* p = (T*)a.pre + m * a.ldp + n;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            fa[i] = *(const u32x4*)(As + (wm + i * 16 + l15) * GROW + g * 16);
-            fb[i] = *(const u32x4*)(Bs + (wn + i * 16 + l15) * GROW + g * 16);
+        for (int e = 0; e < 8; ++e) o[e] = v[e];
+        if (full) {
+            *(VT*)p = __builtin_convertvector(o, VT);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (n + e < a.N) p[e] = (T)v[e];
         }
+    }
+    T* c = (T*)a.C + m * a.ldc + n;
+    if (a.act == LIN_SILU) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int e = 0; e < 8; ++e) v[e] = lin_act(v[e], LIN_SILU);
+    } else if (a.act == LIN_RELU) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+        for (int e = 0; e < 8; ++e) v[e] = lin_act(v[e], LIN_RELU);
+    } else if (a.act == LIN_GELU) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = lin_act(v[e], LIN_GELU);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = v[e];
+    if (full) {
+        *(VT*)c = __builtin_convertvector(o, VT);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (n + e < a.N) c[e] = (T)v[e];
+    }
+}
+__device__ __forceinline__ void gemm_bias(const GemmArgs& a, long n, float (&b)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = a.bias && n + e < a.N ? a.bias[n + e] : 0.f;
+}
+
+template <int I, int N_, typename Fn> __device__ __forceinline__ void gemm_for(Fn&& f) {
+    if constexpr (I < N_) {
+        f(std::integral_constant<int, I>{});
+        gemm_for<I + 1, N_>(f);
+    }
+}
+
+// DMA: both operands have 16-byte aligned rows whose length along the contiguous index is a multiple of a piece, and come
+// by direct loads into LDS; otherwise they are staged through registers, with every access guarded.
+template <typename T, bool AKC, bool BKC, int F, bool DMA>
+__global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
+    typedef GemmOperand<T, AKC, F> OA;
+    typedef GemmOperand<T, BKC, F> OB;
+    constexpr int ES = sizeof(T), TILE = 32 * F, BK = OA::BK, NP = OA::NP, STAGE = OA::BYTES;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];       // [A: 2 stages][B: 2 stages]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
+
+    // the tile: neighbouring tiles on one XCD (workgroups go round the eight XCDs), panels of eight tile columns
+    const unsigned total = gridDim.x, per = total / 8;
+    unsigned lin = blockIdx.x;
+    if (lin < per * 8) lin = (lin & 7) * per + (lin >> 3);
+    const unsigned ntn = (unsigned)((a.N + TILE - 1) / TILE), ntm = (unsigned)((a.M + TILE - 1) / TILE);
+    const unsigned z = lin / (ntn * ntm), id = lin - z * (ntn * ntm);
+    const unsigned panel = id / (ntm * 8), in_panel = id - panel * (ntm * 8);
+    const unsigned pw = ntn - panel * 8 < 8 ? ntn - panel * 8 : 8;
+    const long m0 = (long)(in_panel / pw) * TILE, n0 = (long)(panel * 8 + in_panel % pw) * TILE;
+    const long kbeg = (long)z * a.kper * BK, kend = a.K < kbeg + (long)a.kper * BK ? a.K : kbeg + (long)a.kper * BK;
+    const int nt = (int)((kend - kbeg + BK - 1) / BK);
+
+    const int wm = (wave >> 1) * (TILE / 2), wn = (wave & 1) * (TILE / 2);
+    const char* ap = (const char*)a.A + (AKC ? m0 * a.lda + kbeg : kbeg * a.lda + m0) * ES;
+    const char* bp = (const char*)a.B + (BKC ? n0 * a.ldb + kbeg : kbeg * a.ldb + n0) * ES;
+    const long astep = AKC ? 128 : a.lda * BK * ES, bstep = BKC ? 128 : a.ldb * BK * ES;
+    const int arows = (int)(a.M - m0 < TILE ? a.M - m0 : TILE), brows = (int)(a.N - n0 < TILE ? a.N - n0 : TILE);
+    const int klen = (int)(kend - kbeg < (1L << 30) ? kend - kbeg : (1L << 30));
+
+    // this lane's pieces: offset from the step's start (out of range where the tile ends), and index along k
+    constexpr unsigned NONE = 0x80000000u;
+    unsigned va[NP], vb[NP];
+    int ka[NP], kb[NP], ea[NP], eb[NP];
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+        int row, el;
+        OA::piece((wave * NP + q) * 64 + lane, row, el);
+        const int ma = AKC ? row : el;
+        ka[q] = AKC ? el : row;
+        ea[q] = el;
+        va[q] = ma < arows ? (unsigned)((long)row * a.lda * ES + el * ES) : NONE;
+        OB::piece((wave * NP + q) * 64 + lane, row, el);
+        const int mb = BKC ? row : el;
+        kb[q] = BKC ? el : row;
+        eb[q] = el;
+        vb[q] = mb < brows ? (unsigned)((long)row * a.ldb * ES + el * ES) : NONE;
+    }
+    u32x4 ra[DMA ? 1 : NP], rb[DMA ? 1 : NP];
+    // asks for piece q of both operands of step t (steps behind the last one: zeros, without a memory access)
+    auto request = [&](int t, int q) {
+        const int kleft = klen - t * BK;
+        if constexpr (DMA) {
+            const auto sa = __builtin_amdgcn_make_buffer_rsrc((void*)(ap + t * astep), 0, 0x80000000, 0x00020000);
+            const auto sb = __builtin_amdgcn_make_buffer_rsrc((void*)(bp + t * bstep), 0, 0x80000000, 0x00020000);
+            char* la = smem + (t & 1) * STAGE + (wave * NP + q) * 1024;
+            const unsigned oa = kleft < BK && ka[q] >= kleft ? NONE : va[q], ob = kleft < BK && kb[q] >= kleft ? NONE : vb[q];
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(sa, (__attribute__((address_space(3))) void*)la, 16, oa, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(sb, (__attribute__((address_space(3))) void*)(la + 2 * STAGE), 16, ob, 0, 0, 0);
+        } else {
+            ra[q] = gemm_guarded<T>((const T*)(ap + t * astep + va[q]),
+                                    va[q] == NONE || ka[q] >= kleft ? 0 : AKC ? kleft - ka[q] : arows - ea[q]);
+            rb[q] = gemm_guarded<T>((const T*)(bp + t * bstep + vb[q]),
+                                    vb[q] == NONE || kb[q] >= kleft ? 0 : BKC ? kleft - kb[q] : brows - eb[q]);
+        }
+    };
+    // step t's pieces of this wave are in LDS
+    auto land = [&](int t) {
+        if constexpr (DMA) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        } else {
+            char* la = smem + (t & 1) * STAGE + (wave * NP * 64 + lane) * 16;
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                *(u32x4*)(la + q * 1024) = ra[q];
+                *(u32x4*)(la + 2 * STAGE + q * 1024) = rb[q];
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    };
+
+    f32x4 acc[F][F];       // [row fragment][column fragment]
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    GemmFrag<T, AKC> fa[2][F];
+    GemmFrag<T, BKC> fb[2][F];
+    unsigned aa[2], bb[2];      // fragment addresses of the two halves, in the stage that is read next
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        aa[s] = lds0 + OA::base(lane, wm, s);
+        bb[s] = lds0 + 2 * STAGE + OB::base(lane, wn, s);
+    }
+    auto landed = [&](auto S) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < F; ++i) { fa[S][i].landed(); fb[S][i].landed(); }
+    };
+    // products of half S, with the reads of the other half's fragments (and a step's requests) between them
+    auto multiply = [&](auto S, auto REQ, int t) {
+        constexpr int s = S, r = 1 - S;
+        gemm_for<0, F>([&](auto I) {
+            constexpr int i = I;
+            if constexpr (REQ) {
+                if constexpr (i < NP) request(t + 2, i);
+            }
+            OA::template read<i, r>(fa[r][i], aa[r]);
+            OB::template read<i, r>(fb[r][i], bb[r]);
+#pragma unroll
+            for (int j = 0; j < F; ++j) {
                 if constexpr (ES == 2) {
-                    acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fb[j]),
-                                                                        __builtin_bit_cast(bf16x8, fa[i]), acc[j][i], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fb[s][j].bits()),
+                                                                        __builtin_bit_cast(bf16x8, fa[s][i].bits()),
+                                                                        acc[i][j], 0, 0, 0);
                 } else {
-                    // lane group g holds k = 4 g .. 4 g + 3; product q takes element q of both operands
-                    const f32x4 va = __builtin_bit_cast(f32x4, fa[i]), vb = __builtin_bit_cast(f32x4, fb[j]);
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(vb[q], va[q], acc[j][i], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[s][j].f32(q), fa[s][i].f32(q), acc[i][j], 0, 0, 0);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    auto step = [&](int t) {
+        multiply(std::integral_constant<int, 0>{}, std::false_type{}, t);
+        landed(std::integral_constant<int, 1>{});
+        land(t + 1);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        aa[0] ^= STAGE; aa[1] ^= STAGE; bb[0] ^= STAGE; bb[1] ^= STAGE;
+        multiply(std::integral_constant<int, 1>{}, std::true_type{}, t);
+        landed(std::integral_constant<int, 0>{});
+    };
+
+    if (nt > 0) {
+#pragma unroll
+        for (int q = 0; q < NP; ++q) request(0, q);
+        land(0);
+#pragma unroll
+        for (int q = 0; q < NP; ++q) request(1, q);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        gemm_for<0, F>([&](auto I) {
+            OA::template read<I, 0>(fa[0][I], aa[0]);
+            OB::template read<I, 0>(fb[0][I], bb[0]);
+        });
+        landed(std::integral_constant<int, 0>{});
+        for (int t = 0; t < nt; ++t) step(t);
+        land(nt);            // nothing is on its way into LDS any more
     }
+    __syncthreads();
+
+    // epilogue: 16 rows at a time through LDS, so that memory sees whole rows
+    constexpr int ROW = F * 64 + 16, LPR = F * 2, RPP = 64 / LPR;       // bytes of a row, lanes per row, rows per pass
+    char* tr = smem + wave * 16 * ROW;
+    const int g = lane >> 4, l15 = lane & 15, c = (lane % LPR) * 8, r0 = lane / LPR;
+    const long n = n0 + wn + c;
+    float bias[8];
+    gemm_bias(a, n, bias);
+    const long np = (a.N + 7) & ~7L;
+    gemm_for<0, F>([&](auto I) {
+        constexpr int i = I;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const long m = m0 + wm + i * 16 + l15;
-        if (m >= a.M) continue;
+        for (int j = 0; j < F; ++j) *(f32x4*)(tr + l15 * ROW + j * 64 + g * 16) = acc[i][j];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const long n = n0 + wn + j * 16 + g * 4 + r;
-                if (n >= a.N) continue;
-                float v = acc[j][i][r];
-                if (a.bias) v += a.bias[n];
-                if (a.res) v += (float)((const T*)a.res)[m * a.ldr + n];
-                if (a.pre) ((T*)a.pre)[m * a.ldp + n] = (T)v;
-                ((T*)a.C)[m * a.ldc + n] = (T)lin_act(v, a.act);
+        for (int p = 0; p < 16 / RPP; ++p) {
+            const int row = p * RPP + r0;
+            const long m = m0 + wm + i * 16 + row;
+            const f32x4 lo = *(const f32x4*)(tr + row * ROW + c * 4), hi = *(const f32x4*)(tr + row * ROW + c * 4 + 16);
+            if (m >= a.M || n >= a.N) continue;
+            if (a.part) {
+                float* o = a.part + ((long)z * a.M + m) * np + n;
+                *(f32x4*)o = lo;
+                *(f32x4*)(o + 4) = hi;
+            } else {
+                float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                gemm_finish<T>(a, m, n, v, bias);
             }
+        }
+    });
+}
+
+// joins the parts of a split contraction, in order, and finishes
+template <typename T>
+__global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a, int parts) {
+    const long np = (a.N + 7) & ~7L, pieces = np / 8;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.M * pieces) return;
+    const long m = i / pieces, n = (i - m * pieces) * 8;
+    float bias[8], v[8] = {};
+    gemm_bias(a, n, bias);
+    const float* p = a.part + m * np + n;
+    for (int z = 0; z < parts; ++z, p += a.M * np) {
+        const f32x4 lo = *(const f32x4*)p, hi = *(const f32x4*)(p + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] += lo[e];
+            v[4 + e] += hi[e];
+        }
     }
+    gemm_finish<T>(a, m, n, v, bias);
 }
 
 // dz = dy act'(pre), and the column sums of dz over this workgroup's rows (part [gridDim.x][N])
@@ -122,25 +440,82 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long lddy, 
     if (part) part[blockIdx.x * N + n] = s;
 }
 
-template <typename T>
-int gemm(const GemmArgs& a, bool akc, bool bkc, hipStream_t s) {
-    if (a.M == 0 || a.N == 0) return LDM_OK;
-    const long tiles = ((a.N + GT - 1) / GT) * ((a.M + GT - 1) / GT);
-    LDM_REQUIRE(tiles < (1L << 31), "more output tiles than one launch holds");
-    const unsigned grid = (unsigned)tiles;
-    if (akc && bkc) gemm_any_kernel<T, true, true><<<grid, 256, 0, s>>>(a);
-    else if (akc) gemm_any_kernel<T, true, false><<<grid, 256, 0, s>>>(a);
-    else gemm_any_kernel<T, false, false><<<grid, 256, 0, s>>>(a);
+// Tile and split of one product.
+struct GemmPlan { int F, parts, kper; };
+GemmPlan gemm_plan(int es, long M, long N, long K, bool big_ok) {
+    const long bk = 128 / es, steps = (K + bk - 1) / bk;
+    auto tiles = [&](long t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
+    GemmPlan p;
+    p.F = big_ok && es == 2 && tiles(256) * (steps / 8 > 1 ? steps / 8 : 1) >= 192 ? 8 : 4;
+    const long n = tiles(32 * p.F), slots = p.F == 8 ? 256 : 512;
+    long parts = n > 0 && n < slots ? slots / n : 1;
+    const long most = steps / 4 > 1 ? steps / 4 : 1;         // at least four steps a part
+    if (parts > most) parts = most;
+    if (parts > 64) parts = 64;
+    p.kper = (int)((steps + parts - 1) / parts);
+    if (p.kper < 1) p.kper = 1;
+    p.parts = (int)((steps + p.kper - 1) / p.kper);
+    if (p.parts < 1) p.parts = 1;
+    return p;
+}
+long gemm_part_floats(const GemmPlan& p, long M, long N) { return p.parts > 1 ? p.parts * M * ((N + 7) & ~7L) : 0; }
+
+template <typename T, bool AKC, bool BKC, int F, bool DMA>
+int gemm_launch(const GemmArgs& a, unsigned grid, hipStream_t s) {
+    static bool done[kMaxDevices] = {};
+    constexpr int lds = 4 * GemmOperand<T, AKC, F>::BYTES;
+    LDM_TRY(allow_dynamic_lds((const void*)&gemm_kernel<T, AKC, BKC, F, DMA>, lds, done));
+    gemm_kernel<T, AKC, BKC, F, DMA><<<grid, 256, lds, s>>>(a);
     LDM_HIP(hipGetLastError());
     return LDM_OK;
+}
+
+template <typename T, bool AKC, bool BKC>
+int gemm(GemmArgs a, float* ws, hipStream_t s) {
+    if (a.M == 0 || a.N == 0) return LDM_OK;
+    constexpr long V = 16 / sizeof(T);
+    auto aligned = [&](const void* p, long ld, long len) {
+        return (size_t)p % 16 == 0 && ld % V == 0 && len % V == 0 && ld <= (1L << 21);
+    };
+    const bool dma = aligned(a.A, a.lda, AKC ? a.K : a.M) && aligned(a.B, a.ldb, BKC ? a.K : a.N);
+    LDM_REQUIRE(a.lda <= (1L << 21) && a.ldb <= (1L << 21), "operand rows are more than 2^21 elements apart");
+    const GemmPlan p = gemm_plan(sizeof(T), a.M, a.N, a.K, dma);
+    LDM_REQUIRE(p.parts == 1 || ws, "this product needs a workspace");
+    const long t = 32 * p.F, tiles = ((a.M + t - 1) / t) * ((a.N + t - 1) / t) * p.parts;
+    LDM_REQUIRE(tiles < (1L << 31), "more output tiles than one launch holds");
+    a.kper = p.kper;
+    a.part = p.parts > 1 ? ws : nullptr;
+    if (!dma) LDM_TRY((gemm_launch<T, AKC, BKC, 4, false>(a, (unsigned)tiles, s)));
+    else if (p.F == 4) LDM_TRY((gemm_launch<T, AKC, BKC, 4, true>(a, (unsigned)tiles, s)));
+    else if constexpr (sizeof(T) == 2) LDM_TRY((gemm_launch<T, AKC, BKC, 8, true>(a, (unsigned)tiles, s)));
+    if (p.parts > 1) {
+        const long n = a.M * ((a.N + 7) / 8);
+        gemm_join_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a, p.parts);
+        LDM_HIP(hipGetLastError());
+    }
+    return LDM_OK;
+}
+template <typename T>
+int gemm_by_order(const GemmArgs& a, bool akc, bool bkc, float* ws, hipStream_t s) {
+    return akc ? (bkc ? gemm<T, true, true>(a, ws, s) : gemm<T, true, false>(a, ws, s)) : gemm<T, false, false>(a, ws, s);
 }
 
 long dz_groups(long M, long N) { return M < 512 ? M : 512; }
 
 }  // namespace
 
-int launch_gemm(int dtype, const GemmArgs& a, bool akc, bool bkc, hipStream_t s) {
-    return dtype == LDM_BF16 ? gemm<__bf16>(a, akc, bkc, s) : gemm<float>(a, akc, bkc, s);
+int launch_gemm(int dtype, const GemmArgs& a, bool akc, bool bkc, float* ws, hipStream_t s) {
+    return dtype == LDM_BF16 ? gemm_by_order<__bf16>(a, akc, bkc, ws, s) : gemm_by_order<float>(a, akc, bkc, ws, s);
+}
+
+long gemm_ws_floats(int dtype, long M, long N, long K) {
+    // which tile it will be depends on the alignment as well
+    long n = 0;
+    for (int big = 0; big < 2; ++big) {
+        const long f = gemm_part_floats(gemm_plan(dtype == LDM_BF16 ? 2 : 4, M, N, K, big), M, N);
+        n = f > n ? f : n;
+    }
+    return n;
 }
 
 long linear_dz_ws_floats(long M, long N) { return dz_groups(M, N) * N; }

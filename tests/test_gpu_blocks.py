@@ -302,7 +302,7 @@ def test_rope_gradient_is_the_transposed_map(ops):
 # ---- linear -----------------------------------------------------------------------------------------------------------
 LIN_SHAPES = [(1, 1, 1), (1, 256, 2048), (4, 256, 2048), (2, 17, 33), (5, 8, 8), (16, 100, 64), (31, 64, 128), (64, 33, 7),
               (130, 70, 66), (257, 129, 255), (300, 1024, 512), (1000, 321, 643), (128, 64, 64), (129, 2048, 1),
-              (1, 4100, 5), (700, 1, 300), (512, 512, 512), (2050, 256, 264)]
+              (1, 4100, 5), (700, 1, 300), (512, 512, 512), (2050, 256, 264), (4100, 1032, 2056)]
 
 
 def _act_ref(z, act):
