@@ -329,7 +329,11 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
             OB::template read<i, r>(fb[r][i], bb[r]);
 #pragma unroll
             for (int j = 0; j < F; ++j) {
-                if constexpr (ES == 2) {
+                if constexpr (F == 8) {
+                    // in place by constraint: with all 256 accumulators live the compiler's own choice moves them about
+                    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0"
+                                 : "+a"(acc[i][j]) : "v"(fb[s][j].bits()), "v"(fa[s][i].bits()));
+                } else if constexpr (ES == 2) {
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fb[s][j].bits()),
                                                                         __builtin_bit_cast(bf16x8, fa[s][i].bits()),
                                                                         acc[i][j], 0, 0, 0);
@@ -369,6 +373,8 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         for (int t = 0; t < nt; ++t) step(t);
         land(nt);            // nothing is on its way into LDS any more
     }
+    // the last products' results may be read
+    if constexpr (F == 8) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
     __syncthreads();
 
     // epilogue: 16 rows at a time through LDS, so that memory sees whole rows
@@ -379,10 +385,15 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     float bias[8];
     gemm_bias(a, n, bias);
     const long np = (a.N + 7) & ~7L;
-    gemm_for<0, F>([&](auto I) {
-        constexpr int i = I;
+    // one copy of this code for all row fragments: unrolled over them it would not fit the instruction cache
+#pragma unroll 1
+    for (int i = 0; i < F; ++i) {
+        gemm_for<0, F>([&](auto I) {
+            if (i == I) {
 #pragma unroll
-        for (int j = 0; j < F; ++j) *(f32x4*)(tr + l15 * ROW + j * 64 + g * 16) = acc[i][j];
+                for (int j = 0; j < F; ++j) *(f32x4*)(tr + l15 * ROW + j * 64 + g * 16) = acc[I][j];
+            }
+        });
 #pragma unroll
         for (int p = 0; p < 16 / RPP; ++p) {
             const int row = p * RPP + r0;
@@ -398,7 +409,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
                 gemm_finish<T>(a, m, n, v, bias);
             }
         }
-    });
+    }
 }
 
 // joins the parts of a split contraction, in order, and finishes
