@@ -25,10 +25,12 @@ struct RopeArgs {
     const void* pos;
     int pos_dtype;                 // 0 int32, 1 int64, 2 f32
     long pos_sb, pos_sa, pos_sn;
-    int sec_end[4];                // first pair behind each axis (P for the axes that are not there)
+    int axes;
+    int sec_end[4];                // first pair behind each axis; D for the last one and those that are not there
     const float* inv_freq;         // [P]
     int inverse;
     int nrot, nchunk, tpb, hpg;    // set by launch_rope
+    unsigned groups;
 };
 int launch_rope(int dtype, int interleaved, RopeArgs a, hipStream_t s);
 
@@ -50,7 +52,7 @@ struct GemmArgs {
 long gemm_ws_floats(int dtype, long M, long N, long K);
 int launch_gemm(int dtype, const GemmArgs& a, bool akc, bool bkc, float* ws, hipStream_t s);
 // dz = dy act'(pre) (not written without an activation: dz is dy) and db = column sums of dz (db null: not taken)
-long linear_dz_ws_floats(long M, long N);
+long linear_dz_ws_floats(int dtype, long M, long N);
 int launch_linear_dz(int dtype, const void* dy, long lddy, const void* pre, long ldp, void* dz, long lddz, float* db, float* ws,
                      long M, long N, int act, hipStream_t s);
 

@@ -7,6 +7,7 @@
 // (E[x^2] - mu^2 would lose it for rows far from zero).
 // Rows need no alignment: 16-byte vector accesses at element alignment, which this target's global memory serves.
 #include "blocks.h"
+#include "vec.h"
 
 namespace ldm {
 
@@ -32,80 +33,22 @@ struct LnBwdArgs {
     int C;
 };
 
-template <typename T> struct LnVec;
-template <> struct LnVec<float> {
-    static constexpr int N = 4;
-    typedef float V __attribute__((ext_vector_type(4), aligned(4)));
-    static __device__ __forceinline__ float get(const float* p) { return *p; }
-    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
-    static __device__ __forceinline__ void load(const float* p, float* o) {
-        const V v = *(const V*)p;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = v[e];
-    }
-    static __device__ __forceinline__ void store(float* p, const float* o) {
-        V v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = o[e];
-        *(V*)p = v;
-    }
-};
-template <> struct LnVec<__bf16> {
-    static constexpr int N = 8;
-    typedef __bf16 V __attribute__((ext_vector_type(8), aligned(2)));
-    typedef float F __attribute__((ext_vector_type(8)));
-    static __device__ __forceinline__ float get(const __bf16* p) { return (float)*p; }
-    static __device__ __forceinline__ void put(__bf16* p, float v) { *p = (__bf16)v; }
-    static __device__ __forceinline__ void load(const __bf16* p, float* o) {
-        const F v = __builtin_convertvector(*(const V*)p, F);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = v[e];
-    }
-    static __device__ __forceinline__ void store(__bf16* p, const float* o) {
-        F v;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = o[e];
-        *(V*)p = __builtin_convertvector(v, V);
-    }
-};
-
-// VEC elements at column c of a row of C (zero behind its end)
-template <typename T>
-__device__ __forceinline__ void ln_load(const T* row, int c, int C, float* o) {
-    constexpr int N = LnVec<T>::N;
-    if (c + N <= C) {
-        LnVec<T>::load(row + c, o);
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = c + e < C ? LnVec<T>::get(row + c + e) : 0.f;
-    }
-}
-template <typename T>
-__device__ __forceinline__ void ln_store(T* row, int c, int C, const float* o) {
-    constexpr int N = LnVec<T>::N;
-    if (c + N <= C) {
-        LnVec<T>::store(row + c, o);
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (c + e < C) LnVec<T>::put(row + c + e, o[e]);
-    }
-}
-// NE f32 parameters of the columns c .. c + NE - 1
+// NE f32 parameters of the columns c .. c + NE - 1, in 16-byte loads: every workgroup reads the same few lines, and single
+// words made that the bottleneck of short rows (16384 x 256 in bf16: 18.4 us with words)
 template <int NE>
 __device__ __forceinline__ void ln_param(const float* p, int c, int C, float dflt, float* o) {
 #pragma unroll
-    for (int e = 0; e < NE; ++e) o[e] = p && c + e < C ? p[c + e] : dflt;
+    for (int e = 0; e < NE; e += 4) {
+        if (p) row_floats<float>(row_load<float>(p + c + e, C - c - e), o + e);
+        else o[e] = o[e + 1] = o[e + 2] = o[e + 3] = dflt;
+    }
 }
 
 // sums over the LPR lanes of a row, the same bits in every lane; LPR = 256: the whole workgroup, through `sm` (8 floats)
 template <int LPR>
 __device__ __forceinline__ void ln_sum2(float& a, float& b, float* sm) {
-#pragma unroll
-    for (int m = 1; m < (LPR < 64 ? LPR : 64); m <<= 1) {
-        a += __shfl_xor(a, m);
-        b += __shfl_xor(b, m);
-    }
+    a = lanes_sum<LPR < 64 ? LPR : 64>(a);
+    b = lanes_sum<LPR < 64 ? LPR : 64>(b);
     if constexpr (LPR > 64) {
         __syncthreads();                 // the previous sums have been read
         if ((threadIdx.x & 63) == 0) {
@@ -126,7 +69,7 @@ __device__ __forceinline__ float ln_sum(float a, float* sm) {
 
 template <typename T, int NV, int LPR>
 __global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
-    constexpr int N = LnVec<T>::N, RPB = 256 / LPR;
+    constexpr int N = RowVec<T>::N, RPB = 256 / LPR;
     __shared__ float sm[8];
     const int l = threadIdx.x % LPR;
     float w[NV][N], b[NV][N];
@@ -136,16 +79,25 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
         ln_param<N>(a.b, (v * LPR + l) * N, a.C, 0.f, b[v]);
     }
     const float n = (float)a.C;      // divided by, not multiplied with 1 / C: the mean of a constant row is exact
-    for (long row = (long)blockIdx.x * RPB + threadIdx.x / LPR; row < a.rows; row += (long)gridDim.x * RPB) {
-        const T* xr = (const T*)a.x + row * a.xs;
+    const long step = (long)gridDim.x * RPB;
+    long row = (long)blockIdx.x * RPB + threadIdx.x / LPR;
+    typename RowVec<T>::R next[NV];  // the next row is on its way while this one is reduced
+    auto fetch = [&](long r) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+            next[v] = row_load<T>((const T*)a.x + r * a.xs + (v * LPR + l) * N, a.C - (v * LPR + l) * N);
+    };
+    if (row < a.rows) fetch(row);
+    for (; row < a.rows; row += step) {
         float x[NV][N];
         float s = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            ln_load<T>(xr, (v * LPR + l) * N, a.C, x[v]);
+            row_floats<T>(next[v], x[v]);
 #pragma unroll
             for (int e = 0; e < N; ++e) s += x[v][e];
         }
+        if (row + step < a.rows) fetch(row + step);
         const float mu = ln_sum<LPR>(s, sm) / n;
         float q = 0.f;
 #pragma unroll
@@ -162,7 +114,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
             float o[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) o[e] = x[v][e] * r * w[v][e] + b[v][e];
-            ln_store<T>(yr, (v * LPR + l) * N, a.C, o);
+            row_store<T>(yr + (v * LPR + l) * N, a.C - (v * LPR + l) * N, o);
         }
         if (l == 0) {
             if (a.mean) a.mean[row] = mu;
@@ -175,7 +127,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
 // third time from the caches).
 template <typename T>
 __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(LnFwdArgs a) {
-    constexpr int N = LnVec<T>::N;
+    constexpr int N = RowVec<T>::N;
     __shared__ float sm[8];
     const float n = (float)a.C;
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -183,7 +135,7 @@ __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(LnFwdArgs a) {
         float s = 0.f;
         for (int c = threadIdx.x * N; c < a.C; c += 256 * N) {
             float x[N];
-            ln_load<T>(xr, c, a.C, x);
+            row_floats<T>(row_load<T>(xr + c, a.C - c), x);
 #pragma unroll
             for (int e = 0; e < N; ++e) s += x[e];
         }
@@ -191,7 +143,7 @@ __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(LnFwdArgs a) {
         float q = 0.f;
         for (int c = threadIdx.x * N; c < a.C; c += 256 * N) {
             float x[N];
-            ln_load<T>(xr, c, a.C, x);
+            row_floats<T>(row_load<T>(xr + c, a.C - c), x);
 #pragma unroll
             for (int e = 0; e < N; ++e)
                 if (c + e < a.C) q += (x[e] - mu) * (x[e] - mu);
@@ -200,12 +152,12 @@ __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(LnFwdArgs a) {
         T* yr = (T*)a.y + row * a.ys;
         for (int c = threadIdx.x * N; c < a.C; c += 256 * N) {
             float x[N], w[N], b[N];
-            ln_load<T>(xr, c, a.C, x);
+            row_floats<T>(row_load<T>(xr + c, a.C - c), x);
             ln_param<N>(a.w, c, a.C, 1.f, w);
             ln_param<N>(a.b, c, a.C, 0.f, b);
 #pragma unroll
             for (int e = 0; e < N; ++e) x[e] = (x[e] - mu) * r * w[e] + b[e];
-            ln_store<T>(yr, c, a.C, x);
+            row_store<T>(yr + c, a.C - c, x);
         }
         if (threadIdx.x == 0) {
             if (a.mean) a.mean[row] = mu;
@@ -218,7 +170,7 @@ __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(LnFwdArgs a) {
 // groups are joined through LDS in a fixed order and written as one partial row, which colsum_kernel adds up.
 template <typename T, int NV, int LPR>
 __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
-    constexpr int N = LnVec<T>::N, RPB = 256 / LPR;
+    constexpr int N = RowVec<T>::N, RPB = 256 / LPR;
     __shared__ float sm[8];
     __shared__ float join[256 * N];
     const int l = threadIdx.x % LPR;
@@ -230,17 +182,34 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
         for (int e = 0; e < N; ++e) aw[v][e] = ab[v][e] = 0.f;
     }
     const float inv = 1.0f / (float)a.C;
-    for (long row = (long)blockIdx.x * RPB + threadIdx.x / LPR; row < a.rows; row += (long)gridDim.x * RPB) {
-        const T* xr = (const T*)a.x + row * a.xs;
-        const T* dr = (const T*)a.dy + row * a.dys;
-        float xh[NV][N], g[NV][N];
+    const long step = (long)gridDim.x * RPB;
+    long row = (long)blockIdx.x * RPB + threadIdx.x / LPR;
+    typename RowVec<T>::R nx[NV], nd[NV], na[NV];       // the next row is on its way while this one is reduced
+    float nmu = 0.f, nr = 0.f;
+    auto fetch = [&](long r) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            ln_load<T>(xr, (v * LPR + l) * N, a.C, xh[v]);
-            ln_load<T>(dr, (v * LPR + l) * N, a.C, g[v]);
+            const int c = (v * LPR + l) * N, left = a.C - c;
+            nx[v] = row_load<T>((const T*)a.x + r * a.xs + c, left);
+            nd[v] = row_load<T>((const T*)a.dy + r * a.dys + c, left);
+            if (a.add) na[v] = row_load<T>((const T*)a.add + r * a.as + c, left);
         }
-        const float mu = a.mean[row], r = a.rstd[row];
+        nmu = a.mean[r];
+        nr = a.rstd[r];
+    };
+    if (row < a.rows) fetch(row);
+    for (; row < a.rows; row += step) {
+        float xh[NV][N], g[NV][N];
+        typename RowVec<T>::R add[NV];
+        const float mu = nmu, r = nr;
         float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            row_floats<T>(nx[v], xh[v]);
+            row_floats<T>(nd[v], g[v]);
+            add[v] = na[v];
+        }
+        if (row + step < a.rows) fetch(row + step);
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -263,11 +232,11 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
             for (int e = 0; e < N; ++e) o[e] = r * (g[v][e] - s1 - xh[v][e] * s2);
             if (a.add) {
                 float p[N];
-                ln_load<T>((const T*)a.add + row * a.as, (v * LPR + l) * N, a.C, p);
+                row_floats<T>(add[v], p);
 #pragma unroll
                 for (int e = 0; e < N; ++e) o[e] += p[e];
             }
-            ln_store<T>(or_, (v * LPR + l) * N, a.C, o);
+            row_store<T>(or_ + (v * LPR + l) * N, a.C - (v * LPR + l) * N, o);
         }
     }
     if (!a.part) return;
@@ -293,7 +262,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
 // Rows too long for the registers: dx by re-reading the row, and the columns' sums by a kernel of their own.
 template <typename T>
 __global__ __launch_bounds__(256) void ln_bwd_wide_dx_kernel(LnBwdArgs a) {
-    constexpr int N = LnVec<T>::N;
+    constexpr int N = RowVec<T>::N;
     __shared__ float sm[8];
     const float inv = 1.0f / (float)a.C;
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -303,8 +272,8 @@ __global__ __launch_bounds__(256) void ln_bwd_wide_dx_kernel(LnBwdArgs a) {
         float s1 = 0.f, s2 = 0.f;
         for (int c = threadIdx.x * N; c < a.C; c += 256 * N) {
             float x[N], d[N], w[N];
-            ln_load<T>(xr, c, a.C, x);
-            ln_load<T>(dr, c, a.C, d);
+            row_floats<T>(row_load<T>(xr + c, a.C - c), x);
+            row_floats<T>(row_load<T>(dr + c, a.C - c), d);
             ln_param<N>(a.w, c, a.C, 1.f, w);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
@@ -318,27 +287,27 @@ __global__ __launch_bounds__(256) void ln_bwd_wide_dx_kernel(LnBwdArgs a) {
         s2 *= inv;
         for (int c = threadIdx.x * N; c < a.C; c += 256 * N) {
             float x[N], d[N], w[N], p[N];
-            ln_load<T>(xr, c, a.C, x);
-            ln_load<T>(dr, c, a.C, d);
+            row_floats<T>(row_load<T>(xr + c, a.C - c), x);
+            row_floats<T>(row_load<T>(dr + c, a.C - c), d);
             ln_param<N>(a.w, c, a.C, 1.f, w);
-            if (a.add) ln_load<T>((const T*)a.add + row * a.as, c, a.C, p);
+            if (a.add) row_floats<T>(row_load<T>((const T*)a.add + row * a.as + c, a.C - c), p);
 #pragma unroll
             for (int e = 0; e < N; ++e)
                 x[e] = r * (d[e] * w[e] - s1 - (x[e] - mu) * r * s2) + (a.add ? p[e] : 0.f);
-            ln_store<T>((T*)a.dx + row * a.dxs, c, a.C, x);
+            row_store<T>((T*)a.dx + row * a.dxs + c, a.C - c, x);
         }
     }
 }
 template <typename T>
 __global__ __launch_bounds__(256) void ln_bwd_wide_dw_kernel(LnBwdArgs a) {
-    constexpr int N = LnVec<T>::N;
+    constexpr int N = RowVec<T>::N;
     const int c = (blockIdx.y * 256 + threadIdx.x) * N;
     if (c >= a.C) return;
     float aw[N] = {}, ab[N] = {};
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         float x[N], d[N];
-        ln_load<T>((const T*)a.x + row * a.xs, c, a.C, x);
-        ln_load<T>((const T*)a.dy + row * a.dys, c, a.C, d);
+        row_floats<T>(row_load<T>((const T*)a.x + row * a.xs + c, a.C - c), x);
+        row_floats<T>(row_load<T>((const T*)a.dy + row * a.dys + c, a.C - c), d);
         const float mu = a.mean[row], r = a.rstd[row];
 #pragma unroll
         for (int e = 0; e < N; ++e) {
@@ -354,21 +323,23 @@ __global__ __launch_bounds__(256) void ln_bwd_wide_dw_kernel(LnBwdArgs a) {
         }
 }
 
-// out[k][c] = sum over g of part[k][g][c], in a fixed order: sixteen threads per column take every sixteenth row
+// out[k][c] = sum over g of part[k][g][c], in a fixed order: 32 threads per column take every 32nd row
 __global__ __launch_bounds__(1024) void colsum_kernel(const float* part, int G, int C, float* o0, float* o1) {
-    __shared__ float sm[16][64];
-    const int cl = threadIdx.x & 63, sl = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + cl;
+    __shared__ float sm[32][33];
+    const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + cl;
     const int k = blockIdx.y;
     float s = 0.f;
-    if (c < C)
-        for (int g = sl; g < G; g += 16) s += part[((long)k * G + g) * C + c];
+    if (c < C) {
+#pragma unroll 8
+        for (int g = sl; g < G; g += 32) s += part[((long)k * G + g) * C + c];
+    }
     sm[sl][cl] = s;
     __syncthreads();
     if (sl == 0 && c < C) {
         float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) t += sm[i][cl];
+        for (int i = 0; i < 32; ++i) t += sm[i][cl];
         (k ? o1 : o0)[c] = t;
     }
 }
@@ -433,7 +404,7 @@ int ln_bwd(const LnBwdArgs& a, hipStream_t s) {
         ln_bwd_wide_dx_kernel<T><<<(unsigned)(a.rows < 2048 ? a.rows : 2048), 256, 0, s>>>(a);
         LDM_HIP(hipGetLastError());
         if (a.part) {
-            const unsigned cb = (unsigned)((a.C + 256 * LnVec<T>::N - 1) / (256 * LnVec<T>::N));
+            const unsigned cb = (unsigned)((a.C + 256 * RowVec<T>::N - 1) / (256 * RowVec<T>::N));
             ln_bwd_wide_dw_kernel<T><<<dim3(G, cb), 256, 0, s>>>(a);
         }
     } else {
@@ -446,7 +417,7 @@ int ln_bwd(const LnBwdArgs& a, hipStream_t s) {
 }  // namespace
 
 int launch_colsum(const float* part, int G, int C, int nsums, float* out0, float* out1, hipStream_t s) {
-    colsum_kernel<<<dim3((unsigned)((C + 63) / 64), (unsigned)nsums), 1024, 0, s>>>(part, G, C, out0, out1);
+    colsum_kernel<<<dim3((unsigned)((C + 31) / 32), (unsigned)nsums), 1024, 0, s>>>(part, G, C, out0, out1);
     LDM_HIP(hipGetLastError());
     return LDM_OK;
 }

@@ -1504,6 +1504,7 @@ int ldm_rope(int dtype, const void* q, const void* k, void* oq, void* ok, const 
     }
     a.H[0] = Hq; a.H[1] = Hk;
     a.N = N; a.D = D; a.P = (int)P;
+    a.axes = axes;
     a.tokens = (long)B * N;
     a.pos = pos; a.pos_dtype = pos_type;
     a.pos_sb = pst[0]; a.pos_sa = pst[1]; a.pos_sn = pst[2];
@@ -1542,7 +1543,7 @@ int ldm_linear(int dtype, const void* x, long ldx, const void* w, long ldw, int 
 long ldm_linear_backward_ws_floats(int dtype, long M, long K, long N, int w_order) {
     if (check_linear(dtype, M, K, N, w_order, 0) != LDM_OK) return -1;
     // one after the other: the column sums of dz, dx, dw
-    long n = linear_dz_ws_floats(M, N);
+    long n = linear_dz_ws_floats(dtype, M, N);
     const long nx = gemm_ws_floats(dtype, M, K, N);
     const long nw = w_order == 0 ? gemm_ws_floats(dtype, K, N, M) : gemm_ws_floats(dtype, N, K, M);
     n = nx > n ? nx : n;

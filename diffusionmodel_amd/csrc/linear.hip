@@ -3,6 +3,7 @@
 // All three products are C[m, n] = sum_k A(m, k) B(k, n) on one kernel family; an operand is either contiguous along the
 // contraction (KC) or along its other index.
 #include "blocks.h"
+#include "vec.h"
 #include <type_traits>
 
 namespace ldm {
@@ -433,22 +434,55 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a, int parts) {
     gemm_finish<T>(a, m, n, v, bias);
 }
 
-// dz = dy act'(pre), and the column sums of dz over this workgroup's rows (part [gridDim.x][N])
+// dz = dy act'(pre), and the column sums of dz over this workgroup's rows (part [gridDim.x][N]).  One pass over dy and pre
+// and one write, bound by HBM: a thread keeps eight (f32: four) columns, `ct` threads cover a row's part, 256 / ct rows go
+// at once, and each thread asks for four rows before it uses the first.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long lddy, const T* pre, long ldp, T* dz, long lddz,
-                                                        float* part, long M, long N, int act) {
-    const long n = (long)blockIdx.y * 256 + threadIdx.x;
-    if (n >= N) return;
-    float s = 0.f;
-    for (long m = blockIdx.x; m < M; m += gridDim.x) {
-        float v = (float)dy[m * lddy + n];
-        if (act != LIN_NONE) {
-            v *= lin_dact((float)pre[m * ldp + n], act);
-            dz[m * lddz + n] = (T)v;
+                                                        float* part, long M, long N, int act, int ct) {
+    constexpr int V = RowVec<T>::N, U = 4;
+    __shared__ float join[256 * V];
+    const int c = threadIdx.x % ct, rg = threadIdx.x / ct, rgs = 256 / ct;
+    const long n = ((long)blockIdx.y * ct + c) * V;
+    const int left = n >= N ? 0 : N - n < V ? (int)(N - n) : V;
+    const long step = (long)gridDim.x * rgs;
+    float s[V] = {};
+    for (long m = (long)blockIdx.x * rgs + rg; m < M; m += U * step) {
+        typename RowVec<T>::R vd[U], vp[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long r = m + u * step;
+            vd[u] = row_load<T>(dy + r * lddy + n, r < M ? left : 0);
+            if (act != LIN_NONE) vp[u] = row_load<T>(pre + r * ldp + n, r < M ? left : 0);
         }
-        s += v;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long r = m + u * step;
+            float v[V];
+            row_floats<T>(vd[u], v);
+            if (act != LIN_NONE) {
+                float p[V];
+                row_floats<T>(vp[u], p);
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] *= lin_dact(p[e], act);
+                row_store<T>(dz + r * lddz + n, r < M ? left : 0, v);
+            }
+            if (r < M) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) s[e] += v[e];
+            }
+        }
     }
-    if (part) part[blockIdx.x * N + n] = s;
+    if (!part) return;
+#pragma unroll
+    for (int e = 0; e < V; ++e) join[threadIdx.x * V + e] = s[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < ct * V; i += 256) {
+        float t = 0.f;
+        for (int j = 0; j < rgs; ++j) t += join[j * ct * V + i];
+        const long col = (long)blockIdx.y * ct * V + i;
+        if (col < N) part[blockIdx.x * N + col] = t;
+    }
 }
 
 // Tile and split of one product.
@@ -511,7 +545,21 @@ int gemm_by_order(const GemmArgs& a, bool akc, bool bkc, float* ws, hipStream_t 
     return akc ? (bkc ? gemm<T, true, true>(a, ws, s) : gemm<T, true, false>(a, ws, s)) : gemm<T, false, false>(a, ws, s);
 }
 
-long dz_groups(long M, long N) { return M < 512 ? M : 512; }
+// threads per row of the dz kernel, workgroups along the rows (at least four rows a thread where there are that many) and
+// along the columns
+struct DzShape { int ct; long groups, blocks; };
+DzShape dz_shape(int es, long M, long N) {
+    const long nvec = (N * es + 15) / 16;
+    DzShape d;
+    d.ct = 1;
+    while (d.ct < 256 && d.ct < nvec) d.ct *= 2;
+    d.blocks = (nvec + d.ct - 1) / d.ct;
+    const long rows = (M + 256 / d.ct - 1) / (256 / d.ct);
+    d.groups = (rows + 3) / 4;
+    const long most = d.blocks < 1024 ? 1024 / d.blocks : 1;
+    if (d.groups > most) d.groups = most;
+    return d;
+}
 
 }  // namespace
 
@@ -529,23 +577,25 @@ long gemm_ws_floats(int dtype, long M, long N, long K) {
     return n;
 }
 
-long linear_dz_ws_floats(long M, long N) { return dz_groups(M, N) * N; }
+long linear_dz_ws_floats(int dtype, long M, long N) { return dz_shape(dtype == LDM_BF16 ? 2 : 4, M, N).groups * N; }
 
-int launch_linear_dz(int dtype, const void* dy, long lddy, const void* pre, long ldp, void* dz, long lddz, float* db, float* ws,
-                     long M, long N, int act, hipStream_t s) {
-    const long G = dz_groups(M, N);
+template <typename T>
+static int dz_launch(const void* dy, long lddy, const void* pre, long ldp, void* dz, long lddz, float* db, float* ws, long M,
+                     long N, int act, hipStream_t s) {
+    const DzShape d = dz_shape(sizeof(T), M, N);
+    LDM_REQUIRE(d.blocks <= 65535, "too many columns for one launch");
     if (M > 0 && (act != LIN_NONE || db)) {
-        const dim3 grid((unsigned)G, (unsigned)((N + 255) / 256));
-        if (dtype == LDM_BF16)
-            linear_dz_kernel<__bf16><<<grid, 256, 0, s>>>((const __bf16*)dy, lddy, (const __bf16*)pre, ldp, (__bf16*)dz, lddz,
-                                                          db ? ws : nullptr, M, N, act);
-        else
-            linear_dz_kernel<float><<<grid, 256, 0, s>>>((const float*)dy, lddy, (const float*)pre, ldp, (float*)dz, lddz,
-                                                         db ? ws : nullptr, M, N, act);
+        linear_dz_kernel<T><<<dim3((unsigned)d.groups, (unsigned)d.blocks), 256, 0, s>>>(
+            (const T*)dy, lddy, (const T*)pre, ldp, (T*)dz, lddz, db ? ws : nullptr, M, N, act, d.ct);
         LDM_HIP(hipGetLastError());
     }
     if (!db) return LDM_OK;
-    return launch_colsum(ws, (int)G, (int)N, 1, db, nullptr, s);
+    return launch_colsum(ws, (int)d.groups, (int)N, 1, db, nullptr, s);
+}
+int launch_linear_dz(int dtype, const void* dy, long lddy, const void* pre, long ldp, void* dz, long lddz, float* db, float* ws,
+                     long M, long N, int act, hipStream_t s) {
+    return dtype == LDM_BF16 ? dz_launch<__bf16>(dy, lddy, pre, ldp, dz, lddz, db, ws, M, N, act, s)
+                             : dz_launch<float>(dy, lddy, pre, ldp, dz, lddz, db, ws, M, N, act, s);
 }
 
 }  // namespace ldm

@@ -6,65 +6,51 @@
 // Angles: the product of a position (below 2^29) and an f32 frequency is exact in f64; it is reduced to a fraction of a
 // turn in f64 and only that fraction goes through f32 sine and cosine, so far positions lose nothing.
 #include "blocks.h"
+#include "vec.h"
 
 namespace ldm {
 
 namespace {
 
-template <typename T> struct RoVec;
-template <> struct RoVec<float> {
-    static constexpr int N = 4;
-    typedef float V __attribute__((ext_vector_type(4), aligned(4)));
-    typedef float F __attribute__((ext_vector_type(4)));
-};
-template <> struct RoVec<__bf16> {
-    static constexpr int N = 8;
-    typedef __bf16 V __attribute__((ext_vector_type(8), aligned(2)));
-    typedef float F __attribute__((ext_vector_type(8)));
-};
-
-// n (<= N) elements at p; zero behind them
-template <typename T>
-__device__ __forceinline__ void ro_load(const T* p, int n, float* o) {
-    constexpr int N = RoVec<T>::N;
-    if (n >= N) {
-        const typename RoVec<T>::F v = __builtin_convertvector(*(const typename RoVec<T>::V*)p, typename RoVec<T>::F);
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = v[e];
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = e < n ? (float)p[e] : 0.f;
-    }
-}
-template <typename T>
-__device__ __forceinline__ void ro_store(T* p, int n, const float* o) {
-    constexpr int N = RoVec<T>::N;
-    if (n >= N) {
-        typename RoVec<T>::F v;
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = o[e];
-        *(typename RoVec<T>::V*)p = __builtin_convertvector(v, typename RoVec<T>::V);
-    } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (e < n) p[e] = (T)o[e];
-    }
+// sine and cosine of a fraction of a turn: the nearest quarter is taken off in f64, the rest (at most an eighth, so that
+// its rounding to f32 is 2^-28 of a turn) goes through the Taylor series up to x^9 and x^10, which |x| <= pi / 4 leaves
+// exact to 2e-9
+__device__ __forceinline__ void turn_sincos(double turns, float& sn, float& cs) {
+    const double q4 = turns * 4.0, q = rint(q4);
+    const float x = (float)(q4 - q) * 1.57079632679489662f;
+    // the quarter modulo four: a double of this size holds it exactly
+    const int k = (int)(q - 4.0 * rint(q * 0.25));
+    const float y = x * x;
+    float s = __builtin_fmaf(y, 2.7557319224e-6f, -1.9841269841e-4f);
+    s = __builtin_fmaf(y, s, 8.3333333333e-3f);
+    s = __builtin_fmaf(y, s, -1.6666666667e-1f);
+    s = __builtin_fmaf(x * y, s, x);
+    float c = __builtin_fmaf(y, -2.7557319224e-7f, 2.4801587302e-5f);
+    c = __builtin_fmaf(y, c, -1.3888888889e-3f);
+    c = __builtin_fmaf(y, c, 4.1666666667e-2f);
+    c = __builtin_fmaf(y, c, -0.5f);
+    c = __builtin_fmaf(y, c, 1.0f);
+    const float a = (k & 1) ? c : s, b = (k & 1) ? s : c;
+    sn = (k & 2) ? -a : a;
+    cs = ((k + 1) & 2) ? -b : b;
 }
 
 template <typename T, bool INTER>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
-    constexpr int N = RoVec<T>::N;
+    constexpr int N = RowVec<T>::N;
     const int local = threadIdx.x / a.nchunk, chunk = threadIdx.x - local * a.nchunk;
-    const long token = (long)blockIdx.x * a.tpb + local;
+    // the head groups of the same tokens follow each other, so that a token's heads are read at about the same time
+    const unsigned blk = blockIdx.x / a.groups, grp = blockIdx.x - blk * a.groups;
+    const long token = (long)blk * a.tpb + local;
     if (local >= a.tpb || token >= a.tokens) return;
     const unsigned b = (unsigned)token / (unsigned)a.N, n = (unsigned)token - b * (unsigned)a.N;
 
     // the chunk's two vectors: element offsets and counts
     int e0, e1, n0, n1;
-    float cs[N], sn[N];
     const bool rot = chunk < a.nrot;
+    const int j0 = chunk * N;
     if (rot) {
-        const int j0 = chunk * N, np = a.P - j0 < N ? a.P - j0 : N;
+        const int np = a.P - j0 < N ? a.P - j0 : N;
         if constexpr (INTER) {
             e0 = 2 * j0;
             n0 = 2 * np < N ? 2 * np : N;
@@ -75,20 +61,6 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
             e1 = a.P + j0;
             n0 = n1 = np;
         }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int j = j0 + i < a.P ? j0 + i : a.P - 1;
-            int ax = 0;
-#pragma unroll
-            for (int k = 0; k < 3; ++k) ax += j >= a.sec_end[k];
-            const long po = (long)b * a.pos_sb + (long)ax * a.pos_sa + (long)n * a.pos_sn;
-            const double p = a.pos_dtype == 0 ? (double)((const int*)a.pos)[po]
-                             : a.pos_dtype == 1 ? (double)((const long*)a.pos)[po] : (double)((const float*)a.pos)[po];
-            const double turns = p * (double)a.inv_freq[j] * 0.15915494309189533577;
-            const float f = (float)(turns - rint(turns));
-            sincospif(2.0f * f, &sn[i], &cs[i]);
-            if (a.inverse) sn[i] = -sn[i];
-        }
     } else {
         const int c0 = 2 * a.P + (chunk - a.nrot) * 2 * N, np = a.D - c0;
         e0 = c0;
@@ -96,37 +68,79 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
         n0 = np < N ? np : N;
         n1 = np - n0 < N ? np - n0 : N;
     }
-    int h = blockIdx.y * a.hpg;
-    const int hend = h + a.hpg < a.H[0] + a.H[1] ? h + a.hpg : a.H[0] + a.H[1];
-    for (; h < hend; ++h) {
-        const int w = h >= a.H[0];
-        const int hh = w ? h - a.H[0] : h;
-        const T* src = (const T*)a.in[w] + ((long)b * a.isb[w] + (long)n * a.isn[w] + (long)hh * a.ish[w]);
-        T* dst = (T*)a.out[w] + ((long)b * a.osb[w] + (long)n * a.osn[w] + (long)hh * a.osh[w]);
-        float u[N], v[N];
-        ro_load<T>(src + e0, n0, u);
-        ro_load<T>(src + e1, n1, v);
-        if (rot) {
-            if constexpr (INTER) {
+    // four heads at a time: the next four are on their way while these are turned, the first while the angles are taken
+    const int heads = a.H[0] + a.H[1], h0 = grp * a.hpg, hend = h0 + a.hpg < heads ? h0 + a.hpg : heads;
+    typename RowVec<T>::R nu[4], nv[4];
+    auto fetch = [&](int h) {
 #pragma unroll
-                for (int i = 0; i < N / 2; ++i) {
-                    const float x0 = u[2 * i], y0 = u[2 * i + 1], x1 = v[2 * i], y1 = v[2 * i + 1];
-                    u[2 * i] = x0 * cs[i] - y0 * sn[i];
-                    u[2 * i + 1] = x0 * sn[i] + y0 * cs[i];
-                    v[2 * i] = x1 * cs[N / 2 + i] - y1 * sn[N / 2 + i];
-                    v[2 * i + 1] = x1 * sn[N / 2 + i] + y1 * cs[N / 2 + i];
-                }
-            } else {
+        for (int d = 0; d < 4; ++d) {
+            if (h + d >= hend) continue;
+            const int w = h + d >= a.H[0], hh = w ? h + d - a.H[0] : h + d;
+            const T* src = (const T*)a.in[w] + ((long)b * a.isb[w] + (long)n * a.isn[w] + (long)hh * a.ish[w]);
+            nu[d] = row_load<T>(src + e0, n0);
+            nv[d] = row_load<T>(src + e1, n1);
+        }
+    };
+    fetch(h0);
+    float cs[N], sn[N];
+    if (rot) {
+        // the token's position on each axis and the pairs' frequencies, every load before the first use
+        double pos[4];
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float x = u[i], y = v[i];
-                    u[i] = x * cs[i] - y * sn[i];
-                    v[i] = x * sn[i] + y * cs[i];
+        for (int k = 0; k < 4; ++k) {
+            const long po = (long)b * a.pos_sb + (long)(k < a.axes ? k : 0) * a.pos_sa + (long)n * a.pos_sn;
+            pos[k] = a.pos_dtype == 0 ? (double)((const int*)a.pos)[po]
+                     : a.pos_dtype == 1 ? (double)((const long*)a.pos)[po] : (double)((const float*)a.pos)[po];
+        }
+        float f[N];
+#pragma unroll
+        for (int i = 0; i < N; i += 4) row_floats<float>(row_load<float>(a.inv_freq + j0 + i, a.P - j0 - i), f + i);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int j = j0 + i;
+            const double p = j < a.sec_end[0] ? pos[0] : j < a.sec_end[1] ? pos[1] : j < a.sec_end[2] ? pos[2] : pos[3];
+            const double turns = p * (double)f[i] * 0.15915494309189533577;
+            turn_sincos(a.inverse ? -turns : turns, sn[i], cs[i]);
+        }
+    }
+    for (int h = h0; h < hend; h += 4) {
+        typename RowVec<T>::R lu[4], lv[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            lu[d] = nu[d];
+            lv[d] = nv[d];
+        }
+        fetch(h + 4);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            if (h + d >= hend) continue;
+            const int w = h + d >= a.H[0], hh = w ? h + d - a.H[0] : h + d;
+            T* dst = (T*)a.out[w] + ((long)b * a.osb[w] + (long)n * a.osn[w] + (long)hh * a.osh[w]);
+            float u[N], v[N];
+            row_floats<T>(lu[d], u);
+            row_floats<T>(lv[d], v);
+            if (rot) {
+                if constexpr (INTER) {
+#pragma unroll
+                    for (int i = 0; i < N / 2; ++i) {
+                        const float x0 = u[2 * i], y0 = u[2 * i + 1], x1 = v[2 * i], y1 = v[2 * i + 1];
+                        u[2 * i] = x0 * cs[i] - y0 * sn[i];
+                        u[2 * i + 1] = x0 * sn[i] + y0 * cs[i];
+                        v[2 * i] = x1 * cs[N / 2 + i] - y1 * sn[N / 2 + i];
+                        v[2 * i + 1] = x1 * sn[N / 2 + i] + y1 * cs[N / 2 + i];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const float x = u[i], y = v[i];
+                        u[i] = x * cs[i] - y * sn[i];
+                        v[i] = x * sn[i] + y * cs[i];
+                    }
                 }
             }
+            row_store<T>(dst + e0, n0, u);
+            row_store<T>(dst + e1, n1, v);
         }
-        ro_store<T>(dst + e0, n0, u);
-        ro_store<T>(dst + e1, n1, v);
     }
 }
 
@@ -138,9 +152,17 @@ int launch_rope(int dtype, int interleaved, RopeArgs a, hipStream_t s) {
     a.nrot = (a.P + N - 1) / N;
     a.nchunk = a.nrot + (a.D - 2 * a.P + 2 * N - 1) / (2 * N);
     a.tpb = 256 / a.nchunk;
+    // a group of heads per workgroup, all of them where the tokens alone give eight workgroups per CU: the angles are taken
+    // once for a group.  2 x 8192 tokens, 20 heads of 128 in f32: 76.8 us in two groups of ten, 80.4 in one, 78.1 in four
+    // (and 100.6 with a workgroup per head); one token, 8 heads of 64: 5.2 us in four groups, 7.4 in one
     const int heads = a.H[0] + a.H[1];
-    a.hpg = heads < 8 ? heads : 8;
-    const dim3 grid((unsigned)((a.tokens + a.tpb - 1) / a.tpb), (unsigned)((heads + a.hpg - 1) / a.hpg));
+    const long blocks = (a.tokens + a.tpb - 1) / a.tpb;
+        long groups = 2048 / blocks;
+    groups = groups < 1 ? 1 : groups > (heads + 1) / 2 ? (heads + 1) / 2 : groups;
+    a.hpg = (int)((heads + groups - 1) / groups);
+    a.groups = (unsigned)((heads + a.hpg - 1) / a.hpg);
+    LDM_REQUIRE(blocks * a.groups < (1L << 31), "too many tokens and heads for one launch");
+    const unsigned grid = (unsigned)(blocks * a.groups);
     if (dtype == LDM_BF16) {
         if (interleaved) rope_kernel<__bf16, true><<<grid, 256, 0, s>>>(a);
         else rope_kernel<__bf16, false><<<grid, 256, 0, s>>>(a);
