@@ -128,26 +128,36 @@ def batchnorm_act(h: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor, act:
 # they record no autograd graph, so a tensor that requires a gradient is refused while gradients are recorded.  Workspaces
 # come from torch's allocator for the one call, so calls on several streams and captured graphs do not share them.
 _TD = {torch.bfloat16: _lib.LDM_BF16, torch.float32: _lib.LDM_F32}
+_F32 = (torch.float32,)
+_REAL = (torch.float32, torch.bfloat16, torch.float16, torch.float64)
 LINEAR_ACTS = {None: 0, "none": 0, "silu": 1, "relu": 2, "gelu": 3}
 ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
 _POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+_PACK12, _PACK3 = struct.Struct("12l").pack, struct.Struct("3l").pack
+
+# torch.cuda.current_stream() builds a Stream object (2.6 us, as much as a launch); the raw handle is what is needed
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _data(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _check(name: str, t, like: Optional[torch.Tensor] = None, dtypes=(torch.bfloat16, torch.float32)) -> None:
-    """A device tensor of one of `dtypes`, on `like`'s device, that needs no gradient."""
+def _check(name: str, t, dev: int = -1, dtypes=_TD) -> int:
+    """A device tensor of one of `dtypes`, on device `dev` (-1: any), that needs no gradient.  Returns its device."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a device tensor")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} is {t.dtype}, expected one of {tuple(str(d) for d in dtypes)}")
-    if like is not None and t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+    d = t.get_device()
+    if dev >= 0 and d != dev:
+        raise ValueError(f"{name} is on device {d}, expected {dev}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which this operator does not record: call it under "
                          "torch.no_grad() and use the operator's backward function")
+    return d
 
 
 def _rows(name: str, t: torch.Tensor) -> Tuple[int, int]:
@@ -202,7 +212,7 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
 def _check_out(name: str, out: torch.Tensor, shape, like: torch.Tensor, inputs, same: Optional[torch.Tensor] = None) -> None:
     """An output given by the caller: right shape and type, no element twice, apart from the inputs; `same` is an input
     that it may replace, as the very same view."""
-    _check(name, out, like, (like.dtype,))
+    _check(name, out, like.get_device(), (like.dtype,))
     if tuple(out.shape) != tuple(shape):
         raise ValueError(f"{name} has shape {tuple(out.shape)}, expected {tuple(shape)}")
     reach = 1
@@ -217,23 +227,28 @@ def _check_out(name: str, out: torch.Tensor, shape, like: torch.Tensor, inputs, 
             raise ValueError(f"{name} overlaps an input in memory")
 
 
-def _params(name: str, t: Optional[torch.Tensor], n: int, like: torch.Tensor) -> Optional[torch.Tensor]:
-    """n contiguous f32 values on `like`'s device (another floating type is converted), or None."""
+def _params(name: str, t: Optional[torch.Tensor], n: int, dev: int) -> Optional[torch.Tensor]:
+    """n contiguous f32 values on device `dev` (another floating type is converted), or None."""
     if t is None:
         return None
-    _check(name, t, like, (torch.float32, torch.bfloat16, torch.float16, torch.float64))
+    _check(name, t, dev, _REAL)
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must hold {n} values, has shape {tuple(t.shape)}")
     return t if t.dtype is torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
-def _call(fn, device: torch.device, *args) -> None:
-    """One library call on `device` and its current stream (the function's last argument)."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of x's shape, type and device."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _call(fn, dev: int, *args) -> None:
+    """One library call on device `dev` and its current stream (the function's last argument)."""
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(dev))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
     if rc:
         _lib.check(rc)
 
@@ -244,25 +259,25 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     contiguous, leading axes one run of rows: ldm_layer_norm).  weight and bias hold C values and are used in f32.
     Returns y, or (y, mean, rstd) with `stats`: f32 of shape [...], what layer_norm_backward needs.
     `out` may be x itself."""
-    _check("x", x)
+    dev = _check("x", x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x must have a last axis of at least one element")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
     Cc = x.shape[-1]
     rows, xs = _rows("x", x)
-    w, b = _params("weight", weight, Cc, x), _params("bias", bias, Cc, x)
+    w, b = _params("weight", weight, Cc, dev), _params("bias", bias, Cc, dev)
     if out is None:
-        out, ys = torch.empty(x.shape, dtype=x.dtype, device=x.device), Cc
+        out, ys = _like(x), Cc
     else:
         _check_out("out", out, x.shape, x, (w, b), same=x)
         ys = _rows("out", out)[1]
     mean = rstd = None
     if stats:
-        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
         rstd = torch.empty_like(mean)
     if rows:
-        _call(_lib.load().ldm_layer_norm, x.device, _TD[x.dtype], x.data_ptr(), xs, _data(w), _data(b), eps,
+        _call(_lib.load().ldm_layer_norm, dev, _TD[x.dtype], x.data_ptr(), xs, _data(w), _data(b), eps,
               out.data_ptr(), ys, _data(mean), _data(rstd), rows, Cc)
     return (out, mean, rstd) if stats else out
 
@@ -273,34 +288,35 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     """Gradients of layer_norm (ldm_layer_norm_backward): (dx, dweight, dbias), dx in x's type, the parameters' in f32.
     mean and rstd are the forward pass's statistics; `add` (x's shape and type) is added to dx, the gradient that
     reaches x by the residual branch.  param_grads=False (the default without a weight) leaves dweight and dbias None."""
-    _check("x", x)
+    dev = _check("x", x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x must have a last axis of at least one element")
     for name, t in (("dy", dy), ("add", add)):
-        if t is not None:
-            _check(name, t, x, (x.dtype,))
+        if t is not None or name == "dy":
+            _check(name, t, dev, (x.dtype,))
             if t.shape != x.shape:
                 raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(x.shape)}")
     for name, t in (("mean", mean), ("rstd", rstd)):
-        _check(name, t, x, (torch.float32,))
+        _check(name, t, dev, _F32)
         if t.shape != x.shape[:-1] or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous with shape {tuple(x.shape[:-1])}")
     Cc = x.shape[-1]
     rows, xs = _rows("x", x)
     dys = _rows("dy", dy)[1]
     adds = 0 if add is None else _rows("add", add)[1]
-    w = _params("weight", weight, Cc, x)
+    w = _params("weight", weight, Cc, dev)
     if param_grads is None:
         param_grads = weight is not None
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _like(x)
     lib = _lib.load()
+    code = _TD[x.dtype]
     dw = db = ws = None
     if param_grads:
-        dw = torch.empty(Cc, dtype=torch.float32, device=x.device)
+        dw = x.new_empty(Cc, dtype=torch.float32)
         db = torch.empty_like(dw)
-        ws = torch.empty(lib.ldm_layer_norm_ws_floats(_TD[x.dtype], rows, Cc), dtype=torch.float32, device=x.device)
+        ws = x.new_empty(lib.ldm_layer_norm_ws_floats(code, rows, Cc), dtype=torch.float32)
     if rows or param_grads:
-        _call(lib.ldm_layer_norm_backward, x.device, _TD[x.dtype], dy.data_ptr(), dys, x.data_ptr(), xs, _data(add), adds,
+        _call(lib.ldm_layer_norm_backward, dev, code, dy.data_ptr(), dys, x.data_ptr(), xs, _data(add), adds,
               mean.data_ptr(), rstd.data_ptr(), _data(w), dx.data_ptr(), Cc, _data(dw), _data(db), _data(ws), rows, Cc)
     return dx, dw, db
 
@@ -326,53 +342,56 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, in
     layout "half" pairs (j, P + j), "interleaved" (2j, 2j + 1); elements behind 2P pass through.
     inverse=True turns back: applied to the gradients of the outputs it gives the gradients of q and k.
     Returns (q', k'), or q' if k is None; `out` = (q', k') or q' to write to, which may be the inputs themselves."""
-    _check("q", q)
+    dev = _check("q", q)
     if q.dim() != 4:
         raise ValueError("q must be [B, N, heads, D]")
     B, N, Hq, D = q.shape
     Hk = 0
+    sq = q.stride()
+    sk = (0, 0, 0, 1)
     if k is not None:
-        _check("k", k, q, (q.dtype,))
-        if k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != D:
+        _check("k", k, dev, (q.dtype,))
+        if k.dim() != 4 or k.shape[0] != B or k.shape[1] != N or k.shape[3] != D:
             raise ValueError(f"k must be [{B}, {N}, heads, {D}], has shape {tuple(k.shape)}")
-        Hk = k.shape[2]
-    for name, t in (("q", q), ("k", k)):
-        if t is not None and (t.shape[2] < 1 or D < 1 or (D > 1 and t.stride(3) != 1)):
-            raise ValueError(f"{name} needs at least one head and contiguous head vectors")
-    _check("inv_freq", inv_freq, q, (torch.float32,))
+        Hk, sk = k.shape[2], k.stride()
+    if D < 1 or Hq < 1 or (k is not None and Hk < 1) or (D > 1 and (sq[3] != 1 or sk[3] != 1)):
+        raise ValueError("q and k need at least one head and contiguous head vectors")
+    _check("inv_freq", inv_freq, dev, _F32)
     if inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous vector")
     P = inv_freq.shape[0]
-    sec = (P,) if sections is None else tuple(int(n) for n in sections)
+    sec = (P,) if sections is None else tuple(sections)
     if not 1 <= len(sec) <= 4 or min(sec) < 0 or sum(sec) != P or P < 1 or 2 * P > D:
         raise ValueError(f"sections {sec} must hold one to four counts that add up to inv_freq's {P} pairs, at most D / 2")
-    _check("positions", positions, q, tuple(_POS_TYPES))
-    if positions.dim() not in (2, 3) or tuple(positions.shape[-2:]) != (len(sec), N) or \
-            (positions.dim() == 3 and positions.shape[0] != B):
+    _check("positions", positions, dev, _POS_TYPES)
+    ps, pp = positions.shape, positions.stride()
+    if len(ps) == 2:
+        ps, pp = (B,) + tuple(ps), (0,) + pp
+    if len(ps) != 3 or ps[0] != B or ps[1] != len(sec) or ps[2] != N:
         raise ValueError(f"positions must be [{len(sec)}, {N}] or [{B}, {len(sec)}, {N}], has shape {tuple(positions.shape)}")
     if layout not in ROPE_LAYOUTS:
         raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+    ok = None
     if out is None:
-        oq = torch.empty((B, N, Hq, D), dtype=q.dtype, device=q.device)
-        ok = None if k is None else torch.empty((B, N, Hk, D), dtype=q.dtype, device=q.device)
+        oq = _like(q)
+        so = oq.stride()
+        st = sq[:3] + sk[:3] + so[:3]
+        if k is not None:
+            ok = _like(k)
+            so = ok.stride()
+        st += so[:3]
     else:
         oq, ok = (out, None) if k is None else out
         _check_out("out[0]", oq, q.shape, q, (k, positions, inv_freq), same=q)
         if k is not None:
             _check_out("out[1]", ok, k.shape, q, (q, oq, positions, inv_freq), same=k)
-            if D > 1 and ok.stride(3) != 1:
-                raise ValueError("out[1] needs contiguous head vectors")
-        if D > 1 and oq.stride(3) != 1:
-            raise ValueError("out[0] needs contiguous head vectors")
-    st = []
-    for t in (q, k, oq, ok):
-        st += (0, 0, 0) if t is None else t.stride()[:3]
-    ps = positions.stride() if positions.dim() == 3 else (0,) + positions.stride()
-    if q.numel():
-        _call(_lib.load().ldm_rope, q.device, _TD[q.dtype], q.data_ptr(), _data(k), oq.data_ptr(), _data(ok),
-              struct.pack("12l", *st), B, N, Hq, Hk, D, positions.data_ptr(), _POS_TYPES[positions.dtype],
-              struct.pack("3l", *ps), inv_freq.data_ptr(), struct.pack(f"{len(sec)}i", *sec), len(sec),
-              ROPE_LAYOUTS[layout], int(inverse))
+        if D > 1 and (oq.stride(3) != 1 or (ok is not None and ok.stride(3) != 1)):
+            raise ValueError("the outputs need contiguous head vectors")
+        st = sq[:3] + sk[:3] + oq.stride()[:3] + (oq if ok is None else ok).stride()[:3]
+    if B and N:
+        _call(_lib.load().ldm_rope, dev, _TD[q.dtype], q.data_ptr(), _data(k), oq.data_ptr(), _data(ok),
+              _PACK12(*st), B, N, Hq, Hk, D, positions.data_ptr(), _POS_TYPES[positions.dtype], _PACK3(*pp),
+              inv_freq.data_ptr(), struct.pack(f"{len(sec)}i", *sec), len(sec), ROPE_LAYOUTS[layout], bool(inverse))
     return oq if k is None else (oq, ok)
 
 
@@ -386,16 +405,16 @@ def _weight_order(weight: torch.Tensor) -> Tuple[int, int]:
     raise ValueError("weight must be contiguous along one of its axes")
 
 
-def _check_linear(x: torch.Tensor, weight: torch.Tensor, act: Optional[str]) -> Tuple[int, int]:
-    _check("x", x)
-    _check("weight", weight, x, (x.dtype,))
+def _check_linear(x: torch.Tensor, weight: torch.Tensor, act: Optional[str]) -> Tuple[int, int, int]:
+    dev = _check("x", x)
+    _check("weight", weight, dev, (x.dtype,))
     if weight.dim() != 2 or min(weight.shape) < 1:
         raise ValueError("weight must be [K, N] with K, N >= 1")
     if x.dim() < 1 or x.shape[-1] != weight.shape[0]:
         raise ValueError(f"x must be [..., {weight.shape[0]}], has shape {tuple(x.shape)}")
     if act not in LINEAR_ACTS:
         raise ValueError(f"act must be one of {sorted(a for a in LINEAR_ACTS if a)}, got {act!r}")
-    return weight.shape[0], weight.shape[1]
+    return dev, weight.shape[0], weight.shape[1]
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
@@ -405,29 +424,29 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     like a convolution's; act None, 'silu', 'relu' or 'gelu' (the exact one).  Products accumulate in f32.
     Returns the output in x's type, or (output, z) with save_pre: z, the value before the activation, is what
     linear_backward needs with one.  `out` may be res itself."""
-    K, N = _check_linear(x, weight, act)
+    dev, K, N = _check_linear(x, weight, act)
     M, ldx = _rows("x", x)
     order, ldw = _weight_order(weight)
-    b = _params("bias", bias, N, x)
+    b = _params("bias", bias, N, dev)
     shape = x.shape[:-1] + (N,)
     ldr = 0
     if res is not None:
-        _check("res", res, x, (x.dtype,))
+        _check("res", res, dev, (x.dtype,))
         if res.shape != shape:
             raise ValueError(f"res has shape {tuple(res.shape)}, expected {tuple(shape)}")
         ldr = _rows("res", res)[1]
     if out is None:
-        out, ldo = torch.empty(shape, dtype=x.dtype, device=x.device), N
+        out, ldo = x.new_empty(shape), N
     else:
         _check_out("out", out, shape, x, (x, weight, b), same=res)
         ldo = _rows("out", out)[1]
-    pre = torch.empty(shape, dtype=x.dtype, device=x.device) if save_pre else None
+    pre = torch.empty_like(out, memory_format=torch.contiguous_format) if save_pre else None
     if M:
         lib = _lib.load()
         code = _TD[x.dtype]
         n = lib.ldm_linear_ws_floats(code, M, K, N, order)
-        ws = torch.empty(n, dtype=torch.float32, device=x.device) if n > 0 else None
-        _call(lib.ldm_linear, x.device, code, x.data_ptr(), ldx, weight.data_ptr(), ldw, order, _data(b), _data(res), ldr,
+        ws = x.new_empty(n, dtype=torch.float32) if n > 0 else None
+        _call(lib.ldm_linear, dev, code, x.data_ptr(), ldx, weight.data_ptr(), ldw, order, _data(b), _data(res), ldr,
               LINEAR_ACTS[act], out.data_ptr(), ldo, _data(pre), N, M, K, N, _data(ws))
     return (out, pre) if save_pre else out
 
@@ -438,7 +457,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre
     before the activation and so of `res` (dy itself without an activation); dx = dz W^T; dweight = x^T dz, laid out like
     weight; dbias = column sums of dz, f32.  pre: linear's second output (save_pre), needed with an activation.
     dx, dweight or dbias False leaves that gradient out (None)."""
-    K, N = _check_linear(x, weight, act)
+    dev, K, N = _check_linear(x, weight, act)
     shape = x.shape[:-1] + (N,)
     code_act = LINEAR_ACTS[act]
     if code_act and pre is None:
@@ -446,25 +465,24 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre
     if not code_act:
         pre = None
     for name, t in (("dy", dy), ("pre", pre)):
-        if t is not None:
-            _check(name, t, x, (x.dtype,))
+        if t is not None or name == "dy":
+            _check(name, t, dev, (x.dtype,))
             if t.shape != shape:
                 raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     M, ldx = _rows("x", x)
     lddy = _rows("dy", dy)[1]
     ldp = 0 if pre is None else _rows("pre", pre)[1]
     order, ldw = _weight_order(weight)
-    dev, td = x.device, x.dtype
-    dz = torch.empty(shape, dtype=td, device=dev) if code_act else dy
-    gx = torch.empty(x.shape, dtype=td, device=dev) if dx else None
+    dz = _like(dy) if code_act else dy
+    gx = _like(x) if dx else None
     gw = None
     if dweight:
-        gw = torch.empty((K, N) if order == 0 else (N, K), dtype=td, device=dev)
-    gb = torch.empty(N, dtype=torch.float32, device=dev) if dbias else None
+        gw = _like(weight if order == 0 else weight.t())
+    gb = x.new_empty(N, dtype=torch.float32) if dbias else None
     lib = _lib.load()
-    code = _TD[td]
+    code = _TD[x.dtype]
     n = lib.ldm_linear_backward_ws_floats(code, M, K, N, order)
-    ws = torch.empty(n, dtype=torch.float32, device=dev) if n > 0 else None
+    ws = x.new_empty(n, dtype=torch.float32) if n > 0 else None
     _call(lib.ldm_linear_backward, dev, code, dy.data_ptr(), lddy, x.data_ptr(), ldx, weight.data_ptr(), ldw, order,
           _data(pre), ldp, code_act, dz.data_ptr() if code_act else 0, N, _data(gx), K, _data(gw), N if order == 0 else K,
           _data(gb), _data(ws), M, K, N)
