@@ -208,15 +208,29 @@ __device__ __forceinline__ void gemm_finish(const GemmArgs& a, long m, long n, f
     }
 }
 __device__ __forceinline__ void gemm_bias(const GemmArgs& a, long n, float (&b)[8]) {
+    const int left = n >= a.N ? 0 : a.N - n < 8 ? (int)(a.N - n) : 8;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) b[e] = a.bias && n + e < a.N ? a.bias[n + e] : 0.f;
+    for (int e = 0; e < 8; e += 4) {
+        if (a.bias) row_floats<float>(row_load<float>(a.bias + n + e, left - e), b + e);
+        else b[e] = b[e + 1] = b[e + 2] = b[e + 3] = 0.f;
+    }
 }
 
+// f(0), ..., f(N_ - 1) with the index a constant of the type
 template <int I, int N_, typename Fn> __device__ __forceinline__ void gemm_for(Fn&& f) {
     if constexpr (I < N_) {
         f(std::integral_constant<int, I>{});
         gemm_for<I + 1, N_>(f);
     }
+}
+
+// behind an explicit wait: the compiler takes the value as it stands
+template <typename V> __device__ __forceinline__ void gemm_landed(V& v) { asm volatile("" : "+v"(v)); }
+// marks v as the one of branch I: branches that pick from a register array by a run-time index stay apart (merged, they
+// would make the compiler keep the array in memory)
+template <int I, typename V> __device__ __forceinline__ void gemm_pick(V& v) { asm volatile("; %1" : "+v"(v) : "n"(I)); }
+__device__ __forceinline__ void gemm_mfma_in_place(f32x4& c, const u32x4& a, const u32x4& b) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 
 // DMA: both operands have 16-byte aligned rows whose length along the contiguous index is a multiple of a piece, and come
@@ -269,7 +283,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     }
     u32x4 ra[DMA ? 1 : NP], rb[DMA ? 1 : NP];
     // asks for piece q of both operands of step t (steps behind the last one: zeros, without a memory access)
-    auto request = [&](int t, int q) {
+    auto request = [&](int t, int q) __attribute__((always_inline)) {
         const int kleft = klen - t * BK;
         if constexpr (DMA) {
             const auto sa = __builtin_amdgcn_make_buffer_rsrc((void*)(ap + t * astep), 0, 0x80000000, 0x00020000);
@@ -286,7 +300,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         }
     };
     // step t's pieces of this wave are in LDS
-    auto land = [&](int t) {
+    auto land = [&](int t) __attribute__((always_inline)) {
         if constexpr (DMA) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         } else {
@@ -301,10 +315,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     };
 
     f32x4 acc[F][F];       // [row fragment][column fragment]
-#pragma unroll
-    for (int i = 0; i < F; ++i)
-#pragma unroll
-        for (int j = 0; j < F; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    gemm_for<0, F * F>([&](auto I) __attribute__((always_inline)) { acc[I / F][I % F] = f32x4{0.f, 0.f, 0.f, 0.f}; });
     GemmFrag<T, AKC> fa[2][F];
     GemmFrag<T, BKC> fb[2][F];
     unsigned aa[2], bb[2];      // fragment addresses of the two halves, in the stage that is read next
@@ -313,41 +324,42 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         aa[s] = lds0 + OA::base(lane, wm, s);
         bb[s] = lds0 + 2 * STAGE + OB::base(lane, wn, s);
     }
-    auto landed = [&](auto S) {
+    auto landed = [&](auto S) __attribute__((always_inline)) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-        for (int i = 0; i < F; ++i) { fa[S][i].landed(); fb[S][i].landed(); }
+        gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
+            fa[S][I].landed();
+            fb[S][I].landed();
+        });
     };
     // products of half S, with the reads of the other half's fragments (and a step's requests) between them
-    auto multiply = [&](auto S, auto REQ, int t) {
+    auto multiply = [&](auto S, auto REQ, int t) __attribute__((always_inline)) {
         constexpr int s = S, r = 1 - S;
-        gemm_for<0, F>([&](auto I) {
+        gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
             constexpr int i = I;
             if constexpr (REQ) {
                 if constexpr (i < NP) request(t + 2, i);
             }
             OA::template read<i, r>(fa[r][i], aa[r]);
             OB::template read<i, r>(fb[r][i], bb[r]);
-#pragma unroll
-            for (int j = 0; j < F; ++j) {
+            gemm_for<0, F>([&](auto J) __attribute__((always_inline)) {
+                constexpr int j = J;
                 if constexpr (F == 8) {
                     // in place by constraint: with all 256 accumulators live the compiler's own choice moves them about
-                    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0"
-                                 : "+a"(acc[i][j]) : "v"(fb[s][j].bits()), "v"(fa[s][i].bits()));
+                    gemm_mfma_in_place(acc[i][j], fb[s][j].bits(), fa[s][i].bits());
                 } else if constexpr (ES == 2) {
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fb[s][j].bits()),
                                                                         __builtin_bit_cast(bf16x8, fa[s][i].bits()),
                                                                         acc[i][j], 0, 0, 0);
                 } else {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[s][j].f32(q), fa[s][i].f32(q), acc[i][j], 0, 0, 0);
+                    gemm_for<0, 4>([&](auto Q) __attribute__((always_inline)) {
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[s][j].f32(Q), fa[s][i].f32(Q), acc[i][j], 0, 0, 0);
+                    });
                 }
-            }
+            });
             __builtin_amdgcn_sched_barrier(0);
         });
     };
-    auto step = [&](int t) {
+    auto step = [&](int t) __attribute__((always_inline)) {
         multiply(std::integral_constant<int, 0>{}, std::false_type{}, t);
         landed(std::integral_constant<int, 1>{});
         land(t + 1);
@@ -366,7 +378,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         for (int q = 0; q < NP; ++q) request(1, q);
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        gemm_for<0, F>([&](auto I) {
+        gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
             OA::template read<I, 0>(fa[0][I], aa[0]);
             OB::template read<I, 0>(fb[0][I], bb[0]);
         });
@@ -378,38 +390,124 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     if constexpr (F == 8) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
     __syncthreads();
 
-    // epilogue: 16 rows at a time through LDS, so that memory sees whole rows
-    constexpr int ROW = F * 64 + 16, LPR = F * 2, RPP = 64 / LPR;       // bytes of a row, lanes per row, rows per pass
+    // epilogue: 16 rows at a time through LDS, so that memory sees whole rows.  One copy of the code for all row fragments
+    // (unrolled over them it would not fit the instruction cache), and no load between the stores: loads and stores count
+    // together and in order, so a wait for one would be a wait for every store before it (256 x 256 outputs without a
+    // residual: 11.7 us with such waits, _EPI_ without).
+    constexpr int ROW = F * 64 + 16, LPR = F * 2, RPP = 64 / LPR, P = 16 / RPP;     // bytes of a row, lanes per row, rows
+    typedef typename RowVec<T>::R R;                                               // per pass, passes
+    constexpr int H = 16 / RowVec<T>::N / 2;                                       // vectors of T in eight columns
     char* tr = smem + wave * 16 * ROW;
     const int g = lane >> 4, l15 = lane & 15, c = (lane % LPR) * 8, r0 = lane / LPR;
-    const long n = n0 + wn + c;
-    float bias[8];
-    gemm_bias(a, n, bias);
-    const long np = (a.N + 7) & ~7L;
-    // one copy of this code for all row fragments: unrolled over them it would not fit the instruction cache
-#pragma unroll 1
-    for (int i = 0; i < F; ++i) {
-        gemm_for<0, F>([&](auto I) {
-            if (i == I) {
-#pragma unroll
-                for (int j = 0; j < F; ++j) *(f32x4*)(tr + l15 * ROW + j * 64 + g * 16) = acc[I][j];
-            }
+    const long n = n0 + wn + c, mw = m0 + wm + r0;
+    auto spill = [&](int i) __attribute__((always_inline)) {
+        gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
+            if (i == I) gemm_for<0, F>([&](auto J) __attribute__((always_inline)) {
+                f32x4 v = acc[I][J];
+                gemm_pick<I>(v);
+                *(f32x4*)(tr + l15 * ROW + J * 64 + g * 16) = v;
+            });
         });
+    };
+    auto take = [&](int p, float (&v)[8]) {
+        const f32x4 lo = *(const f32x4*)(tr + (p * RPP + r0) * ROW + c * 4), hi = *(const f32x4*)(tr + (p * RPP + r0) * ROW + c * 4 + 16);
 #pragma unroll
-        for (int p = 0; p < 16 / RPP; ++p) {
-            const int row = p * RPP + r0;
-            const long m = m0 + wm + i * 16 + row;
-            const f32x4 lo = *(const f32x4*)(tr + row * ROW + c * 4), hi = *(const f32x4*)(tr + row * ROW + c * 4 + 16);
-            if (m >= a.M || n >= a.N) continue;
-            if (a.part) {
-                float* o = a.part + ((long)z * a.M + m) * np + n;
-                *(f32x4*)o = lo;
-                *(f32x4*)(o + 4) = hi;
-            } else {
-                float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                gemm_finish<T>(a, m, n, v, bias);
+        for (int e = 0; e < 4; ++e) {
+            v[e] = lo[e];
+            v[4 + e] = hi[e];
+        }
+    };
+    if (a.part) {
+        const long np = (a.N + 7) & ~7L;
+        float* part = a.part + (long)z * a.M * np;
+#pragma unroll 1
+        for (int i = 0; i < F; ++i) {
+            spill(i);
+            float v[P][8];
+#pragma unroll
+            for (int p = 0; p < P; ++p) take(p, v[p]);
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const long m = mw + i * 16 + p * RPP;
+                if (m >= a.M || n >= a.N) continue;
+                *(f32x4*)(part + m * np + n) = f32x4{v[p][0], v[p][1], v[p][2], v[p][3]};
+                *(f32x4*)(part + m * np + n + 4) = f32x4{v[p][4], v[p][5], v[p][6], v[p][7]};
             }
         }
+        return;
+    }
+    float bias[8];
+    gemm_bias(a, n, bias);
+    if (n0 + TILE > a.N) {
+        // the last tile column, where a piece of eight may be cut: guarded, piece by piece
+#pragma unroll 1
+        for (int i = 0; i < F; ++i) {
+            spill(i);
+#pragma unroll 1
+            for (int p = 0; p < P; ++p) {
+                float v[8];
+                take(p, v);
+                const long m = mw + i * 16 + p * RPP;
+                if (m < a.M && n < a.N) gemm_finish<T>(a, m, n, v, bias);
+            }
+        }
+        return;
+    }
+    R res[F][P * H];
+    if (a.res) {
+        gemm_for<0, F * P * H>([&](auto I) __attribute__((always_inline)) {
+            constexpr int i = I / (P * H), p = I / H % P, h = I % H;
+            const long m = mw + i * 16 + p * RPP < a.M ? mw + i * 16 + p * RPP : a.M - 1;
+            res[i][p * H + h] = *(const typename RowVec<T>::V*)((const T*)a.res + m * a.ldr + n + h * RowVec<T>::N);
+        });
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    gemm_for<0, 8>([&](auto E) __attribute__((always_inline)) { gemm_landed(bias[E]); });
+    if (a.res) gemm_for<0, F * P * H>([&](auto I) __attribute__((always_inline)) { gemm_landed(res[I / (P * H)][I % (P * H)]); });
+#pragma unroll 1
+    for (int i = 0; i < F; ++i) {
+        spill(i);
+        float v[P][8];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            take(p, v[p]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[p][e] += bias[e];
+        }
+        if (a.res) {
+            gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
+                if (i == I)
+                    gemm_for<0, P * H>([&](auto Q) __attribute__((always_inline)) {
+                        float r[RowVec<T>::N];
+                        R x = res[I][Q];
+                        gemm_pick<I>(x);
+                        row_floats<T>(x, r);
+#pragma unroll
+                        for (int e = 0; e < RowVec<T>::N; ++e) v[Q / H][(Q % H) * RowVec<T>::N + e] += r[e];
+                    });
+            });
+        }
+        const long m = mw + i * 16;
+        auto put = [&](T* out, long ld) __attribute__((always_inline)) {
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                if (m + p * RPP < a.M) {
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+                        row_store<T>(out + (m + p * RPP) * ld + n + h * RowVec<T>::N, RowVec<T>::N, v[p] + h * RowVec<T>::N);
+                }
+        };
+        if (a.pre) put((T*)a.pre, a.ldp);
+        auto activate = [&](auto A) __attribute__((always_inline)) {
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[p][e] = lin_act(v[p][e], A);
+        };
+        if (a.act == LIN_SILU) activate(std::integral_constant<int, LIN_SILU>{});
+        else if (a.act == LIN_RELU) activate(std::integral_constant<int, LIN_RELU>{});
+        else if (a.act == LIN_GELU) activate(std::integral_constant<int, LIN_GELU>{});
+        put((T*)a.C, a.ldc);
     }
 }
 
