@@ -97,21 +97,24 @@ template <> struct GemmFrag<float, false> {
 
 // One operand's tile: where its pieces lie in memory and LDS.
 //   KC:   LDS row r (of TILE) holds 128 bytes of the contraction, piece p at slot p ^ ((r >> 1) & 7)
-//   else: LDS row k (of BK) holds TILE elements; bf16: 32-byte chunk c at c ^ ((k & 3) + 4 ((k >> 3) & 1)),
-//         f32: 64-byte chunk c at c ^ ((k >> 2) & 3)
+//   else: LDS row k (of BK) holds TILE elements; bf16: 32-byte chunk c at c ^ ((k & 3) + 4 ((k >> 3) & 1)), in rows of only
+//         four chunks at c ^ (((k >> 1) & 1) + 2 ((k >> 3) & 1)); f32: 64-byte chunk c at c ^ ((k >> 2) & 3)
 template <typename T, bool KC, int F> struct GemmOperand {
     static constexpr int ES = sizeof(T), TILE = 32 * F, BK = 128 / ES, BYTES = TILE * 128;
     static constexpr int RB = KC ? 128 : TILE * ES;          // bytes of an LDS row
     static constexpr int NP = BYTES / 4096;                  // pieces per lane and step
 
+    static constexpr int turn(int k) {
+        return RB == 128 ? ((k >> 1) & 1) | (((k >> 3) & 1) << 1) : (k & 3) | (((k >> 3) & 1) << 2);
+    }
     // fragment f (16 rows / columns from w0 + 16 f) of half step s: the address without the parts that are immediate
     static __device__ __forceinline__ unsigned base(int lane, int w0, int s) {
         const int l15 = lane & 15, g = lane >> 4;
         if constexpr (KC) {
             return (w0 + l15) * 128 + (((s * 4 + g) ^ (l15 >> 1)) << 4);
         } else if constexpr (ES == 2) {
-            const int row = g * 8 + (l15 >> 2), f = (l15 >> 2) | ((g & 1) << 2);
-            return row * RB + (((w0 >> 4) ^ f) << 5) + (l15 & 3) * 8;
+            const int row = g * 8 + (l15 >> 2);
+            return row * RB + (((w0 >> 4) ^ turn(row)) << 5) + (l15 & 3) * 8;
         } else {
             return (g * 4) * RB + (((w0 >> 4) ^ g) << 6) + l15 * 4;
         }
@@ -127,7 +130,7 @@ template <typename T, bool KC, int F> struct GemmOperand {
         const int p = slot % (RB / 16);
         int q;
         if constexpr (KC) q = p ^ ((row >> 1) & 7);
-        else if constexpr (ES == 2) q = p ^ (((row & 3) | (((row >> 3) & 1) << 2)) << 1);
+        else if constexpr (ES == 2) q = p ^ (turn(row) << 1);
         else q = p ^ (((row >> 2) & 3) << 2);
         el = q * (16 / ES);
     }
@@ -233,14 +236,17 @@ __device__ __forceinline__ void gemm_mfma_in_place(f32x4& c, const u32x4& a, con
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 
+// Steps in LDS: the one that is read and those on their way.  A small tile's step is over long before memory answers.
+constexpr int gemm_stages(int F, bool dma) { return F == 2 && dma ? 4 : 2; }
+
 // DMA: both operands have 16-byte aligned rows whose length along the contiguous index is a multiple of a piece, and come
 // by direct loads into LDS; otherwise they are staged through registers, with every access guarded.
 template <typename T, bool AKC, bool BKC, int F, bool DMA>
 __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     typedef GemmOperand<T, AKC, F> OA;
     typedef GemmOperand<T, BKC, F> OB;
-    constexpr int ES = sizeof(T), TILE = 32 * F, BK = OA::BK, NP = OA::NP, STAGE = OA::BYTES;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];       // [A: 2 stages][B: 2 stages]
+    constexpr int ES = sizeof(T), TILE = 32 * F, BK = OA::BK, NP = OA::NP, STAGE = OA::BYTES, NS = gemm_stages(F, DMA);
+    extern __shared__ __attribute__((aligned(1024))) char smem[];       // [A: NS stages][B: NS stages]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
 
@@ -288,10 +294,10 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         if constexpr (DMA) {
             const auto sa = __builtin_amdgcn_make_buffer_rsrc((void*)(ap + t * astep), 0, 0x80000000, 0x00020000);
             const auto sb = __builtin_amdgcn_make_buffer_rsrc((void*)(bp + t * bstep), 0, 0x80000000, 0x00020000);
-            char* la = smem + (t & 1) * STAGE + (wave * NP + q) * 1024;
+            char* la = smem + (t % NS) * STAGE + (wave * NP + q) * 1024;
             const unsigned oa = kleft < BK && ka[q] >= kleft ? NONE : va[q], ob = kleft < BK && kb[q] >= kleft ? NONE : vb[q];
             __builtin_amdgcn_raw_ptr_buffer_load_lds(sa, (__attribute__((address_space(3))) void*)la, 16, oa, 0, 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(sb, (__attribute__((address_space(3))) void*)(la + 2 * STAGE), 16, ob, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(sb, (__attribute__((address_space(3))) void*)(la + NS * STAGE), 16, ob, 0, 0, 0);
         } else {
             ra[q] = gemm_guarded<T>((const T*)(ap + t * astep + va[q]),
                                     va[q] == NONE || ka[q] >= kleft ? 0 : AKC ? kleft - ka[q] : arows - ea[q]);
@@ -299,16 +305,16 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
                                     vb[q] == NONE || kb[q] >= kleft ? 0 : BKC ? kleft - kb[q] : brows - eb[q]);
         }
     };
-    // step t's pieces of this wave are in LDS
+    // step t's pieces of this wave are in LDS (requests of later steps may still be on their way: they count in order)
     auto land = [&](int t) __attribute__((always_inline)) {
         if constexpr (DMA) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * 2 * NP) : "memory");
         } else {
-            char* la = smem + (t & 1) * STAGE + (wave * NP * 64 + lane) * 16;
+            char* la = smem + (t % NS) * STAGE + (wave * NP * 64 + lane) * 16;
 #pragma unroll
             for (int q = 0; q < NP; ++q) {
                 *(u32x4*)(la + q * 1024) = ra[q];
-                *(u32x4*)(la + 2 * STAGE + q * 1024) = rb[q];
+                *(u32x4*)(la + NS * STAGE + q * 1024) = rb[q];
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
@@ -318,11 +324,12 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     gemm_for<0, F * F>([&](auto I) __attribute__((always_inline)) { acc[I / F][I % F] = f32x4{0.f, 0.f, 0.f, 0.f}; });
     GemmFrag<T, AKC> fa[2][F];
     GemmFrag<T, BKC> fb[2][F];
-    unsigned aa[2], bb[2];      // fragment addresses of the two halves, in the stage that is read next
+    unsigned aa[2], bb[2];      // fragment addresses of the two halves in stage 0, and the stage that is read
+    int stage = 0;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         aa[s] = lds0 + OA::base(lane, wm, s);
-        bb[s] = lds0 + 2 * STAGE + OB::base(lane, wn, s);
+        bb[s] = lds0 + NS * STAGE + OB::base(lane, wn, s);
     }
     auto landed = [&](auto S) __attribute__((always_inline)) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -337,10 +344,10 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
             constexpr int i = I;
             if constexpr (REQ) {
-                if constexpr (i < NP) request(t + 2, i);
+                if constexpr (i < NP) request(t + NS, i);
             }
-            OA::template read<i, r>(fa[r][i], aa[r]);
-            OB::template read<i, r>(fb[r][i], bb[r]);
+            OA::template read<i, r>(fa[r][i], aa[r] + stage * STAGE);
+            OB::template read<i, r>(fb[r][i], bb[r] + stage * STAGE);
             gemm_for<0, F>([&](auto J) __attribute__((always_inline)) {
                 constexpr int j = J;
                 if constexpr (F == 8) {
@@ -365,17 +372,25 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         land(t + 1);
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        aa[0] ^= STAGE; aa[1] ^= STAGE; bb[0] ^= STAGE; bb[1] ^= STAGE;
+        stage = stage + 1 == NS ? 0 : stage + 1;
         multiply(std::integral_constant<int, 1>{}, std::true_type{}, t);
         landed(std::integral_constant<int, 0>{});
     };
 
     if (nt > 0) {
+        if constexpr (DMA) {
 #pragma unroll
-        for (int q = 0; q < NP; ++q) request(0, q);
-        land(0);
+            for (int t = 0; t < NS; ++t)
 #pragma unroll
-        for (int q = 0; q < NP; ++q) request(1, q);
+                for (int q = 0; q < NP; ++q) request(t, q);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * 2 * NP) : "memory");
+        } else {
+#pragma unroll
+            for (int q = 0; q < NP; ++q) request(0, q);
+            land(0);
+#pragma unroll
+            for (int q = 0; q < NP; ++q) request(1, q);
+        }
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
@@ -384,7 +399,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         });
         landed(std::integral_constant<int, 0>{});
         for (int t = 0; t < nt; ++t) step(t);
-        land(nt);            // nothing is on its way into LDS any more
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            // nothing is on its way into LDS any more
     }
     // the last products' results may be read
     if constexpr (F == 8) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
@@ -583,30 +598,47 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long lddy, 
     }
 }
 
-// Tile and split of one product.
+// Tile and split of one product: the pair with the least estimated time.  The estimate is what the kernels measured (us):
+// a workgroup costs `fixed` (first loads, epilogue) and per step of the contraction `busy` where several share a CU and hide
+// each other's waits, `lone` where one has a CU for itself; a split adds a launch and the traffic of its f32 parts.
+//   bf16, 16384 x 1024 outputs of K = 1024:  tiles of 256: 38.3 us, 128: 40.5, 64: 69.0      (K = 256: 21.2, 21.2, 38.0)
+//   bf16,  1024 x 1024 outputs of K = 2048:  128: 23.3 us, in two parts 19.7; 64: 12.1, in two parts 17.4
+//   bf16,   256 x 1024 outputs of K = 16384: 128: 152.6 us whole, 30.9 in sixteen parts; 64: 66.1 whole, 24.4 in four
+// f32 steps are bound by their matrix instructions, a sixteenth of bf16's rate; operands staged through registers cost
+// about twice the direct loads' step.
 struct GemmPlan { int F, parts, kper; };
-GemmPlan gemm_plan(int es, long M, long N, long K, bool big_ok) {
-    const long bk = 128 / es, steps = (K + bk - 1) / bk;
-    auto tiles = [&](long t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
-    GemmPlan p;
-    p.F = big_ok && es == 2 && tiles(256) * (steps / 8 > 1 ? steps / 8 : 1) >= 192 ? 8 : 4;
-    const long n = tiles(32 * p.F), slots = p.F == 8 ? 256 : 512;
-    long parts = n > 0 && n < slots ? slots / n : 1;
-    const long most = steps / 4 > 1 ? steps / 4 : 1;         // at least four steps a part
-    if (parts > most) parts = most;
-    if (parts > 64) parts = 64;
-    p.kper = (int)((steps + parts - 1) / parts);
-    if (p.kper < 1) p.kper = 1;
-    p.parts = (int)((steps + p.kper - 1) / p.kper);
-    if (p.parts < 1) p.parts = 1;
-    return p;
+GemmPlan gemm_plan(int es, long M, long N, long K, bool dma) {
+    struct Cost { int F; double fixed, busy, lone; };
+    static const Cost bf16_dma[3] = {{8, 11.0, 1.5, 1.5}, {4, 3.4, 0.45, 0.60}, {2, 1.7, 0.17, 0.25}};
+    static const Cost bf16_reg[2] = {{4, 3.4, 0.80, 1.20}, {2, 1.7, 0.34, 0.50}};
+    static const Cost f32[2] = {{4, 4.0, 1.90, 2.0}, {2, 1.8, 0.50, 0.55}};
+    const Cost* costs = es == 4 ? f32 : dma ? bf16_dma : bf16_reg;
+    const int n = es == 2 && dma ? 3 : 2;
+    const long bk = 128 / es, steps = K > 0 ? (K + bk - 1) / bk : 1;
+    GemmPlan best = {2, 1, (int)steps};
+    double least = 1e30;
+    for (int i = 0; i < n; ++i) {
+        const long t = 32 * costs[i].F, tiles = ((M + t - 1) / t) * ((N + t - 1) / t);
+        for (long want = 1; want <= 64 && want <= steps; want *= 2) {
+            const long kper = (steps + want - 1) / want, parts = (steps + kper - 1) / kper;
+            const long per_cu = (tiles * parts + 255) / 256;
+            double us = per_cu <= 1 ? costs[i].fixed + kper * costs[i].lone : per_cu * (costs[i].fixed + kper * costs[i].busy);
+            if (parts > 1) us += 4.0 + (double)M * N * (8.0 * parts + es) / 7e6;
+            if (us < least) {
+                least = us;
+                best = {costs[i].F, (int)parts, (int)kper};
+            }
+            if (tiles * parts >= 1024) break;       // more parts only add traffic
+        }
+    }
+    return best;
 }
 long gemm_part_floats(const GemmPlan& p, long M, long N) { return p.parts > 1 ? p.parts * M * ((N + 7) & ~7L) : 0; }
 
 template <typename T, bool AKC, bool BKC, int F, bool DMA>
 int gemm_launch(const GemmArgs& a, unsigned grid, hipStream_t s) {
     static bool done[kMaxDevices] = {};
-    constexpr int lds = 4 * GemmOperand<T, AKC, F>::BYTES;
+    constexpr int lds = 2 * gemm_stages(F, DMA) * GemmOperand<T, AKC, F>::BYTES;
     LDM_TRY(allow_dynamic_lds((const void*)&gemm_kernel<T, AKC, BKC, F, DMA>, lds, done));
     gemm_kernel<T, AKC, BKC, F, DMA><<<grid, 256, lds, s>>>(a);
     LDM_HIP(hipGetLastError());
@@ -628,7 +660,9 @@ int gemm(GemmArgs a, float* ws, hipStream_t s) {
     LDM_REQUIRE(tiles < (1L << 31), "more output tiles than one launch holds");
     a.kper = p.kper;
     a.part = p.parts > 1 ? ws : nullptr;
-    if (!dma) LDM_TRY((gemm_launch<T, AKC, BKC, 4, false>(a, (unsigned)tiles, s)));
+    if (!dma && p.F == 2) LDM_TRY((gemm_launch<T, AKC, BKC, 2, false>(a, (unsigned)tiles, s)));
+    else if (!dma) LDM_TRY((gemm_launch<T, AKC, BKC, 4, false>(a, (unsigned)tiles, s)));
+    else if (p.F == 2) LDM_TRY((gemm_launch<T, AKC, BKC, 2, true>(a, (unsigned)tiles, s)));
     else if (p.F == 4) LDM_TRY((gemm_launch<T, AKC, BKC, 4, true>(a, (unsigned)tiles, s)));
     else if constexpr (sizeof(T) == 2) LDM_TRY((gemm_launch<T, AKC, BKC, 8, true>(a, (unsigned)tiles, s)));
     if (p.parts > 1) {
@@ -668,8 +702,8 @@ int launch_gemm(int dtype, const GemmArgs& a, bool akc, bool bkc, float* ws, hip
 long gemm_ws_floats(int dtype, long M, long N, long K) {
     // which tile it will be depends on the alignment as well
     long n = 0;
-    for (int big = 0; big < 2; ++big) {
-        const long f = gemm_part_floats(gemm_plan(dtype == LDM_BF16 ? 2 : 4, M, N, K, big), M, N);
+    for (int dma = 0; dma < 2; ++dma) {
+        const long f = gemm_part_floats(gemm_plan(dtype == LDM_BF16 ? 2 : 4, M, N, K, dma), M, N);
         n = f > n ? f : n;
     }
     return n;

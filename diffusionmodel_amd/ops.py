@@ -6,6 +6,7 @@ attention."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import struct
 from typing import Optional, Sequence, Tuple
 
@@ -417,6 +418,13 @@ def _check_linear(x: torch.Tensor, weight: torch.Tensor, act: Optional[str]) -> 
     return dev, weight.shape[0], weight.shape[1]
 
 
+@functools.lru_cache(maxsize=4096)
+def _linear_ws(backward: bool, *shape: int) -> int:
+    """Floats of workspace; shape = (type code, M, K, N, weight order)."""
+    lib = _lib.load()
+    return (lib.ldm_linear_backward_ws_floats if backward else lib.ldm_linear_ws_floats)(*shape)
+
+
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
            res: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, save_pre: bool = False):
     """act(x @ weight + bias + res) (ldm_linear): x [..., K] and weight [K, N] (burn's Linear layout, or a transposed view
@@ -444,7 +452,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     if M:
         lib = _lib.load()
         code = _TD[x.dtype]
-        n = lib.ldm_linear_ws_floats(code, M, K, N, order)
+        n = _linear_ws(False, code, M, K, N, order)
         ws = x.new_empty(n, dtype=torch.float32) if n > 0 else None
         _call(lib.ldm_linear, dev, code, x.data_ptr(), ldx, weight.data_ptr(), ldw, order, _data(b), _data(res), ldr,
               LINEAR_ACTS[act], out.data_ptr(), ldo, _data(pre), N, M, K, N, _data(ws))
@@ -481,7 +489,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre
     gb = x.new_empty(N, dtype=torch.float32) if dbias else None
     lib = _lib.load()
     code = _TD[x.dtype]
-    n = lib.ldm_linear_backward_ws_floats(code, M, K, N, order)
+    n = _linear_ws(True, code, M, K, N, order)
     ws = x.new_empty(n, dtype=torch.float32) if n > 0 else None
     _call(lib.ldm_linear_backward, dev, code, dy.data_ptr(), lddy, x.data_ptr(), ldx, weight.data_ptr(), ldw, order,
           _data(pre), ldp, code_act, dz.data_ptr() if code_act else 0, N, _data(gx), K, _data(gw), N if order == 0 else K,
