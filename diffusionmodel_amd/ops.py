@@ -135,9 +135,9 @@ LINEAR_ACTS = {None: 0, "none": 0, "silu": 1, "relu": 2, "gelu": 3}
 ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
 _POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
-_PACK12, _PACK3 = struct.Struct("12l").pack, struct.Struct("3l").pack
-
-# torch.cuda.current_stream() builds a Stream object (2.6 us, as much as a launch); the raw handle is what is needed
+# torch.cuda.current_stream() builds a Stream object (2.6 us, as much as a launch); the raw handle is what is needed.  Small
+# calls are bound by what happens here before the launch, so the checks below take the ordinary case first.
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
@@ -148,23 +148,26 @@ def _data(t: Optional[torch.Tensor]) -> int:
 
 def _check(name: str, t, dev: int = -1, dtypes=_TD) -> int:
     """A device tensor of one of `dtypes`, on device `dev` (-1: any), that needs no gradient.  Returns its device."""
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and not t.requires_grad:
+        d = t.get_device()
+        if d >= 0 and (dev < 0 or d == dev):
+            return d
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a device tensor")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} is {t.dtype}, expected one of {tuple(str(d) for d in dtypes)}")
-    d = t.get_device()
-    if dev >= 0 and d != dev:
-        raise ValueError(f"{name} is on device {d}, expected {dev}")
-    if t.requires_grad and torch.is_grad_enabled():
+    if dev >= 0 and t.get_device() != dev:
+        raise ValueError(f"{name} is on device {t.get_device()}, expected {dev}")
+    if torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which this operator does not record: call it under "
                          "torch.no_grad() and use the operator's backward function")
-    return d
+    return t.get_device()
 
 
 def _rows(name: str, t: torch.Tensor) -> Tuple[int, int]:
     """(rows, row stride) of t [..., C] as one matrix; its last axis must be contiguous."""
     if t.is_contiguous():
-        c = t.shape[-1]
+        c = t.size(-1)
         return (t.numel() // c if c else 0), c
     if t.shape[-1] != 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must be contiguous along its last axis")
@@ -233,19 +236,19 @@ def _params(name: str, t: Optional[torch.Tensor], n: int, dev: int) -> Optional[
     if t is None:
         return None
     _check(name, t, dev, _REAL)
-    if t.dim() != 1 or t.shape[0] != n:
+    if t.dim() != 1 or t.numel() != n:
         raise ValueError(f"{name} must hold {n} values, has shape {tuple(t.shape)}")
     return t if t.dtype is torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
 def _like(x: torch.Tensor) -> torch.Tensor:
     """A contiguous tensor of x's shape, type and device."""
-    return torch.empty_like(x, memory_format=torch.contiguous_format)
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _call(fn, dev: int, *args) -> None:
     """One library call on device `dev` and its current stream (the function's last argument)."""
-    if dev == torch.cuda.current_device():
+    if dev == _device():
         rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
@@ -261,21 +264,22 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     Returns y, or (y, mean, rstd) with `stats`: f32 of shape [...], what layer_norm_backward needs.
     `out` may be x itself."""
     dev = _check("x", x)
-    if x.dim() < 1 or x.shape[-1] < 1:
+    shape = x.shape
+    if not shape or shape[-1] < 1:
         raise ValueError("x must have a last axis of at least one element")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    Cc = x.shape[-1]
+    Cc = shape[-1]
     rows, xs = _rows("x", x)
     w, b = _params("weight", weight, Cc, dev), _params("bias", bias, Cc, dev)
     if out is None:
         out, ys = _like(x), Cc
     else:
-        _check_out("out", out, x.shape, x, (w, b), same=x)
+        _check_out("out", out, shape, x, (w, b), same=x)
         ys = _rows("out", out)[1]
     mean = rstd = None
     if stats:
-        mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+        mean = x.new_empty(shape[:-1], dtype=torch.float32)
         rstd = torch.empty_like(mean)
     if rows:
         _call(_lib.load().ldm_layer_norm, dev, _TD[x.dtype], x.data_ptr(), xs, _data(w), _data(b), eps,
@@ -344,78 +348,83 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, in
     inverse=True turns back: applied to the gradients of the outputs it gives the gradients of q and k.
     Returns (q', k'), or q' if k is None; `out` = (q', k') or q' to write to, which may be the inputs themselves."""
     dev = _check("q", q)
-    if q.dim() != 4:
-        raise ValueError("q must be [B, N, heads, D]")
-    B, N, Hq, D = q.shape
-    Hk = 0
-    sq = q.stride()
-    sk = (0, 0, 0, 1)
     if k is not None:
         _check("k", k, dev, (q.dtype,))
-        if k.dim() != 4 or k.shape[0] != B or k.shape[1] != N or k.shape[3] != D:
-            raise ValueError(f"k must be [{B}, {N}, heads, {D}], has shape {tuple(k.shape)}")
-        Hk, sk = k.shape[2], k.stride()
-    if D < 1 or Hq < 1 or (k is not None and Hk < 1) or (D > 1 and (sq[3] != 1 or sk[3] != 1)):
-        raise ValueError("q and k need at least one head and contiguous head vectors")
     _check("inv_freq", inv_freq, dev, _F32)
     if inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous vector")
-    P = inv_freq.shape[0]
-    sec = (P,) if sections is None else tuple(sections)
-    if not 1 <= len(sec) <= 4 or min(sec) < 0 or sum(sec) != P or P < 1 or 2 * P > D:
-        raise ValueError(f"sections {sec} must hold one to four counts that add up to inv_freq's {P} pairs, at most D / 2")
     _check("positions", positions, dev, _POS_TYPES)
-    ps, pp = positions.shape, positions.stride()
-    if len(ps) == 2:
-        ps, pp = (B,) + tuple(ps), (0,) + pp
-    if len(ps) != 3 or ps[0] != B or ps[1] != len(sec) or ps[2] != N:
-        raise ValueError(f"positions must be [{len(sec)}, {N}] or [{B}, {len(sec)}, {N}], has shape {tuple(positions.shape)}")
-    if layout not in ROPE_LAYOUTS:
-        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
     ok = None
     if out is None:
         oq = _like(q)
-        so = oq.stride()
-        st = sq[:3] + sk[:3] + so[:3]
         if k is not None:
             ok = _like(k)
-            so = ok.stride()
-        st += so[:3]
     else:
         oq, ok = (out, None) if k is None else out
         _check_out("out[0]", oq, q.shape, q, (k, positions, inv_freq), same=q)
         if k is not None:
             _check_out("out[1]", ok, k.shape, q, (q, oq, positions, inv_freq), same=k)
-        if D > 1 and (oq.stride(3) != 1 or (ok is not None and ok.stride(3) != 1)):
-            raise ValueError("the outputs need contiguous head vectors")
-        st = sq[:3] + sk[:3] + oq.stride()[:3] + (oq if ok is None else ok).stride()[:3]
-    if B and N:
-        _call(_lib.load().ldm_rope, dev, _TD[q.dtype], q.data_ptr(), _data(k), oq.data_ptr(), _data(ok),
-              _PACK12(*st), B, N, Hq, Hk, D, positions.data_ptr(), _POS_TYPES[positions.dtype], _PACK3(*pp),
-              inv_freq.data_ptr(), struct.pack(f"{len(sec)}i", *sec), len(sec), ROPE_LAYOUTS[layout], bool(inverse))
+    strides, dims, pos_strides, sec, axes = _rope_plan(
+        q.shape, q.stride(), None if k is None else k.shape, None if k is None else k.stride(), oq.stride(),
+        None if k is None else ok.stride(), positions.shape, positions.stride(), inv_freq.numel(),
+        sections if sections is None else tuple(sections), layout)
+    if q.numel():
+        _call(_lib.load().ldm_rope, dev, _TD[q.dtype], q.data_ptr(), _data(k), oq.data_ptr(), _data(ok), strides, *dims,
+              positions.data_ptr(), _POS_TYPES[positions.dtype], pos_strides, inv_freq.data_ptr(), sec, axes,
+              ROPE_LAYOUTS[layout], bool(inverse))
     return oq if k is None else (oq, ok)
+
+
+@functools.lru_cache(maxsize=1024)
+def _rope_plan(qs, sq, ks, sk, so, sok, ps, pp, P, sections, layout):
+    """Checks the shapes and strides of a rope call and packs them for the library."""
+    if len(qs) != 4:
+        raise ValueError("q must be [B, N, heads, D]")
+    B, N, Hq, D = qs
+    Hk = 0
+    if ks is None:
+        sk = sok = (0, 0, 0, 1)
+    else:
+        if len(ks) != 4 or ks[0] != B or ks[1] != N or ks[3] != D:
+            raise ValueError(f"k must be [{B}, {N}, heads, {D}], has shape {tuple(ks)}")
+        Hk = ks[2]
+    if D < 1 or Hq < 1 or (ks is not None and Hk < 1) or (D > 1 and not sq[3] == sk[3] == so[3] == sok[3] == 1):
+        raise ValueError("q, k and their outputs need at least one head and contiguous head vectors")
+    sec = (P,) if sections is None else sections
+    if not 1 <= len(sec) <= 4 or min(sec) < 0 or sum(sec) != P or P < 1 or 2 * P > D:
+        raise ValueError(f"sections {sec} must hold one to four counts that add up to inv_freq's {P} pairs, at most D / 2")
+    if len(ps) == 2:
+        ps, pp = (B,) + tuple(ps), (0,) + tuple(pp)
+    if len(ps) != 3 or ps[0] != B or ps[1] != len(sec) or ps[2] != N:
+        raise ValueError(f"positions must be [{len(sec)}, {N}] or [{B}, {len(sec)}, {N}], has shape {tuple(ps)}")
+    if layout not in ROPE_LAYOUTS:
+        raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+    return (struct.pack("12l", *(tuple(sq[:3]) + tuple(sk[:3]) + tuple(so[:3]) + tuple(sok[:3]))), (B, N, Hq, Hk, D),
+            struct.pack("3l", *pp), struct.pack(f"{len(sec)}i", *sec), len(sec))
 
 
 def _weight_order(weight: torch.Tensor) -> Tuple[int, int]:
     """(order, leading stride) of a weight [K, N]: 0 for rows of N, 1 for a transposed weight (rows of K)."""
     K, N = weight.shape
-    if N == 1 or weight.stride(1) == 1:
-        return 0, (weight.stride(0) if K > 1 else N)
-    if K == 1 or weight.stride(0) == 1:
-        return 1, weight.stride(1)
+    s0, s1 = weight.stride()
+    if N == 1 or s1 == 1:
+        return 0, (s0 if K > 1 else N)
+    if K == 1 or s0 == 1:
+        return 1, s1
     raise ValueError("weight must be contiguous along one of its axes")
 
 
 def _check_linear(x: torch.Tensor, weight: torch.Tensor, act: Optional[str]) -> Tuple[int, int, int]:
     dev = _check("x", x)
     _check("weight", weight, dev, (x.dtype,))
-    if weight.dim() != 2 or min(weight.shape) < 1:
+    ws = weight.shape
+    if len(ws) != 2 or min(ws) < 1:
         raise ValueError("weight must be [K, N] with K, N >= 1")
-    if x.dim() < 1 or x.shape[-1] != weight.shape[0]:
-        raise ValueError(f"x must be [..., {weight.shape[0]}], has shape {tuple(x.shape)}")
+    if x.dim() < 1 or x.size(-1) != ws[0]:
+        raise ValueError(f"x must be [..., {ws[0]}], has shape {tuple(x.shape)}")
     if act not in LINEAR_ACTS:
         raise ValueError(f"act must be one of {sorted(a for a in LINEAR_ACTS if a)}, got {act!r}")
-    return dev, weight.shape[0], weight.shape[1]
+    return dev, ws[0], ws[1]
 
 
 @functools.lru_cache(maxsize=4096)
