@@ -50,19 +50,24 @@ __device__ __forceinline__ float lin_dact(float z, int act) {
 }
 
 // ---- the matrix kernel ---------------------------------------------------------------------------------------------
-// A workgroup of four waves (2 x 2) computes a tile of TILE x TILE outputs (TILE = 32 F), each wave F x F fragments of
-// 16 x 16.  A step of the contraction is 128 bytes of it (64 bf16, 32 f32); two steps are staged in LDS, one being read
-// while the other arrives.  Both operands keep their memory order in LDS: KC operands as rows of 128 bytes, read by
-// ds_read_b128; the others as rows along their contiguous index, read by transposing loads (bf16) or single words (f32).
-// 16-byte pieces are XOR-swizzled so that each group of lanes that the LDS serves at once touches every bank once.
+// A workgroup of four waves (2 x 2) computes tiles of TILE x TILE outputs (TILE = 32 F), each wave F x F fragments of
+// 16 x 16.  A step of the contraction is 128 bytes of it (64 bf16, 32 f32); NS steps are in LDS, one being read while the
+// others arrive.  Both operands keep their memory order in LDS: KC operands as rows of 128 bytes, read by ds_read_b128;
+// the others as rows along their contiguous index, read by transposing loads (bf16) or single words (f32).  16-byte
+// pieces are XOR-swizzled so that each group of lanes that the LDS serves at once touches every bank once.
 //
 // The products are taken transposed (first operand = B's columns, second = A's rows), so that a lane's four accumulators
 // of a fragment are four consecutive columns of one row.
 //
 // Per step a wave first multiplies the fragments of the step's first half while it reads those of the second, then waits
 // for the next step's data, meets the other waves, and multiplies the second half while it reads the next step's first
-// fragments and asks for the step after it.  One barrier per step; nothing in front of a product is read later than one
+// fragments and asks for the step NS later.  One barrier per step; nothing in front of a product is read later than one
 // half step before it.
+//
+// A wave of the 256 tile has its SIMD for itself and sends an instruction every four cycles or so, 256 in the time of half
+// a step's products: what is not a product has to fit between them.  (Walking over several tiles with the requests
+// running ahead over a tile's end was measured: its bookkeeping made the step longer than the first loads it hid,
+// 497 us against 459 for 65536 x 4096 x 1024.)
 // Fragment reads that the compiler does not wait for: GemmFrag::landed() behind an explicit wait makes the values usable.
 template <typename T, bool KC> struct GemmFrag;
 template <typename T> struct GemmFrag<T, true> {
@@ -124,91 +129,38 @@ template <typename T, bool KC, int F> struct GemmOperand {
         else if constexpr (ES == 2) fr.template read<s * 32 * RB, 4 * RB>(b ^ (f << 5));
         else fr.template read<s * 16 * RB, RB>(b ^ (f << 6));
     }
-    // the piece of memory that goes to 16-byte slot `slot` of the tile: row of the tile and element within the row
-    static __device__ __forceinline__ void piece(int slot, int& row, int& el) {
-        row = slot / (RB / 16);
-        const int p = slot % (RB / 16);
-        int q;
-        if constexpr (KC) q = p ^ ((row >> 1) & 7);
-        else if constexpr (ES == 2) q = p ^ (turn(row) << 1);
-        else q = p ^ (((row >> 2) & 3) << 2);
-        el = q * (16 / ES);
+    // A wave writes 64 consecutive 16-byte slots of the tile at a time.  Lane `lane` of load q of wave w: row
+    // first_row(w, lane) + q ROWS, from element(w, q, lane) of that row on.
+    static constexpr int ROWS = 1024 / RB;
+    static __device__ __forceinline__ int first_row(int w, int lane) { return w * NP * ROWS + lane / (RB / 16); }
+    static __device__ __forceinline__ int element(int w, int q, int lane) {
+        const int p = lane % (RB / 16), row = w * NP * ROWS + q * ROWS + lane / (RB / 16);
+        const int x = KC ? p ^ ((row >> 1) & 7) : ES == 2 ? p ^ (turn(row) << 1) : p ^ (((row >> 2) & 3) << 2);
+        return x * (16 / ES);
     }
 };
 
-// the first n of 16 / sizeof(T) elements at p (element aligned), zeros for the rest; n may be zero or less, or more than all
-typedef u32x4 gemm_u16_a2 __attribute__((aligned(2)));
-typedef u32x4 gemm_u16_a4 __attribute__((aligned(4)));
-template <typename T> __device__ __forceinline__ u32x4 gemm_guarded(const T* p, int n) {
-    constexpr int N = 16 / sizeof(T);
-    u32x4 v = {0u, 0u, 0u, 0u};
-    if (n >= N) {
-        if constexpr (sizeof(T) == 2) v = *(const gemm_u16_a2*)p;
-        else v = *(const gemm_u16_a4*)p;
-    } else if (n > 0) {
-#pragma unroll
-        for (int e = 0; e < N - 1; ++e)
-            if (e < n) {
-                if constexpr (sizeof(T) == 2) v[e >> 1] |= (unsigned)((const unsigned short*)p)[e] << ((e & 1) * 16);
-                else v[e] = ((const unsigned*)p)[e];
-            }
-    }
-    return v;
+// v without its first n elements of type T: the rest moved to the front, zeros behind
+template <typename T> __device__ __forceinline__ u32x4 gemm_drop(u32x4 v, int n) {
+    const int bits = n * (int)sizeof(T) * 8;
+    unsigned long long lo = ((unsigned long long)v[1] << 32) | v[0], hi = ((unsigned long long)v[3] << 32) | v[2];
+    const unsigned long long l = bits >= 64 ? hi >> (bits & 63) : bits ? (lo >> bits) | (hi << (64 - bits)) : lo;
+    const unsigned long long h = bits >= 64 ? 0 : hi >> bits;
+    return u32x4{(unsigned)l, (unsigned)(l >> 32), (unsigned)h, (unsigned)(h >> 32)};
 }
 
-// 8 outputs of row m from column n on: bias, residual, the value before the activation, the activation
+// the outputs of row m from column n to the last, fewer than eight: bias, residual, the value before the activation, the
+// activation
 template <typename T>
-__device__ __forceinline__ void gemm_finish(const GemmArgs& a, long m, long n, float (&v)[8], const float (&bias)[8]) {
-    typedef T VT __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-    typedef float VF __attribute__((ext_vector_type(8)));
-    const bool full = n + 8 <= a.N;
+__device__ __forceinline__ void gemm_finish(const GemmArgs& a, long m, long n, const float (&v)[8], const float (&bias)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += bias[e];
-    if (a.res) {
-        const T* r = (const T*)a.res + m * a.ldr + n;
-        if (full) {
-            const VF f = __builtin_convertvector(*(const VT*)r, VF);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += f[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (n + e < a.N) v[e] += (float)r[e];
+    for (int e = 0; e < 7; ++e)
+        if (n + e < a.N) {
+            float x = v[e] + bias[e];
+            if (a.res) x += (float)((const T*)a.res)[m * a.ldr + n + e];
+            if (a.pre) ((T*)a.pre)[m * a.ldp + n + e] = (T)x;
+            ((T*)a.C)[m * a.ldc + n + e] = (T)lin_act(x, a.act);
         }
-    }
-    VF o;
-    if (a.pre) {
-        T* p = (T*)a.pre + m * a.ldp + n;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = v[e];
-        if (full) {
-            *(VT*)p = __builtin_convertvector(o, VT);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (n + e < a.N) p[e] = (T)v[e];
-        }
-    }
-    T* c = (T*)a.C + m * a.ldc + n;
-    if (a.act == LIN_SILU) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = lin_act(v[e], LIN_SILU);
-    } else if (a.act == LIN_RELU) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = lin_act(v[e], LIN_RELU);
-    } else if (a.act == LIN_GELU) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = lin_act(v[e], LIN_GELU);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = v[e];
-    if (full) {
-        *(VT*)c = __builtin_convertvector(o, VT);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (n + e < a.N) c[e] = (T)v[e];
-    }
 }
 __device__ __forceinline__ void gemm_bias(const GemmArgs& a, long n, float (&b)[8]) {
     const int left = n >= a.N ? 0 : a.N - n < 8 ? (int)(a.N - n) : 8;
@@ -227,6 +179,15 @@ template <int I, int N_, typename Fn> __device__ __forceinline__ void gemm_for(F
     }
 }
 
+// 16 bytes per lane from base + lane_off to LDS at dst (of the wave) + 16 lane; offsets from 2^31 on: zeros, no access
+__device__ __forceinline__ void gemm_dma(const char* base, char* dst, unsigned lane_off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x80000000, 0x00020000),
+                                             (__attribute__((address_space(3))) void*)dst, 16, lane_off, 0, 0, 0);
+}
+// waits until all but N_ of this wave's memory operations are done (they end in order)
+template <int N_> __device__ __forceinline__ void gemm_all_but() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N_ < 63 ? N_ : 63) : "memory");
+}
 // behind an explicit wait: the compiler takes the value as it stands
 template <typename V> __device__ __forceinline__ void gemm_landed(V& v) { asm volatile("" : "+v"(v)); }
 // marks v as the one of branch I: branches that pick from a register array by a run-time index stay apart (merged, they
@@ -238,20 +199,26 @@ __device__ __forceinline__ void gemm_mfma_in_place(f32x4& c, const u32x4& a, con
 
 // Steps in LDS: the one that is read and those on their way.  A small tile's step is over long before memory answers.
 constexpr int gemm_stages(int F, bool dma) { return F == 2 && dma ? 4 : 2; }
+constexpr int gemm_lds(int F, bool dma) { return 2 * gemm_stages(F, dma) * F * 4096; }
 
 // DMA: both operands have 16-byte aligned rows whose length along the contiguous index is a multiple of a piece, and come
-// by direct loads into LDS; otherwise they are staged through registers, with every access guarded.
+// by direct loads into LDS.  Otherwise pieces are loaded at element alignment into registers, two steps ahead, and written
+// to LDS one step before they are read; a piece that would leave its row is taken from the row's end and moved into
+// place, so the loads need no branches (which would make the compiler wait for all of them).  That takes rows of at
+// least one piece.
 template <typename T, bool AKC, bool BKC, int F, bool DMA>
 __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     typedef GemmOperand<T, AKC, F> OA;
     typedef GemmOperand<T, BKC, F> OB;
-    constexpr int ES = sizeof(T), TILE = 32 * F, BK = OA::BK, NP = OA::NP, STAGE = OA::BYTES, NS = gemm_stages(F, DMA);
-    extern __shared__ __attribute__((aligned(1024))) char smem[];       // [A: NS stages][B: NS stages]
+    constexpr int ES = sizeof(T), V = 16 / ES, TILE = 32 * F, BK = OA::BK, NP = OA::NP, STAGE = OA::BYTES;
+    constexpr int NS = gemm_stages(F, DMA);
+    constexpr int SETS = !DMA && F == 2 ? 2 : 1;          // register sets (more do not fit a tile of 128)
+    extern __shared__ __attribute__((aligned(1024))) char smem[];       // [A: NS stages][B: NS stages], then the epilogue's
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
 
-    // the tile: neighbouring tiles on one XCD (workgroups go round the eight XCDs), panels of eight tile columns
-    const unsigned total = gridDim.x, per = total / 8;
+    // the tile: workgroups go round the eight XCDs, and each XCD has a run of neighbouring tiles, in panels of eight columns
+    const unsigned per = gridDim.x / 8;
     unsigned lin = blockIdx.x;
     if (lin < per * 8) lin = (lin & 7) * per + (lin >> 3);
     const unsigned ntn = (unsigned)((a.N + TILE - 1) / TILE), ntm = (unsigned)((a.M + TILE - 1) / TILE);
@@ -259,69 +226,98 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     const unsigned panel = id / (ntm * 8), in_panel = id - panel * (ntm * 8);
     const unsigned pw = ntn - panel * 8 < 8 ? ntn - panel * 8 : 8;
     const long m0 = (long)(in_panel / pw) * TILE, n0 = (long)(panel * 8 + in_panel % pw) * TILE;
-    const long kbeg = (long)z * a.kper * BK, kend = a.K < kbeg + (long)a.kper * BK ? a.K : kbeg + (long)a.kper * BK;
-    const int nt = (int)((kend - kbeg + BK - 1) / BK);
-
+    const long kbeg = (long)z * a.kper * BK;
+    const int klen = (int)(a.K - kbeg < (long)a.kper * BK ? a.K - kbeg : (long)a.kper * BK);
+    int nt = (klen + BK - 1) / BK;
+    if (SETS == 2) nt += nt & 1;          // the register sets take turns: an even number of steps, the last one all zeros
     const int wm = (wave >> 1) * (TILE / 2), wn = (wave & 1) * (TILE / 2);
+
+    // the step that is asked for next, and this lane's pieces of it
     const char* ap = (const char*)a.A + (AKC ? m0 * a.lda + kbeg : kbeg * a.lda + m0) * ES;
     const char* bp = (const char*)a.B + (BKC ? n0 * a.ldb + kbeg : kbeg * a.ldb + n0) * ES;
     const long astep = AKC ? 128 : a.lda * BK * ES, bstep = BKC ? 128 : a.ldb * BK * ES;
-    const int arows = (int)(a.M - m0 < TILE ? a.M - m0 : TILE), brows = (int)(a.N - n0 < TILE ? a.N - n0 : TILE);
-    const int klen = (int)(kend - kbeg < (1L << 30) ? kend - kbeg : (1L << 30));
-
-    // this lane's pieces: offset from the step's start (out of range where the tile ends), and index along k
+    const int arows = (int)(a.M - m0 < (1 << 30) ? a.M - m0 : (1 << 30));      // rows / columns to the end of the matrix
+    const int brows = (int)(a.N - n0 < (1 << 30) ? a.N - n0 : (1 << 30));
+    int kleft = klen, rstage = 0;
+    const int rowa = OA::first_row(wave, lane), rowb = OB::first_row(wave, lane);
     constexpr unsigned NONE = 0x80000000u;
-    unsigned va[NP], vb[NP];
-    int ka[NP], kb[NP], ea[NP], eb[NP];
-#pragma unroll
-    for (int q = 0; q < NP; ++q) {
-        int row, el;
-        OA::piece((wave * NP + q) * 64 + lane, row, el);
-        const int ma = AKC ? row : el;
-        ka[q] = AKC ? el : row;
-        ea[q] = el;
-        va[q] = ma < arows ? (unsigned)((long)row * a.lda * ES + el * ES) : NONE;
-        OB::piece((wave * NP + q) * 64 + lane, row, el);
-        const int mb = BKC ? row : el;
-        kb[q] = BKC ? el : row;
-        eb[q] = el;
-        vb[q] = mb < brows ? (unsigned)((long)row * a.ldb * ES + el * ES) : NONE;
-    }
-    u32x4 ra[DMA ? 1 : NP], rb[DMA ? 1 : NP];
-    // asks for piece q of both operands of step t (steps behind the last one: zeros, without a memory access)
-    auto request = [&](int t, int q) __attribute__((always_inline)) {
-        const int kleft = klen - t * BK;
-        if constexpr (DMA) {
-            const auto sa = __builtin_amdgcn_make_buffer_rsrc((void*)(ap + t * astep), 0, 0x80000000, 0x00020000);
-            const auto sb = __builtin_amdgcn_make_buffer_rsrc((void*)(bp + t * bstep), 0, 0x80000000, 0x00020000);
-            char* la = smem + (t % NS) * STAGE + (wave * NP + q) * 1024;
-            const unsigned oa = kleft < BK && ka[q] >= kleft ? NONE : va[q], ob = kleft < BK && kb[q] >= kleft ? NONE : vb[q];
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(sa, (__attribute__((address_space(3))) void*)la, 16, oa, 0, 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(sb, (__attribute__((address_space(3))) void*)(la + NS * STAGE), 16, ob, 0, 0, 0);
-        } else {
-            ra[q] = gemm_guarded<T>((const T*)(ap + t * astep + va[q]),
-                                    va[q] == NONE || ka[q] >= kleft ? 0 : AKC ? kleft - ka[q] : arows - ea[q]);
-            rb[q] = gemm_guarded<T>((const T*)(bp + t * bstep + vb[q]),
-                                    vb[q] == NONE || kb[q] >= kleft ? 0 : BKC ? kleft - kb[q] : brows - eb[q]);
+    unsigned va[DMA ? NP : 1], vb[DMA ? NP : 1];         // offsets from the step's start
+    if constexpr (DMA)
+        gemm_for<0, NP>([&](auto Q) __attribute__((always_inline)) {
+            constexpr int q = Q;
+            const int ya = rowa + q * OA::ROWS, xa = OA::element(wave, q, lane);
+            const int yb = rowb + q * OB::ROWS, xb = OB::element(wave, q, lane);
+            va[q] = (AKC ? ya : xa) < arows ? (unsigned)(ya * (int)a.lda + xa) * ES : NONE;
+            vb[q] = (BKC ? yb : xb) < brows ? (unsigned)(yb * (int)a.ldb + xb) * ES : NONE;
+        });
+    // the pieces behind the end of the contraction leave the offsets when the last step, or none, is asked for: a branch
+    // that two or three steps take, instead of a comparison per piece in all of them
+    auto narrow = [&]() __attribute__((always_inline)) {
+        if (DMA && kleft < BK) {
+            asm volatile("" ::: "memory");
+            gemm_for<0, NP>([&](auto Q) __attribute__((always_inline)) {
+                constexpr int q = Q;
+                if ((AKC ? OA::element(wave, q, lane) : rowa + q * OA::ROWS) >= kleft) va[q] = NONE;
+                if ((BKC ? OB::element(wave, q, lane) : rowb + q * OB::ROWS) >= kleft) vb[q] = NONE;
+            });
         }
     };
-    // step t's pieces of this wave are in LDS (requests of later steps may still be on their way: they count in order)
-    auto land = [&](int t) __attribute__((always_inline)) {
+    u32x4 ra[SETS][DMA ? 1 : NP], rb[SETS][DMA ? 1 : NP];
+    int rk[SETS] = {};                    // kleft of the steps in the register sets
+    // asks for piece Q of both operands (register set S); behind the last step: zeros, no memory access (DMA), or the
+    // first elements of the matrix, which are not used
+    auto request = [&](auto Q, auto S) __attribute__((always_inline)) {
+        constexpr int q = Q;
         if constexpr (DMA) {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * 2 * NP) : "memory");
+            char* la = smem + rstage * STAGE + (wave * NP + q) * 1024;
+            gemm_dma(ap, la, va[q]);
+            gemm_dma(bp, la + NS * STAGE, vb[q]);
         } else {
-            char* la = smem + (t % NS) * STAGE + (wave * NP * 64 + lane) * 16;
-#pragma unroll
-            for (int q = 0; q < NP; ++q) {
-                *(u32x4*)(la + q * 1024) = ra[q];
-                *(u32x4*)(la + NS * STAGE + q * 1024) = rb[q];
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            typedef typename RowVec<T>::V U;
+            const bool live = kleft > 0;
+            const char* pa = live ? ap : (const char*)a.A;
+            const char* pb = live ? bp : (const char*)a.B;
+            // KC: the row no further than the last, the piece no further than the end of k; else the other way round
+            auto upto = [](int v, int most) __attribute__((always_inline)) { return v < most ? v : most; };
+            const int ya = rowa + q * OA::ROWS, xa = OA::element(wave, q, lane), yb = rowb + q * OB::ROWS, xb = OB::element(wave, q, lane);
+            const int ra_ = live ? upto(ya, (AKC ? arows : kleft) - 1) : 0, ca = live ? upto(xa, (AKC ? kleft : arows) - V) : 0;
+            const int rb_ = live ? upto(yb, (BKC ? brows : kleft) - 1) : 0, cb = live ? upto(xb, (BKC ? kleft : brows) - V) : 0;
+            const long ea = (long)ra_ * a.lda + ca, eb = (long)rb_ * a.ldb + cb;
+            ra[S][q] = __builtin_bit_cast(u32x4, (typename RowVec<T>::R)*(const U*)(pa + ea * ES));
+            rb[S][q] = __builtin_bit_cast(u32x4, (typename RowVec<T>::R)*(const U*)(pb + eb * ES));
         }
+    };
+    auto requested = [&](auto S) __attribute__((always_inline)) {       // the step is complete: on to the next
+        rk[S] = kleft;
+        rstage = rstage + 1 == NS ? 0 : rstage + 1;
+        kleft -= BK;
+        ap += astep;
+        bp += bstep;
+        narrow();
+    };
+    // this wave's pieces of register set S are written to stage `st`
+    auto write = [&](auto S, int st) __attribute__((always_inline)) {
+        char* la = smem + st * STAGE + (wave * NP * 64 + lane) * 16;
+        // pieces that were taken from the end of their row, and those behind the end of k
+        if (rk[S] < BK || (!AKC && arows < TILE) || (!BKC && brows < TILE)) {
+            gemm_for<0, NP>([&](auto Q) __attribute__((always_inline)) {
+                constexpr int q = Q;
+                const int xa = OA::element(wave, q, lane), xb = OB::element(wave, q, lane);
+                const int da = xa - ((AKC ? rk[S] : arows) - V), db = xb - ((BKC ? rk[S] : brows) - V);
+                if (da > 0) ra[S][q] = gemm_drop<T>(ra[S][q], da < V ? da : V - 1);
+                if (db > 0) rb[S][q] = gemm_drop<T>(rb[S][q], db < V ? db : V - 1);
+                if ((AKC ? xa : rowa + q * OA::ROWS) >= rk[S]) ra[S][q] = u32x4{0u, 0u, 0u, 0u};
+                if ((BKC ? xb : rowb + q * OB::ROWS) >= rk[S]) rb[S][q] = u32x4{0u, 0u, 0u, 0u};
+            });
+        }
+        gemm_for<0, NP>([&](auto Q) __attribute__((always_inline)) {
+            *(u32x4*)(la + Q * 1024) = ra[S][Q];
+            *(u32x4*)(la + NS * STAGE + Q * 1024) = rb[S][Q];
+        });
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
 
     f32x4 acc[F][F];       // [row fragment][column fragment]
-    gemm_for<0, F * F>([&](auto I) __attribute__((always_inline)) { acc[I / F][I % F] = f32x4{0.f, 0.f, 0.f, 0.f}; });
     GemmFrag<T, AKC> fa[2][F];
     GemmFrag<T, BKC> fb[2][F];
     unsigned aa[2], bb[2];      // fragment addresses of the two halves in stage 0, and the stage that is read
@@ -338,213 +334,329 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
             fb[S][I].landed();
         });
     };
-    // products of half S, with the reads of the other half's fragments (and a step's requests) between them
-    auto multiply = [&](auto S, auto REQ, int t) __attribute__((always_inline)) {
-        constexpr int s = S, r = 1 - S;
+    // products of half H, with the reads of the other half's fragments, and in the second half the requests (register set
+    // S), between them
+    auto multiply = [&](auto H, auto S) __attribute__((always_inline)) {
+        constexpr int h = H, r = 1 - h;
         gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
             constexpr int i = I;
-            if constexpr (REQ) {
-                if constexpr (i < NP) request(t + NS, i);
-            }
+            if constexpr (h == 1 && i < NP) request(I, S);
             OA::template read<i, r>(fa[r][i], aa[r] + stage * STAGE);
             OB::template read<i, r>(fb[r][i], bb[r] + stage * STAGE);
             gemm_for<0, F>([&](auto J) __attribute__((always_inline)) {
                 constexpr int j = J;
                 if constexpr (F == 8) {
                     // in place by constraint: with all 256 accumulators live the compiler's own choice moves them about
-                    gemm_mfma_in_place(acc[i][j], fb[s][j].bits(), fa[s][i].bits());
+                    gemm_mfma_in_place(acc[i][j], fb[h][j].bits(), fa[h][i].bits());
                 } else if constexpr (ES == 2) {
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fb[s][j].bits()),
-                                                                        __builtin_bit_cast(bf16x8, fa[s][i].bits()),
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fb[h][j].bits()),
+                                                                        __builtin_bit_cast(bf16x8, fa[h][i].bits()),
                                                                         acc[i][j], 0, 0, 0);
                 } else {
+                    // lane group g holds k = 4 g .. 4 g + 3; product q takes element q of both operands
                     gemm_for<0, 4>([&](auto Q) __attribute__((always_inline)) {
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[s][j].f32(Q), fa[s][i].f32(Q), acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[h][j].f32(Q), fa[h][i].f32(Q), acc[i][j], 0, 0, 0);
                     });
                 }
             });
             __builtin_amdgcn_sched_barrier(0);
         });
     };
-    auto step = [&](int t) __attribute__((always_inline)) {
-        multiply(std::integral_constant<int, 0>{}, std::false_type{}, t);
-        landed(std::integral_constant<int, 1>{});
-        land(t + 1);
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        stage = stage + 1 == NS ? 0 : stage + 1;
-        multiply(std::integral_constant<int, 1>{}, std::true_type{}, t);
-        landed(std::integral_constant<int, 0>{});
-    };
 
-    if (nt > 0) {
-        if constexpr (DMA) {
-#pragma unroll
-            for (int t = 0; t < NS; ++t)
-#pragma unroll
-                for (int q = 0; q < NP; ++q) request(t, q);
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * 2 * NP) : "memory");
-        } else {
-#pragma unroll
-            for (int q = 0; q < NP; ++q) request(0, q);
-            land(0);
-#pragma unroll
-            for (int q = 0; q < NP; ++q) request(1, q);
-        }
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
-            OA::template read<I, 0>(fa[0][I], aa[0]);
-            OB::template read<I, 0>(fb[0][I], bb[0]);
-        });
-        landed(std::integral_constant<int, 0>{});
-        for (int t = 0; t < nt; ++t) step(t);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            // nothing is on its way into LDS any more
-    }
-    // the last products' results may be read
-    if constexpr (F == 8) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-    __syncthreads();
-
-    // epilogue: 16 rows at a time through LDS, so that memory sees whole rows.  One copy of the code for all row fragments
+    // outputs: 16 rows at a time through LDS, so that memory sees whole rows.  One copy of the code for all row fragments
     // (unrolled over them it would not fit the instruction cache), and no load between the stores: loads and stores count
     // together and in order, so a wait for one would be a wait for every store before it (256 x 256 outputs without a
-    // residual: 11.7 us with such waits, _EPI_ without).
-    constexpr int ROW = F * 64 + 16, LPR = F * 2, RPP = 64 / LPR, P = 16 / RPP;     // bytes of a row, lanes per row, rows
-    typedef typename RowVec<T>::R R;                                               // per pass, passes
-    constexpr int H = 16 / RowVec<T>::N / 2;                                       // vectors of T in eight columns
-    char* tr = smem + wave * 16 * ROW;
+    // residual: 11.7 us with such waits, 6.0 without).
+    constexpr int LPR = F * 2, RPP = 64 / LPR, P = 16 / RPP;                       // lanes per row, rows per pass, passes
+    typedef typename RowVec<T>::R R;
+    constexpr int H = 8 / RowVec<T>::N;                                            // vectors of T in eight columns
+    char* tr = smem + wave * 16 * F * 64;
     const int g = lane >> 4, l15 = lane & 15, c = (lane % LPR) * 8, r0 = lane / LPR;
-    const long n = n0 + wn + c, mw = m0 + wm + r0;
-    auto spill = [&](int i) __attribute__((always_inline)) {
-        gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
-            if (i == I) gemm_for<0, F>([&](auto J) __attribute__((always_inline)) {
-                f32x4 v = acc[I][J];
-                gemm_pick<I>(v);
-                *(f32x4*)(tr + l15 * ROW + J * 64 + g * 16) = v;
+    // slot of 16-byte piece p of row r
+    auto slot = [&](int r, int p) __attribute__((always_inline)) { return (r * F * 4 + (p ^ (F == 2 ? r >> 1 : r))) * 16; };
+    auto finish = [&]() __attribute__((always_inline)) {
+        const long n = n0 + wn + c, mw = m0 + wm + r0;
+        auto spill = [&](int i) __attribute__((always_inline)) {
+            gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
+                if (i == I) gemm_for<0, F>([&](auto J) __attribute__((always_inline)) {
+                    f32x4 v = acc[I][J];
+                    gemm_pick<I>(v);
+                    *(f32x4*)(tr + slot(l15, J * 4 + g)) = v;
+                });
             });
-        });
-    };
-    auto take = [&](int p, float (&v)[8]) {
-        const f32x4 lo = *(const f32x4*)(tr + (p * RPP + r0) * ROW + c * 4), hi = *(const f32x4*)(tr + (p * RPP + r0) * ROW + c * 4 + 16);
+        };
+        auto take = [&](int p, float (&v)[8]) __attribute__((always_inline)) {
+            const int r = p * RPP + r0;
+            const f32x4 lo = *(const f32x4*)(tr + slot(r, c / 4)), hi = *(const f32x4*)(tr + slot(r, c / 4 + 1));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[e] = lo[e];
-            v[4 + e] = hi[e];
+            for (int e = 0; e < 4; ++e) {
+                v[e] = lo[e];
+                v[4 + e] = hi[e];
+            }
+        };
+        if (a.part) {
+            const long np = (a.N + 7) & ~7L;
+            float* part = a.part + (long)z * a.M * np;
+#pragma unroll 1
+            for (int i = 0; i < F; ++i) {
+                spill(i);
+                float v[P][8];
+#pragma unroll
+                for (int p = 0; p < P; ++p) take(p, v[p]);
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const long m = mw + i * 16 + p * RPP;
+                    if (m >= a.M || n >= a.N) continue;
+                    *(f32x4*)(part + m * np + n) = f32x4{v[p][0], v[p][1], v[p][2], v[p][3]};
+                    *(f32x4*)(part + m * np + n + 4) = f32x4{v[p][4], v[p][5], v[p][6], v[p][7]};
+                }
+            }
+            return;
         }
-    };
-    if (a.part) {
-        const long np = (a.N + 7) & ~7L;
-        float* part = a.part + (long)z * a.M * np;
+        float bias[8];
+        gemm_bias(a, n, bias);
+        const bool full = n + 8 <= a.N;         // else the piece is cut by the last column, or lies behind it
+        const int rows = (int)(a.M - m0 < TILE ? a.M - m0 : TILE), rl = wm + r0;
+        R res[F][P * H];
+        if (a.res) {
+            const char* rp = (const char*)a.res + (m0 * a.ldr + n0) * ES;
+            const int ld = (int)a.ldr * ES;
+            if (full)
+                gemm_for<0, F * P * H>([&](auto I) __attribute__((always_inline)) {
+                    constexpr int i = I / (P * H), p = I / H % P, h = I % H;
+                    const int r = rl + i * 16 + p * RPP < rows ? rl + i * 16 + p * RPP : rows - 1;
+                    res[i][p * H + h] = *(const typename RowVec<T>::V*)(rp + (unsigned)(r * ld + (wn + c) * ES + h * 16));
+                });
+        }
+        if (a.res || a.bias) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        gemm_for<0, 8>([&](auto E) __attribute__((always_inline)) { gemm_landed(bias[E]); });
+        if (a.res)
+            gemm_for<0, F * P * H>([&](auto I) __attribute__((always_inline)) { gemm_landed(res[I / (P * H)][I % (P * H)]); });
 #pragma unroll 1
         for (int i = 0; i < F; ++i) {
             spill(i);
             float v[P][8];
 #pragma unroll
-            for (int p = 0; p < P; ++p) take(p, v[p]);
-#pragma unroll
             for (int p = 0; p < P; ++p) {
-                const long m = mw + i * 16 + p * RPP;
-                if (m >= a.M || n >= a.N) continue;
-                *(f32x4*)(part + m * np + n) = f32x4{v[p][0], v[p][1], v[p][2], v[p][3]};
-                *(f32x4*)(part + m * np + n + 4) = f32x4{v[p][4], v[p][5], v[p][6], v[p][7]};
+                take(p, v[p]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[p][e] += bias[e];
             }
-        }
-        return;
-    }
-    float bias[8];
-    gemm_bias(a, n, bias);
-    if (n0 + TILE > a.N) {
-        // the last tile column, where a piece of eight may be cut: guarded, piece by piece
-#pragma unroll 1
-        for (int i = 0; i < F; ++i) {
-            spill(i);
-#pragma unroll 1
-            for (int p = 0; p < P; ++p) {
-                float v[8];
-                take(p, v);
-                const long m = mw + i * 16 + p * RPP;
-                if (m < a.M && n < a.N) gemm_finish<T>(a, m, n, v, bias);
+            if (a.res) {
+                gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
+                    if (i == I)
+                        gemm_for<0, P * H>([&](auto Q) __attribute__((always_inline)) {
+                            float r[RowVec<T>::N];
+                            R x = res[I][Q];
+                            gemm_pick<I>(x);
+                            row_floats<T>(x, r);
+#pragma unroll
+                            for (int e = 0; e < RowVec<T>::N; ++e) v[Q / H][(Q % H) * RowVec<T>::N + e] += r[e];
+                        });
+                });
             }
-        }
-        return;
-    }
-    R res[F][P * H];
-    if (a.res) {
-        gemm_for<0, F * P * H>([&](auto I) __attribute__((always_inline)) {
-            constexpr int i = I / (P * H), p = I / H % P, h = I % H;
-            const long m = mw + i * 16 + p * RPP < a.M ? mw + i * 16 + p * RPP : a.M - 1;
-            res[i][p * H + h] = *(const typename RowVec<T>::V*)((const T*)a.res + m * a.ldr + n + h * RowVec<T>::N);
-        });
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    gemm_for<0, 8>([&](auto E) __attribute__((always_inline)) { gemm_landed(bias[E]); });
-    if (a.res) gemm_for<0, F * P * H>([&](auto I) __attribute__((always_inline)) { gemm_landed(res[I / (P * H)][I % (P * H)]); });
+            auto put = [&](void* out, long ld) __attribute__((always_inline)) {
+                char* o = (char*)out + (m0 * ld + n0) * ES;
+                const int ldb = (int)ld * ES;
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+                    if (full && rl + i * 16 + p * RPP < rows) {
+#pragma unroll
+                        for (int h = 0; h < H; ++h)
+                            row_store<T>((T*)(o + (unsigned)((rl + i * 16 + p * RPP) * ldb + (wn + c) * ES + h * 16)), RowVec<T>::N,
+                                         v[p] + h * RowVec<T>::N);
+                    }
+            };
+            if (a.pre) put(a.pre, a.ldp);
+            auto activate = [&](auto A) __attribute__((always_inline)) {
+#pragma unroll
+                for (int p = 0; p < P; ++p)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[p][e] = lin_act(v[p][e], A);
+            };
+            if (a.act == LIN_SILU) activate(std::integral_constant<int, LIN_SILU>{});
+            else if (a.act == LIN_RELU) activate(std::integral_constant<int, LIN_RELU>{});
+            else if (a.act == LIN_GELU) activate(std::integral_constant<int, LIN_GELU>{});
+            put(a.C, a.ldc);
+            if (n0 + TILE > a.N && (a.N & 7)) {
+                // the piece that the last column cuts: element by element
 #pragma unroll 1
-    for (int i = 0; i < F; ++i) {
-        spill(i);
-        float v[P][8];
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-            take(p, v[p]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[p][e] += bias[e];
-        }
-        if (a.res) {
-            gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
-                if (i == I)
-                    gemm_for<0, P * H>([&](auto Q) __attribute__((always_inline)) {
-                        float r[RowVec<T>::N];
-                        R x = res[I][Q];
-                        gemm_pick<I>(x);
-                        row_floats<T>(x, r);
-#pragma unroll
-                        for (int e = 0; e < RowVec<T>::N; ++e) v[Q / H][(Q % H) * RowVec<T>::N + e] += r[e];
-                    });
-            });
-        }
-        const long m = mw + i * 16;
-        auto put = [&](T* out, long ld) __attribute__((always_inline)) {
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-                if (m + p * RPP < a.M) {
-#pragma unroll
-                    for (int h = 0; h < H; ++h)
-                        row_store<T>(out + (m + p * RPP) * ld + n + h * RowVec<T>::N, RowVec<T>::N, v[p] + h * RowVec<T>::N);
+                for (int p = 0; p < P; ++p) {
+                    float w[8];
+                    take(p, w);
+                    const long m = mw + i * 16 + p * RPP;
+                    if (m < a.M && n < a.N && !full) gemm_finish<T>(a, m, n, w, bias);
                 }
-        };
-        if (a.pre) put((T*)a.pre, a.ldp);
-        auto activate = [&](auto A) __attribute__((always_inline)) {
+            }
+        }
+    };
+
+    const std::integral_constant<int, 0> c0;
+    const std::integral_constant<int, 1> c1;
+    auto ask = [&](auto S) __attribute__((always_inline)) {
+        gemm_for<0, NP>([&](auto Q) __attribute__((always_inline)) { request(Q, S); });
+        requested(S);
+    };
+    narrow();
+    if constexpr (DMA) {
+        for (int t = 0; t < NS; ++t) ask(c0);
+        gemm_all_but<(NS - 1) * 2 * NP>();
+    } else {
+        // sets hold the steps 1, 2 (of two) or the step 1 when the loop starts
+        ask(c0);
+        if constexpr (SETS == 2) ask(c1);
+        write(c0, 0);
+        ask(c0);
+    }
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    gemm_for<0, F * F>([&](auto I) __attribute__((always_inline)) { acc[I / F][I % F] = f32x4{0.f, 0.f, 0.f, 0.f}; });
+    gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
+        OA::template read<I, 0>(fa[0][I], aa[0]);
+        OB::template read<I, 0>(fb[0][I], bb[0]);
+    });
+    landed(c0);
+    // a step; S: the register set that holds the next one
+    auto step = [&](auto S) __attribute__((always_inline)) {
+        multiply(c0, S);
+        landed(c1);
+        const int next = stage + 1 == NS ? 0 : stage + 1;
+        if constexpr (DMA) gemm_all_but<(NS - 2) * 2 * NP>();       // the later steps that were asked for
+        else write(S, next);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        stage = next;
+        multiply(c1, S);
+        requested(S);
+        landed(c0);
+    };
+    if constexpr (SETS == 1) {
+        for (int t = 0; t < nt; ++t) step(c0);
+    } else {
+        for (int t = 0; t < nt; t += 2) {
+            step(c1);
+            step(c0);
+        }
+    }
+    // nothing is on its way into LDS any more, and the last products' results may be read
+    gemm_all_but<0>();
+    if constexpr (F == 8) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+    __syncthreads();
+    finish();
+}
+
+// Any sizes, strides and alignment, element by element: 64 x 64 outputs per workgroup, 64 bytes of the contraction per step.
+// Serves the products with an operand whose rows are shorter than one 16-byte piece.
+constexpr int GT = 64, GROW = 64 + 16;      // bytes of an LDS row: 64 of data, padded against bank conflicts
+template <typename T, bool AKC, bool BKC>
+__global__ __launch_bounds__(256) void gemm_any_kernel(GemmArgs a) {
+    constexpr int ES = sizeof(T), KB = 64 / ES;
+    __shared__ __attribute__((aligned(16))) char As[GT * GROW];
+    __shared__ __attribute__((aligned(16))) char Bs[GT * GROW];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int g = lane >> 4, l15 = lane & 15;
+    const unsigned ntn = (unsigned)((a.N + GT - 1) / GT), ntm = (unsigned)((a.M + GT - 1) / GT);
+    const unsigned z = blockIdx.x / (ntn * ntm), id = blockIdx.x - z * (ntn * ntm);
+    const long m0 = (long)(id / ntn) * GT, n0 = (long)(id % ntn) * GT;
+    const long kbeg = (long)z * a.kper * 2 * KB, kmost = kbeg + (long)a.kper * 2 * KB, kend = a.K < kmost ? a.K : kmost;
+    const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
+    f32x4 acc[2][2] = {};      // [n][m]
+    for (long k0 = kbeg; k0 < kend; k0 += KB) {
+        __syncthreads();
+        for (int i = tid; i < GT * KB; i += 256) {
+            const int r = AKC ? i / KB : i % GT, k = AKC ? i % KB : i / GT;
+            T v = (T)0.f;
+            if (m0 + r < a.M && k0 + k < kend) v = ((const T*)a.A)[AKC ? (m0 + r) * a.lda + k0 + k : (k0 + k) * a.lda + m0 + r];
+            *(T*)(As + r * GROW + k * ES) = v;
+        }
+        for (int i = tid; i < GT * KB; i += 256) {
+            const int r = BKC ? i / KB : i % GT, k = BKC ? i % KB : i / GT;
+            T v = (T)0.f;
+            if (n0 + r < a.N && k0 + k < kend) v = ((const T*)a.B)[BKC ? (n0 + r) * a.ldb + k0 + k : (k0 + k) * a.ldb + n0 + r];
+            *(T*)(Bs + r * GROW + k * ES) = v;
+        }
+        __syncthreads();
+        u32x4 fa[2], fb[2];
 #pragma unroll
-            for (int p = 0; p < P; ++p)
+        for (int i = 0; i < 2; ++i) {
+            fa[i] = *(const u32x4*)(As + (wm + i * 16 + l15) * GROW + g * 16);
+            fb[i] = *(const u32x4*)(Bs + (wn + i * 16 + l15) * GROW + g * 16);
+        }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[p][e] = lin_act(v[p][e], A);
-        };
-        if (a.act == LIN_SILU) activate(std::integral_constant<int, LIN_SILU>{});
-        else if (a.act == LIN_RELU) activate(std::integral_constant<int, LIN_RELU>{});
-        else if (a.act == LIN_GELU) activate(std::integral_constant<int, LIN_GELU>{});
-        put((T*)a.C, a.ldc);
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if constexpr (ES == 2) {
+                    acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fb[j]),
+                                                                        __builtin_bit_cast(bf16x8, fa[i]), acc[j][i], 0, 0, 0);
+                } else {
+                    const f32x4 va = __builtin_bit_cast(f32x4, fa[i]), vb = __builtin_bit_cast(f32x4, fb[j]);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        acc[j][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(vb[q], va[q], acc[j][i], 0, 0, 0);
+                }
+            }
+    }
+    const long np = (a.N + 7) & ~7L;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const long m = m0 + wm + i * 16 + l15;
+        if (m >= a.M) continue;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const long n = n0 + wn + j * 16 + g * 4 + r;
+                if (n >= a.N) continue;
+                float v = acc[j][i][r];
+                if (a.part) {
+                    a.part[((long)z * a.M + m) * np + n] = v;
+                    continue;
+                }
+                if (a.bias) v += a.bias[n];
+                if (a.res) v += (float)((const T*)a.res)[m * a.ldr + n];
+                if (a.pre) ((T*)a.pre)[m * a.ldp + n] = (T)v;
+                ((T*)a.C)[m * a.ldc + n] = (T)lin_act(v, a.act);
+            }
     }
 }
 
 // joins the parts of a split contraction, in order, and finishes
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a, int parts) {
+    constexpr int V = RowVec<T>::N;
     const long np = (a.N + 7) & ~7L, pieces = np / 8;
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
     if (i >= a.M * pieces) return;
     const long m = i / pieces, n = (i - m * pieces) * 8;
-    float bias[8], v[8] = {};
-    gemm_bias(a, n, bias);
+    const int left = a.N - n < 8 ? (int)(a.N - n) : 8;
+    float v[8];
+    gemm_bias(a, n, v);
     const float* p = a.part + m * np + n;
+    float s[8] = {};
     for (int z = 0; z < parts; ++z, p += a.M * np) {
         const f32x4 lo = *(const f32x4*)p, hi = *(const f32x4*)(p + 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            v[e] += lo[e];
-            v[4 + e] += hi[e];
+            s[e] += lo[e];
+            s[4 + e] += hi[e];
         }
     }
-    gemm_finish<T>(a, m, n, v, bias);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += s[e];
+#pragma unroll
+    for (int h = 0; h < 8; h += V) {
+        if (a.res) {
+            float r[V];
+            row_floats<T>(row_load<T>((const T*)a.res + m * a.ldr + n + h, left - h), r);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[h + e] += r[e];
+        }
+        if (a.pre) row_store<T>((T*)a.pre + m * a.ldp + n + h, left - h, v + h);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[h + e] = lin_act(v[h + e], a.act);
+        row_store<T>((T*)a.C + m * a.ldc + n + h, left - h, v + h);
+    }
 }
 
 // dz = dy act'(pre), and the column sums of dz over this workgroup's rows (part [gridDim.x][N]).  One pass over dy and pre
@@ -638,9 +750,8 @@ long gemm_part_floats(const GemmPlan& p, long M, long N) { return p.parts > 1 ? 
 template <typename T, bool AKC, bool BKC, int F, bool DMA>
 int gemm_launch(const GemmArgs& a, unsigned grid, hipStream_t s) {
     static bool done[kMaxDevices] = {};
-    constexpr int lds = 2 * gemm_stages(F, DMA) * GemmOperand<T, AKC, F>::BYTES;
-    LDM_TRY(allow_dynamic_lds((const void*)&gemm_kernel<T, AKC, BKC, F, DMA>, lds, done));
-    gemm_kernel<T, AKC, BKC, F, DMA><<<grid, 256, lds, s>>>(a);
+    LDM_TRY(allow_dynamic_lds((const void*)&gemm_kernel<T, AKC, BKC, F, DMA>, gemm_lds(F, DMA), done));
+    gemm_kernel<T, AKC, BKC, F, DMA><<<grid, 256, gemm_lds(F, DMA), s>>>(a);
     LDM_HIP(hipGetLastError());
     return LDM_OK;
 }
@@ -649,18 +760,25 @@ template <typename T, bool AKC, bool BKC>
 int gemm(GemmArgs a, float* ws, hipStream_t s) {
     if (a.M == 0 || a.N == 0) return LDM_OK;
     constexpr long V = 16 / sizeof(T);
-    auto aligned = [&](const void* p, long ld, long len) {
-        return (size_t)p % 16 == 0 && ld % V == 0 && len % V == 0 && ld <= (1L << 21);
-    };
-    const bool dma = aligned(a.A, a.lda, AKC ? a.K : a.M) && aligned(a.B, a.ldb, BKC ? a.K : a.N);
-    LDM_REQUIRE(a.lda <= (1L << 21) && a.ldb <= (1L << 21), "operand rows are more than 2^21 elements apart");
+    const long alen = AKC ? a.K : a.M, blen = BKC ? a.K : a.N;          // elements of an operand's row
+    auto aligned = [&](const void* p, long ld, long len) { return (size_t)p % 16 == 0 && ld % V == 0 && len % V == 0; };
+    const bool dma = aligned(a.A, a.lda, alen) && aligned(a.B, a.ldb, blen);
+    // the kernel's offsets within a tile are 32 bits
+    constexpr long most = 1L << 21;
+    LDM_REQUIRE(a.lda <= most && a.ldb <= most && a.ldc <= most && (!a.res || a.ldr <= most) && (!a.pre || a.ldp <= most),
+                "rows of a matrix are more than 2^21 elements apart");
     const GemmPlan p = gemm_plan(sizeof(T), a.M, a.N, a.K, dma);
     LDM_REQUIRE(p.parts == 1 || ws, "this product needs a workspace");
-    const long t = 32 * p.F, tiles = ((a.M + t - 1) / t) * ((a.N + t - 1) / t) * p.parts;
+    // rows too short for a piece, or an empty contraction, which has no row at all to read
+    const bool any = a.K == 0 || alen < V || blen < V;
+    const long t = any ? GT : 32 * p.F, tiles = ((a.M + t - 1) / t) * ((a.N + t - 1) / t) * p.parts;
     LDM_REQUIRE(tiles < (1L << 31), "more output tiles than one launch holds");
     a.kper = p.kper;
     a.part = p.parts > 1 ? ws : nullptr;
-    if (!dma && p.F == 2) LDM_TRY((gemm_launch<T, AKC, BKC, 2, false>(a, (unsigned)tiles, s)));
+    if (any) {
+        gemm_any_kernel<T, AKC, BKC><<<(unsigned)tiles, 256, 0, s>>>(a);
+        LDM_HIP(hipGetLastError());
+    } else if (!dma && p.F == 2) LDM_TRY((gemm_launch<T, AKC, BKC, 2, false>(a, (unsigned)tiles, s)));
     else if (!dma) LDM_TRY((gemm_launch<T, AKC, BKC, 4, false>(a, (unsigned)tiles, s)));
     else if (p.F == 2) LDM_TRY((gemm_launch<T, AKC, BKC, 2, true>(a, (unsigned)tiles, s)));
     else if (p.F == 4) LDM_TRY((gemm_launch<T, AKC, BKC, 4, true>(a, (unsigned)tiles, s)));
