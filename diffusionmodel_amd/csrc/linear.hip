@@ -12,26 +12,27 @@ namespace {
 
 // exp and the reciprocal by the hardware's instructions (one step of f32 each)
 __device__ __forceinline__ float lin_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
-// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and e = exp(-z^2 / 2): Abramowitz and Stegun 7.1.26, erfc(x) = poly(t) exp(-x^2) with
-// t = 1 / (1 + 0.3275911 x), off by at most 1.5e-7; the negative side takes erfc itself, without 1 - ...  A tile's epilogue
-// has few cycles for this: 12 instructions, where the library's erff would cost as much as a tile of 256 products.
-__device__ __forceinline__ float lin_phi(float z, float& e) {
-    const float x = __builtin_fabsf(z) * 0.70710678118654752f;
-    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
-    float p = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
-    p = __builtin_fmaf(t, p, 1.421413741f);
-    p = __builtin_fmaf(t, p, -0.284496736f);
-    p = __builtin_fmaf(t, p, 0.254829592f);
-    e = lin_exp(-x * x);
-    const float tail = 0.5f * t * p * e;
-    return z >= 0.f ? 1.0f - tail : tail;
+// q = (1 - erf(|z| / sqrt 2)) / 2 and e = exp(-z^2 / 2): Abramowitz and Stegun 7.1.26, erfc(x) = t poly(t) exp(-x^2) with
+// t = 1 / (1 + 0.3275911 x), off by at most 1.5e-7.  A tile's epilogue has few cycles for this: 9 instructions, where the
+// library's erff would cost as much as a tile of 256 products.
+__device__ __forceinline__ float lin_tail(float z, float& e) {
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.23164189f, __builtin_fabsf(z), 1.0f));      // 0.3275911 / sqrt 2
+    float p = __builtin_fmaf(t, 0.5307027145f, -0.7265760135f);                                         // halved
+    p = __builtin_fmaf(t, p, 0.7107068705f);
+    p = __builtin_fmaf(t, p, -0.142248368f);
+    p = __builtin_fmaf(t, p, 0.127414796f);
+    const float u = z * 0.84932180028801905f;                                                           // sqrt(log2(e) / 2)
+    e = __builtin_amdgcn_exp2f(-u * u);
+    return t * p * e;
 }
 __device__ __forceinline__ float lin_act(float v, int act) {
     if (act == LIN_SILU) return v * __builtin_amdgcn_rcpf(1.0f + lin_exp(-v));
     if (act == LIN_RELU) return v < 0.f ? 0.f : v;
     if (act == LIN_GELU) {
+        // v Phi(v) = max(v, 0) - |v| q on either side of zero; q is 0 long before |v| = 64, and 0 * infinity is avoided
         float e;
-        return v * lin_phi(v, e);
+        const float q = lin_tail(v, e), w = __builtin_fabsf(v);
+        return __builtin_fmaf(-(w > 64.f ? 64.f : w), q, v < 0.f ? 0.f : v);
     }
     return v;
 }
@@ -43,8 +44,8 @@ __device__ __forceinline__ float lin_dact(float z, int act) {
     if (act == LIN_RELU) return z > 0.f ? 1.f : 0.f;
     if (act == LIN_GELU) {
         float e;
-        const float phi = lin_phi(z, e);
-        return __builtin_fmaf(z * 0.39894228040143268f, e, phi);
+        const float q = lin_tail(z, e);
+        return __builtin_fmaf(z * 0.39894228040143268f, e, z < 0.f ? q : 1.0f - q);
     }
     return 1.f;
 }
@@ -363,48 +364,53 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         });
     };
 
-    // outputs: 16 rows at a time through LDS, so that memory sees whole rows.  One copy of the code for all row fragments
+    // outputs: 32 rows at a time through LDS, so that memory sees whole rows.  One copy of the code for all row fragments
     // (unrolled over them it would not fit the instruction cache), and no load between the stores: loads and stores count
     // together and in order, so a wait for one would be a wait for every store before it (256 x 256 outputs without a
     // residual: 11.7 us with such waits, 6.0 without).
     constexpr int LPR = F * 2, RPP = 64 / LPR, P = 16 / RPP;                       // lanes per row, rows per pass, passes
     typedef typename RowVec<T>::R R;
     constexpr int H = 8 / RowVec<T>::N;                                            // vectors of T in eight columns
-    char* tr = smem + wave * 16 * F * 64;
+    char* tr = smem + wave * 32 * F * 64;
     const int g = lane >> 4, l15 = lane & 15, c = (lane % LPR) * 8, r0 = lane / LPR;
     // slot of 16-byte piece p of row r
     auto slot = [&](int r, int p) __attribute__((always_inline)) { return (r * F * 4 + (p ^ (F == 2 ? r >> 1 : r))) * 16; };
-    auto finish = [&]() __attribute__((always_inline)) {
+    // G row fragments at a time; RES: with a residual, whose registers leave room for one
+    auto finish = [&](auto G_, auto RES) __attribute__((always_inline)) {
+        constexpr int G = G_;
         const long n = n0 + wn + c, mw = m0 + wm + r0;
+        // the row fragments i .. i + G - 1 (i a multiple of G) go to LDS
         auto spill = [&](int i) __attribute__((always_inline)) {
-            gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
-                if (i == I) gemm_for<0, F>([&](auto J) __attribute__((always_inline)) {
-                    f32x4 v = acc[I][J];
+            gemm_for<0, F / G>([&](auto I) __attribute__((always_inline)) {
+                if (i == I * G) gemm_for<0, F * G>([&](auto J) __attribute__((always_inline)) {
+                    f32x4 v = acc[I * G + J / F][J % F];
                     gemm_pick<I>(v);
-                    *(f32x4*)(tr + slot(l15, J * 4 + g)) = v;
+                    *(f32x4*)(tr + J / F * 16 * F * 64 + slot(l15, J % F * 4 + g)) = v;
                 });
             });
         };
+        // eight columns of pass p (of G P) of them
         auto take = [&](int p, float (&v)[8]) __attribute__((always_inline)) {
-            const int r = p * RPP + r0;
-            const f32x4 lo = *(const f32x4*)(tr + slot(r, c / 4)), hi = *(const f32x4*)(tr + slot(r, c / 4 + 1));
+            const int r = p % P * RPP + r0;
+            const char* t = tr + p / P * 16 * F * 64;
+            const f32x4 lo = *(const f32x4*)(t + slot(r, c / 4)), hi = *(const f32x4*)(t + slot(r, c / 4 + 1));
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 v[e] = lo[e];
                 v[4 + e] = hi[e];
             }
         };
-        if (a.part) {
+        if (!RES && a.part) {
             const long np = (a.N + 7) & ~7L;
             float* part = a.part + (long)z * a.M * np;
 #pragma unroll 1
-            for (int i = 0; i < F; ++i) {
+            for (int i = 0; i < F; i += G) {
                 spill(i);
-                float v[P][8];
+                float v[G * P][8];
 #pragma unroll
-                for (int p = 0; p < P; ++p) take(p, v[p]);
+                for (int p = 0; p < G * P; ++p) take(p, v[p]);
 #pragma unroll
-                for (int p = 0; p < P; ++p) {
+                for (int p = 0; p < G * P; ++p) {
                     const long m = mw + i * 16 + p * RPP;
                     if (m >= a.M || n >= a.N) continue;
                     *(f32x4*)(part + m * np + n) = f32x4{v[p][0], v[p][1], v[p][2], v[p][3]};
@@ -417,8 +423,8 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         gemm_bias(a, n, bias);
         const bool full = n + 8 <= a.N;         // else the piece is cut by the last column, or lies behind it
         const int rows = (int)(a.M - m0 < TILE ? a.M - m0 : TILE), rl = wm + r0;
-        R res[F][P * H];
-        if (a.res) {
+        R res[RES ? F : 1][P * H];
+        if constexpr (RES) {
             const char* rp = (const char*)a.res + (m0 * a.ldr + n0) * ES;
             const int ld = (int)a.ldr * ES;
             if (full)
@@ -428,26 +434,26 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
                     res[i][p * H + h] = *(const typename RowVec<T>::V*)(rp + (unsigned)(r * ld + (wn + c) * ES + h * 16));
                 });
         }
-        if (a.res || a.bias) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (RES || a.bias) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         gemm_for<0, 8>([&](auto E) __attribute__((always_inline)) { gemm_landed(bias[E]); });
-        if (a.res)
+        if constexpr (RES)
             gemm_for<0, F * P * H>([&](auto I) __attribute__((always_inline)) { gemm_landed(res[I / (P * H)][I % (P * H)]); });
 #pragma unroll 1
-        for (int i = 0; i < F; ++i) {
+        for (int i = 0; i < F; i += G) {
             spill(i);
-            float v[P][8];
+            float v[G * P][8];
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
+            for (int p = 0; p < G * P; ++p) {
                 take(p, v[p]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[p][e] += bias[e];
             }
-            if (a.res) {
-                gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
-                    if (i == I)
-                        gemm_for<0, P * H>([&](auto Q) __attribute__((always_inline)) {
+            if constexpr (RES) {
+                gemm_for<0, F / G>([&](auto I) __attribute__((always_inline)) {
+                    if (i == I * G)
+                        gemm_for<0, G * P * H>([&](auto Q) __attribute__((always_inline)) {
                             float r[RowVec<T>::N];
-                            R x = res[I][Q];
+                            R x = res[I * G + Q / (P * H)][Q % (P * H)];
                             gemm_pick<I>(x);
                             row_floats<T>(x, r);
 #pragma unroll
@@ -459,7 +465,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
                 char* o = (char*)out + (m0 * ld + n0) * ES;
                 const int ldb = (int)ld * ES;
 #pragma unroll
-                for (int p = 0; p < P; ++p)
+                for (int p = 0; p < G * P; ++p)
                     if (full && rl + i * 16 + p * RPP < rows) {
 #pragma unroll
                         for (int h = 0; h < H; ++h)
@@ -470,7 +476,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
             if (a.pre) put(a.pre, a.ldp);
             auto activate = [&](auto A) __attribute__((always_inline)) {
 #pragma unroll
-                for (int p = 0; p < P; ++p)
+                for (int p = 0; p < G * P; ++p)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[p][e] = lin_act(v[p][e], A);
             };
@@ -481,7 +487,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
             if (n0 + TILE > a.N && (a.N & 7)) {
                 // the piece that the last column cuts: element by element
 #pragma unroll 1
-                for (int p = 0; p < P; ++p) {
+                for (int p = 0; p < G * P; ++p) {
                     float w[8];
                     take(p, w);
                     const long m = mw + i * 16 + p * RPP;
@@ -542,7 +548,8 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     gemm_all_but<0>();
     if constexpr (F == 8) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
     __syncthreads();
-    finish();
+    if (a.res && !a.part) finish(std::integral_constant<int, F == 8 ? 1 : 2>{}, std::true_type{});
+    else finish(std::integral_constant<int, 2>{}, std::false_type{});
 }
 
 // Any sizes, strides and alignment, element by element: 64 x 64 outputs per workgroup, 64 bytes of the contraction per step.
