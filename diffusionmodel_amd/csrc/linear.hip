@@ -31,8 +31,9 @@ __device__ __forceinline__ float lin_act(float v, int act) {
     if (act == LIN_GELU) {
         // v Phi(v) = max(v, 0) - |v| q on either side of zero; q is 0 long before |v| = 64, and 0 * infinity is avoided
         float e;
-        const float q = lin_tail(v, e), w = __builtin_fabsf(v);
-        return __builtin_fmaf(-(w > 64.f ? 64.f : w), q, v < 0.f ? 0.f : v);
+        const float q = lin_tail(v, e);
+        return __builtin_fmaf(-__builtin_amdgcn_fmed3f(__builtin_fabsf(v), 0.f, 64.f), q,
+                              __builtin_amdgcn_fmed3f(v, 0.f, __builtin_inff()));
     }
     return v;
 }
@@ -150,14 +151,13 @@ template <typename T> __device__ __forceinline__ u32x4 gemm_drop(u32x4 v, int n)
     return u32x4{(unsigned)l, (unsigned)(l >> 32), (unsigned)h, (unsigned)(h >> 32)};
 }
 
-// the outputs of row m from column n to the last, fewer than eight: bias, residual, the value before the activation, the
-// activation
+// the outputs of row m from column n to the last, fewer than eight: residual, the value before the activation, the activation
 template <typename T>
-__device__ __forceinline__ void gemm_finish(const GemmArgs& a, long m, long n, const float (&v)[8], const float (&bias)[8]) {
+__device__ __forceinline__ void gemm_finish(const GemmArgs& a, long m, long n, const float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 7; ++e)
         if (n + e < a.N) {
-            float x = v[e] + bias[e];
+            float x = v[e];
             if (a.res) x += (float)((const T*)a.res)[m * a.ldr + n + e];
             if (a.pre) ((T*)a.pre)[m * a.ldp + n + e] = (T)x;
             ((T*)a.C)[m * a.ldc + n + e] = (T)lin_act(x, a.act);
@@ -194,6 +194,8 @@ template <typename V> __device__ __forceinline__ void gemm_landed(V& v) { asm vo
 // marks v as the one of branch I: branches that pick from a register array by a run-time index stay apart (merged, they
 // would make the compiler keep the array in memory)
 template <int I, typename V> __device__ __forceinline__ void gemm_pick(V& v) { asm volatile("; %1" : "+v"(v) : "n"(I)); }
+// the same for a value in accumulation registers, which LDS takes as they are
+template <int I, typename V> __device__ __forceinline__ void gemm_pick_acc(V& v) { asm volatile("; %1" : "+a"(v) : "n"(I)); }
 __device__ __forceinline__ void gemm_mfma_in_place(f32x4& c, const u32x4& a, const u32x4& b) {
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
@@ -213,6 +215,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     typedef GemmOperand<T, BKC, F> OB;
     constexpr int ES = sizeof(T), V = 16 / ES, TILE = 32 * F, BK = OA::BK, NP = OA::NP, STAGE = OA::BYTES;
     constexpr int NS = gemm_stages(F, DMA);
+    typedef typename RowVec<T>::R R;
     constexpr int SETS = !DMA && F == 2 ? 2 : 1;          // register sets (more do not fit a tile of 128)
     extern __shared__ __attribute__((aligned(1024))) char smem[];       // [A: NS stages][B: NS stages], then the epilogue's
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -242,25 +245,37 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     int kleft = klen, rstage = 0;
     const int rowa = OA::first_row(wave, lane), rowb = OB::first_row(wave, lane);
     constexpr unsigned NONE = 0x80000000u;
-    unsigned va[DMA ? NP : 1], vb[DMA ? NP : 1];         // offsets from the step's start
-    if constexpr (DMA)
+    unsigned va[NP], vb[NP];             // byte offsets from the step's start (through registers: signed)
+    // Direct loads: pieces outside the matrix have none.  Through registers: a row no further than the last, a piece no
+    // further than the end of its row, which may lie before the step's start (write() moves it into place).  The end of
+    // the contraction counts when the last step, or none, is asked for: a branch that two or three steps take, instead of
+    // comparisons per piece in all of them.
+    auto upto = [](int v, int most) __attribute__((always_inline)) { return v < most ? v : most; };
+    auto offsets = [&]() __attribute__((always_inline)) {
         gemm_for<0, NP>([&](auto Q) __attribute__((always_inline)) {
             constexpr int q = Q;
             const int ya = rowa + q * OA::ROWS, xa = OA::element(wave, q, lane);
             const int yb = rowb + q * OB::ROWS, xb = OB::element(wave, q, lane);
-            va[q] = (AKC ? ya : xa) < arows ? (unsigned)(ya * (int)a.lda + xa) * ES : NONE;
-            vb[q] = (BKC ? yb : xb) < brows ? (unsigned)(yb * (int)a.ldb + xb) * ES : NONE;
+            const int enda = AKC ? arows : kleft, enda_x = AKC ? kleft : arows;        // rows, elements of a row
+            const int endb = BKC ? brows : kleft, endb_x = BKC ? kleft : brows;
+            if constexpr (DMA) {
+                va[q] = ya < enda && xa < enda_x ? (unsigned)(ya * (int)a.lda + xa) * ES : NONE;
+                vb[q] = yb < endb && xb < endb_x ? (unsigned)(yb * (int)a.ldb + xb) * ES : NONE;
+            } else {
+                // (nothing left: the first elements of the matrix, which are not used)
+                va[q] = kleft > 0 ? (unsigned)((upto(ya, enda - 1) * (int)a.lda + upto(xa, enda_x - V)) * ES) : 0;
+                vb[q] = kleft > 0 ? (unsigned)((upto(yb, endb - 1) * (int)a.ldb + upto(xb, endb_x - V)) * ES) : 0;
+            }
         });
-    // the pieces behind the end of the contraction leave the offsets when the last step, or none, is asked for: a branch
-    // that two or three steps take, instead of a comparison per piece in all of them
+    };
     auto narrow = [&]() __attribute__((always_inline)) {
-        if (DMA && kleft < BK) {
+        if (kleft < BK) {
             asm volatile("" ::: "memory");
-            gemm_for<0, NP>([&](auto Q) __attribute__((always_inline)) {
-                constexpr int q = Q;
-                if ((AKC ? OA::element(wave, q, lane) : rowa + q * OA::ROWS) >= kleft) va[q] = NONE;
-                if ((BKC ? OB::element(wave, q, lane) : rowb + q * OB::ROWS) >= kleft) vb[q] = NONE;
-            });
+            offsets();
+            if (!DMA && kleft <= 0) {
+                ap = (const char*)a.A;
+                bp = (const char*)a.B;
+            }
         }
     };
     u32x4 ra[SETS][DMA ? 1 : NP], rb[SETS][DMA ? 1 : NP];
@@ -275,17 +290,8 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
             gemm_dma(bp, la + NS * STAGE, vb[q]);
         } else {
             typedef typename RowVec<T>::V U;
-            const bool live = kleft > 0;
-            const char* pa = live ? ap : (const char*)a.A;
-            const char* pb = live ? bp : (const char*)a.B;
-            // KC: the row no further than the last, the piece no further than the end of k; else the other way round
-            auto upto = [](int v, int most) __attribute__((always_inline)) { return v < most ? v : most; };
-            const int ya = rowa + q * OA::ROWS, xa = OA::element(wave, q, lane), yb = rowb + q * OB::ROWS, xb = OB::element(wave, q, lane);
-            const int ra_ = live ? upto(ya, (AKC ? arows : kleft) - 1) : 0, ca = live ? upto(xa, (AKC ? kleft : arows) - V) : 0;
-            const int rb_ = live ? upto(yb, (BKC ? brows : kleft) - 1) : 0, cb = live ? upto(xb, (BKC ? kleft : brows) - V) : 0;
-            const long ea = (long)ra_ * a.lda + ca, eb = (long)rb_ * a.ldb + cb;
-            ra[S][q] = __builtin_bit_cast(u32x4, (typename RowVec<T>::R)*(const U*)(pa + ea * ES));
-            rb[S][q] = __builtin_bit_cast(u32x4, (typename RowVec<T>::R)*(const U*)(pb + eb * ES));
+            ra[S][q] = __builtin_bit_cast(u32x4, (R)*(const U*)(ap + (int)va[q]));
+            rb[S][q] = __builtin_bit_cast(u32x4, (R)*(const U*)(bp + (int)vb[q]));
         }
     };
     auto requested = [&](auto S) __attribute__((always_inline)) {       // the step is complete: on to the next
@@ -369,7 +375,6 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     // together and in order, so a wait for one would be a wait for every store before it (256 x 256 outputs without a
     // residual: 11.7 us with such waits, 6.0 without).
     constexpr int LPR = F * 2, RPP = 64 / LPR, P = 16 / RPP;                       // lanes per row, rows per pass, passes
-    typedef typename RowVec<T>::R R;
     constexpr int H = 8 / RowVec<T>::N;                                            // vectors of T in eight columns
     char* tr = smem + wave * 32 * F * 64;
     const int g = lane >> 4, l15 = lane & 15, c = (lane % LPR) * 8, r0 = lane / LPR;
@@ -384,7 +389,8 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
             gemm_for<0, F / G>([&](auto I) __attribute__((always_inline)) {
                 if (i == I * G) gemm_for<0, F * G>([&](auto J) __attribute__((always_inline)) {
                     f32x4 v = acc[I * G + J / F][J % F];
-                    gemm_pick<I>(v);
+                    if constexpr (F == 8) gemm_pick_acc<I>(v);
+                    else gemm_pick<I>(v);
                     *(f32x4*)(tr + J / F * 16 * F * 64 + slot(l15, J % F * 4 + g)) = v;
                 });
             });
@@ -419,8 +425,6 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
             }
             return;
         }
-        float bias[8];
-        gemm_bias(a, n, bias);
         const bool full = n + 8 <= a.N;         // else the piece is cut by the last column, or lies behind it
         const int rows = (int)(a.M - m0 < TILE ? a.M - m0 : TILE), rl = wm + r0;
         R res[RES ? F : 1][P * H];
@@ -434,20 +438,16 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
                     res[i][p * H + h] = *(const typename RowVec<T>::V*)(rp + (unsigned)(r * ld + (wn + c) * ES + h * 16));
                 });
         }
-        if (RES || a.bias) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        gemm_for<0, 8>([&](auto E) __attribute__((always_inline)) { gemm_landed(bias[E]); });
-        if constexpr (RES)
+        if constexpr (RES) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             gemm_for<0, F * P * H>([&](auto I) __attribute__((always_inline)) { gemm_landed(res[I / (P * H)][I % (P * H)]); });
+        }
 #pragma unroll 1
         for (int i = 0; i < F; i += G) {
             spill(i);
             float v[G * P][8];
 #pragma unroll
-            for (int p = 0; p < G * P; ++p) {
-                take(p, v[p]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[p][e] += bias[e];
-            }
+            for (int p = 0; p < G * P; ++p) take(p, v[p]);
             if constexpr (RES) {
                 gemm_for<0, F / G>([&](auto I) __attribute__((always_inline)) {
                     if (i == I * G)
@@ -491,7 +491,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
                     float w[8];
                     take(p, w);
                     const long m = mw + i * 16 + p * RPP;
-                    if (m < a.M && n < a.N && !full) gemm_finish<T>(a, m, n, w, bias);
+                    if (m < a.M && n < a.N && !full) gemm_finish<T>(a, m, n, w);
                 }
             }
         }
@@ -503,7 +503,13 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         gemm_for<0, NP>([&](auto Q) __attribute__((always_inline)) { request(Q, S); });
         requested(S);
     };
-    narrow();
+    f32x4 bias[F];
+    const int bias_left = a.bias && !a.part ? upto(brows, TILE) : 0;
+    gemm_for<0, F>([&](auto J) __attribute__((always_inline)) {
+        const int at = wn + J * 16 + (lane >> 4) * 4;
+        bias[J] = row_load<float>(a.bias + n0 + at, bias_left - at);
+    });
+    offsets();
     if constexpr (DMA) {
         for (int t = 0; t < NS; ++t) ask(c0);
         gemm_all_but<(NS - 1) * 2 * NP>();
@@ -516,7 +522,10 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     }
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    gemm_for<0, F * F>([&](auto I) __attribute__((always_inline)) { acc[I / F][I % F] = f32x4{0.f, 0.f, 0.f, 0.f}; });
+    // the sums start from the bias (the parts of a split contraction from zero)
+    gemm_for<0, F * F>([&](auto I) __attribute__((always_inline)) {
+        acc[I / F][I % F] = bias[I % F];
+    });
     gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
         OA::template read<I, 0>(fa[0][I], aa[0]);
         OB::template read<I, 0>(fb[0][I], bb[0]);
@@ -738,7 +747,7 @@ GemmPlan gemm_plan(int es, long M, long N, long K, bool dma) {
     double least = 1e30;
     for (int i = 0; i < n; ++i) {
         const long t = 32 * costs[i].F, tiles = ((M + t - 1) / t) * ((N + t - 1) / t);
-        for (long want = 1; want <= 64 && want <= steps; want *= 2) {
+        for (long want = 1; want <= 64 && want <= steps; ++want) {
             const long kper = (steps + want - 1) / want, parts = (steps + kper - 1) / kper;
             const long per_cu = (tiles * parts + 255) / 256;
             double us = per_cu <= 1 ? costs[i].fixed + kper * costs[i].lone : per_cu * (costs[i].fixed + kper * costs[i].busy);
