@@ -31,6 +31,7 @@ struct RopeArgs {
     int inverse;
     int nrot, nchunk, tpb, hpg;    // set by launch_rope
     unsigned groups;
+    bool through;
 };
 int launch_rope(int dtype, int interleaved, RopeArgs a, hipStream_t s);
 
@@ -48,6 +49,7 @@ struct GemmArgs {
     int act;
     float* part;                   // set by launch_gemm: partial sums [parts][M][N rounded up to 8] of a split contraction
     int kper;                      // set by launch_gemm: steps of the contraction per part
+    bool through;                  // set by launch_gemm: outputs are written through the L2
 };
 long gemm_ws_floats(int dtype, long M, long N, long K);
 int launch_gemm(int dtype, const GemmArgs& a, bool akc, bool bkc, float* ws, hipStream_t s);

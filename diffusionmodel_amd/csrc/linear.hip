@@ -470,7 +470,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
 #pragma unroll
                         for (int h = 0; h < H; ++h)
                             row_store<T>((T*)(o + (unsigned)((rl + i * 16 + p * RPP) * ldb + (wn + c) * ES + h * 16)), RowVec<T>::N,
-                                         v[p] + h * RowVec<T>::N);
+                                         v[p] + h * RowVec<T>::N, ES == 2 && a.through);
                     }
             };
             if (a.pre) put(a.pre, a.ldp);
@@ -790,6 +790,9 @@ int gemm(GemmArgs a, float* ws, hipStream_t s) {
     const long t = any ? GT : 32 * p.F, tiles = ((a.M + t - 1) / t) * ((a.N + t - 1) / t) * p.parts;
     LDM_REQUIRE(tiles < (1L << 31), "more output tiles than one launch holds");
     a.kper = p.kper;
+    // bf16: a lane's eight columns are one access, and a row's lanes cover whole lines
+    a.through = sizeof(T) == 2 && a.M * a.N * (a.pre ? 4 : 2) <= kThroughBytes && a.N % 64 == 0 && a.ldc % 64 == 0 &&
+                (size_t)a.C % 128 == 0 && (!a.pre || (a.ldp % 64 == 0 && (size_t)a.pre % 128 == 0));
     a.part = p.parts > 1 ? ws : nullptr;
     if (any) {
         gemm_any_kernel<T, AKC, BKC><<<(unsigned)tiles, 256, 0, s>>>(a);

@@ -49,24 +49,17 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
     int e0, e1, n0, n1;
     const bool rot = chunk < a.nrot;
     const int j0 = chunk * N;
-    if (rot) {
-        const int np = a.P - j0 < N ? a.P - j0 : N;
-        if constexpr (INTER) {
-            e0 = 2 * j0;
-            n0 = 2 * np < N ? 2 * np : N;
-            e1 = e0 + N;
-            n1 = 2 * np - n0;
-        } else {
-            e0 = j0;
-            e1 = a.P + j0;
-            n0 = n1 = np;
-        }
+    // (pairs side by side: two vectors that stand half a head apart, so that the lanes of each access are neighbours)
+    if (rot && !INTER) {
+        e0 = j0;
+        e1 = a.P + j0;
+        n0 = n1 = a.P - j0;
     } else {
-        const int c0 = 2 * a.P + (chunk - a.nrot) * 2 * N, np = a.D - c0;
-        e0 = c0;
-        e1 = c0 + N;
-        n0 = np < N ? np : N;
-        n1 = np - n0 < N ? np - n0 : N;
+        const int first = rot ? 0 : 2 * a.P, last = rot ? 2 * a.P : a.D, half = rot ? a.nrot : a.nchunk - a.nrot;
+        e0 = first + (rot ? chunk : chunk - a.nrot) * N;
+        e1 = e0 + half * N;
+        n0 = last - e0;
+        n1 = last - e1;
     }
     // four heads at a time: the next four are on their way while these are turned, the first while the angles are taken
     const int heads = a.H[0] + a.H[1], h0 = grp * a.hpg, hend = h0 + a.hpg < heads ? h0 + a.hpg : heads;
@@ -93,11 +86,19 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
                      : a.pos_dtype == 1 ? (double)((const long*)a.pos)[po] : (double)((const float*)a.pos)[po];
         }
         float f[N];
+        // the pairs' numbers: j0 .. j0 + N - 1, or half of them from each vector
+        const int j1 = INTER ? e0 / 2 : j0, j2 = INTER ? e1 / 2 - N / 2 : j0;
 #pragma unroll
-        for (int i = 0; i < N; i += 4) row_floats<float>(row_load<float>(a.inv_freq + j0 + i, a.P - j0 - i), f + i);
+        for (int i = 0; i < N; i += INTER ? N / 2 : 4) {
+            const int j = (i < N / 2 ? j1 : j2) + i, most = INTER ? N / 2 : 4;
+            float t[4];
+            row_floats<float>(row_load<float>(a.inv_freq + j, a.P - j < most ? a.P - j : most), t);
+#pragma unroll
+            for (int e = 0; e < most; ++e) f[i + e] = t[e];
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int j = j0 + i;
+            const int j = (i < N / 2 ? j1 : j2) + i;
             const double p = j < a.sec_end[0] ? pos[0] : j < a.sec_end[1] ? pos[1] : j < a.sec_end[2] ? pos[2] : pos[3];
             const double turns = p * (double)f[i] * 0.15915494309189533577;
             turn_sincos(a.inverse ? -turns : turns, sn[i], cs[i]);
@@ -138,8 +139,8 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
                     }
                 }
             }
-            row_store<T>(dst + e0, n0, u);
-            row_store<T>(dst + e1, n1, v);
+            row_store<T>(dst + e0, n0, u, a.through);
+            row_store<T>(dst + e1, n1, v, a.through);
         }
     }
 }
@@ -149,18 +150,22 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
 int launch_rope(int dtype, int interleaved, RopeArgs a, hipStream_t s) {
     const int N = dtype == LDM_BF16 ? 8 : 4;
     if (a.tokens == 0) return LDM_OK;
-    a.nrot = (a.P + N - 1) / N;
+    a.nrot = interleaved ? ((2 * a.P + N - 1) / N + 1) / 2 : (a.P + N - 1) / N;      // two vectors a thread
     a.nchunk = a.nrot + (a.D - 2 * a.P + 2 * N - 1) / (2 * N);
     a.tpb = 256 / a.nchunk;
     // a group of heads per workgroup, all of them where the tokens alone give eight workgroups per CU: the angles are taken
     // once for a group.  2 x 8192 tokens, 20 heads of 128 in f32: 76.8 us in two groups of ten, 80.4 in one, 78.1 in four
     // (and 100.6 with a workgroup per head); one token, 8 heads of 64: 5.2 us in four groups, 7.4 in one
-    const int heads = a.H[0] + a.H[1];
+    const int heads = a.H[0] + a.H[1], es = dtype == LDM_BF16 ? 2 : 4;
     const long blocks = (a.tokens + a.tpb - 1) / a.tpb;
         long groups = 2048 / blocks;
     groups = groups < 1 ? 1 : groups > (heads + 1) / 2 ? (heads + 1) / 2 : groups;
     a.hpg = (int)((heads + groups - 1) / groups);
     a.groups = (unsigned)((heads + a.hpg - 1) / a.hpg);
+    // written through where each access of the lanes covers half lines at least (the second access fills them)
+    a.through = a.tokens * heads * a.D * es <= kThroughBytes && (interleaved ? 2 : 1) * a.P * es % 64 == 0 && a.D * es % 64 == 0;
+    for (int w = 0; w < 2 && a.H[w]; ++w)
+        a.through = a.through && ((size_t)a.out[w] | (size_t)(a.osb[w] * es) | (size_t)(a.osn[w] * es) | (size_t)(a.osh[w] * es)) % 64 == 0;
     LDM_REQUIRE(blocks * a.groups < (1L << 31), "too many tokens and heads for one launch");
     const unsigned grid = (unsigned)(blocks * a.groups);
     if (dtype == LDM_BF16) {

@@ -4,6 +4,11 @@
 
 namespace ldm {
 
+// Whether an output of `bytes` is written through: what the caches hold of it at the end of a launch is at most some 32 MB,
+// a few us; against large outputs that is nothing and the detour costs (65536 x 1024 bf16 behind a product: 1 % slower,
+// 16384 x 1024 with its value before the activation 6 % faster).
+constexpr long kThroughBytes = 96L << 20;
+
 // N elements of T as one 16-byte access.  The rows of a slice are element aligned only; this target's global memory serves
 // such accesses at any address that the element allows.
 template <typename T> struct RowVec;
@@ -33,15 +38,23 @@ __device__ __forceinline__ typename RowVec<T>::R row_load(const T* p, int n) {
     }
     return v;
 }
+// 16 bytes, written through: nothing dirty is left in this XCD's L2 for the end of the launch, which would have to write it
+// back before the next launch starts.  Only for stores that cover whole lines at once: partial ones go to memory one by one
+// (20011 rows of 1031 f32: 67 us against 34 written back).  The s_nop keeps the data registers until the store has read
+// them: the compiler does not know the instruction.
+template <typename R> __device__ __forceinline__ void store_through(void* p, const R& v) {
+    asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" ::"v"(p), "v"(v) : "memory");
+}
 template <typename T>
-__device__ __forceinline__ void row_store(T* p, int n, const float* o) {
+__device__ __forceinline__ void row_store(T* p, int n, const float* o, bool through = false) {
     constexpr int N = RowVec<T>::N;
     typename RowVec<T>::F f;
 #pragma unroll
     for (int e = 0; e < N; ++e) f[e] = o[e];
     const typename RowVec<T>::R v = __builtin_convertvector(f, typename RowVec<T>::R);
     if (n >= N) {
-        *(typename RowVec<T>::V*)p = v;
+        if (through) store_through(p, v);
+        else *(typename RowVec<T>::V*)p = v;
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e)
