@@ -105,15 +105,17 @@ template <> struct GemmFrag<float, false> {
 // One operand's tile: where its pieces lie in memory and LDS.
 //   KC:   LDS row r (of TILE) holds 128 bytes of the contraction, piece p at slot p ^ ((r >> 1) & 7)
 //   else: LDS row k (of BK) holds TILE elements; bf16: 32-byte chunk c at c ^ ((k & 3) + 4 ((k >> 3) & 1)), in rows of only
-//         four chunks at c ^ (((k >> 1) & 1) + 2 ((k >> 3) & 1)); f32: 64-byte chunk c at c ^ ((k >> 2) & 3)
+//         four chunks at c ^ (((k >> 1) & 1) + 2 ((k >> 3) & 1)), of two at c ^ ((k >> 3) & 1); f32: 64-byte chunk c at
+//         c ^ ((k >> 2) & 3), in rows of two chunks at c ^ ((k >> 2) & 1)
 template <typename T, bool KC, int F> struct GemmOperand {
     static constexpr int ES = sizeof(T), TILE = 32 * F, BK = 128 / ES, BYTES = TILE * 128;
     static constexpr int RB = KC ? 128 : TILE * ES;          // bytes of an LDS row
     static constexpr int NP = BYTES / 4096;                  // pieces per lane and step
 
     static constexpr int turn(int k) {
-        return RB == 128 ? ((k >> 1) & 1) | (((k >> 3) & 1) << 1) : (k & 3) | (((k >> 3) & 1) << 2);
+        return RB == 64 ? (k >> 3) & 1 : RB == 128 ? ((k >> 1) & 1) | (((k >> 3) & 1) << 1) : (k & 3) | (((k >> 3) & 1) << 2);
     }
+    static constexpr int turn32(int k) { return (k >> 2) & (RB == 128 ? 1 : 3); }
     // fragment f (16 rows / columns from w0 + 16 f) of half step s: the address without the parts that are immediate
     static __device__ __forceinline__ unsigned base(int lane, int w0, int s) {
         const int l15 = lane & 15, g = lane >> 4;
@@ -123,7 +125,7 @@ template <typename T, bool KC, int F> struct GemmOperand {
             const int row = g * 8 + (l15 >> 2);
             return row * RB + (((w0 >> 4) ^ turn(row)) << 5) + (l15 & 3) * 8;
         } else {
-            return (g * 4) * RB + (((w0 >> 4) ^ g) << 6) + l15 * 4;
+            return (g * 4) * RB + (((w0 >> 4) ^ turn32(g * 4)) << 6) + l15 * 4;
         }
     }
     template <int f, int s> static __device__ __forceinline__ void read(GemmFrag<T, KC>& fr, unsigned b) {
@@ -137,7 +139,7 @@ template <typename T, bool KC, int F> struct GemmOperand {
     static __device__ __forceinline__ int first_row(int w, int lane) { return w * NP * ROWS + lane / (RB / 16); }
     static __device__ __forceinline__ int element(int w, int q, int lane) {
         const int p = lane % (RB / 16), row = w * NP * ROWS + q * ROWS + lane / (RB / 16);
-        const int x = KC ? p ^ ((row >> 1) & 7) : ES == 2 ? p ^ (turn(row) << 1) : p ^ (((row >> 2) & 3) << 2);
+        const int x = KC ? p ^ ((row >> 1) & 7) : ES == 2 ? p ^ (turn(row) << 1) : p ^ (turn32(row) << 2);
         return x * (16 / ES);
     }
 };
@@ -561,6 +563,117 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     else finish(std::integral_constant<int, 2>{}, std::false_type{});
 }
 
+// Few rows: the weights are read once and that is all there is to do, so the contraction is split over the waves of a
+// workgroup and joined in LDS, without a second launch.  A workgroup computes 32 x 32 outputs; its wave w takes the steps
+// w, w + 4, ... of the contraction and keeps four of them on the way in LDS of its own, with no barrier before the end.
+template <typename T, bool BKC>
+__global__ __launch_bounds__(256) void gemm_few_kernel(GemmArgs a) {
+    typedef GemmOperand<T, true, 1> OA;
+    typedef GemmOperand<T, BKC, 1> OB;
+    constexpr int ES = sizeof(T), BK = OA::BK, NS = 4, Q = OA::BYTES / 1024;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];       // per wave: [A: NS steps][B: NS steps]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    char* mine = smem + wave * 2 * NS * OA::BYTES;
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)mine;
+    const unsigned ntm = (unsigned)((a.M + 31) / 32);
+    const long m0 = (long)(blockIdx.x % ntm) * 32, n0 = (long)(blockIdx.x / ntm) * 32;
+    const int arows = (int)(a.M - m0 < 32 ? a.M - m0 : 32), brows = (int)(a.N - n0 < 32 ? a.N - n0 : 32);
+    const int steps = (int)((a.K + BK - 1) / BK), nt = (steps - wave + 3) / 4;
+    const char* ap = (const char*)a.A + m0 * a.lda * ES + wave * 128;
+    const char* bp = (const char*)a.B + (BKC ? n0 * a.ldb * ES + wave * 128 : ((long)wave * BK * a.ldb + n0) * ES);
+    const long astep = 512, bstep = BKC ? 512 : 4 * a.ldb * BK * ES;
+    int kleft = (int)a.K - wave * BK;
+    constexpr unsigned NONE = 0x80000000u;
+    unsigned va[Q], vb[Q];
+    auto offsets = [&]() __attribute__((always_inline)) {
+        gemm_for<0, Q>([&](auto I) __attribute__((always_inline)) {
+            constexpr int q = I;
+            const int ya = OA::first_row(0, lane) + q * OA::ROWS, xa = OA::element(0, q, lane);
+            const int yb = OB::first_row(0, lane) + q * OB::ROWS, xb = OB::element(0, q, lane);
+            va[q] = ya < arows && xa < kleft ? (unsigned)(ya * (int)a.lda + xa) * ES : NONE;
+            vb[q] = yb < (BKC ? brows : kleft) && xb < (BKC ? kleft : brows) ? (unsigned)(yb * (int)a.ldb + xb) * ES : NONE;
+        });
+    };
+    auto request = [&](int t) __attribute__((always_inline)) {
+        if (kleft < BK) {
+            asm volatile("" ::: "memory");
+            offsets();
+        }
+        char* la = mine + (t & (NS - 1)) * OA::BYTES;
+        gemm_for<0, Q>([&](auto I) __attribute__((always_inline)) {
+            gemm_dma(ap, la + I * 1024, va[I]);
+            gemm_dma(bp, la + NS * OA::BYTES + I * 1024, vb[I]);
+        });
+        kleft -= 4 * BK;
+        ap += astep;
+        bp += bstep;
+    };
+    f32x4 acc[2][2] = {};                 // [row fragment][column fragment]
+    GemmFrag<T, true> fa[2][2];
+    GemmFrag<T, BKC> fb[2][2];
+    const unsigned aa[2] = {lds0 + OA::base(lane, 0, 0), lds0 + OA::base(lane, 0, 1)};
+    const unsigned bb[2] = {lds0 + NS * OA::BYTES + OB::base(lane, 0, 0), lds0 + NS * OA::BYTES + OB::base(lane, 0, 1)};
+    offsets();
+    for (int t = 0; t < NS; ++t) request(t);
+    for (int t = 0; t < nt; ++t) {
+        gemm_all_but<(NS - 1) * 2 * Q>();
+        const unsigned st = (t & (NS - 1)) * OA::BYTES;
+        gemm_for<0, 2>([&](auto S) __attribute__((always_inline)) {
+            gemm_for<0, 2>([&](auto I) __attribute__((always_inline)) {
+                OA::template read<I, S>(fa[S][I], aa[S] + st);
+                OB::template read<I, S>(fb[S][I], bb[S] + st);
+            });
+        });
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        gemm_for<0, 2>([&](auto S) __attribute__((always_inline)) {
+            gemm_for<0, 2>([&](auto I) __attribute__((always_inline)) {
+                fa[S][I].landed();
+                fb[S][I].landed();
+            });
+        });
+        request(t + NS);
+        gemm_for<0, 8>([&](auto I) __attribute__((always_inline)) {
+            constexpr int h = I / 4, i = I / 2 % 2, j = I % 2;
+            if constexpr (ES == 2) {
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fb[h][j].bits()),
+                                                                    __builtin_bit_cast(bf16x8, fa[h][i].bits()), acc[i][j], 0, 0, 0);
+            } else {
+                gemm_for<0, 4>([&](auto E) __attribute__((always_inline)) {
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[h][j].f32(E), fa[h][i].f32(E), acc[i][j], 0, 0, 0);
+                });
+            }
+        });
+    }
+    gemm_all_but<0>();                    // nothing is on its way into LDS any more
+    __syncthreads();
+    // the waves' sums, 32 x 32 each (rows of 36 floats), then four columns per thread
+    float* join = (float*)smem;
+    constexpr int ROW = 36;
+    const int g = lane >> 4, l15 = lane & 15;
+    gemm_for<0, 4>([&](auto I) __attribute__((always_inline)) {
+        constexpr int i = I / 2, j = I % 2;
+        *(f32x4*)(join + (wave * 32 + i * 16 + l15) * ROW + j * 16 + g * 4) = acc[i][j];
+    });
+    __syncthreads();
+    const int r = tid / 8, c = (tid % 8) * 4, left = brows - c;
+    if (r >= arows || left <= 0) return;
+    const long m = m0 + r, n = n0 + c;
+    float v[4];
+    row_floats<float>(row_load<float>(a.bias + n, a.bias ? left : 0), v);
+    for (int w = 0; w < 4; ++w) {
+        const f32x4 p = *(const f32x4*)(join + (w * 32 + r) * ROW + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += p[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e < left) {
+            if (a.res) v[e] += (float)((const T*)a.res)[m * a.ldr + n + e];
+            if (a.pre) ((T*)a.pre)[m * a.ldp + n + e] = (T)v[e];
+            ((T*)a.C)[m * a.ldc + n + e] = (T)lin_act(v[e], a.act);
+        }
+}
+
 // Any sizes, strides and alignment, element by element: 64 x 64 outputs per workgroup, 64 bytes of the contraction per step.
 // Serves the products with an operand whose rows are shorter than one 16-byte piece.
 constexpr int GT = 64, GROW = 64 + 16;      // bytes of an LDS row: 64 of data, padded against bank conflicts
@@ -772,6 +885,11 @@ int gemm_launch(const GemmArgs& a, unsigned grid, hipStream_t s) {
     return LDM_OK;
 }
 
+// products for gemm_few_kernel: up to 64 rows, and in bf16 at most 16 MB of weights, whose rows it reads in pieces of 64
+// bytes (us, against the 64 tile; [K, N] weights): 4 rows bf16 2048 x 256: 5.6 / 12.9, 1024 x 1024: 6.0 / 6.7, 4096 x 4096:
+// 20.0 / 13.8; f32 2048 x 256: 13.0 / 21.5, 4096 x 4096: 24.3 / 27.4
+bool gemm_is_few(int es, long M, long N, long K) { return M <= 64 && (es == 4 || K * N <= (1L << 23)); }
+
 template <typename T, bool AKC, bool BKC>
 int gemm(GemmArgs a, float* ws, hipStream_t s) {
     if (a.M == 0 || a.N == 0) return LDM_OK;
@@ -783,6 +901,17 @@ int gemm(GemmArgs a, float* ws, hipStream_t s) {
     constexpr long most = 1L << 21;
     LDM_REQUIRE(a.lda <= most && a.ldb <= most && a.ldc <= most && (!a.res || a.ldr <= most) && (!a.pre || a.ldp <= most),
                 "rows of a matrix are more than 2^21 elements apart");
+    if constexpr (AKC)
+        if (dma && gemm_is_few(sizeof(T), a.M, a.N, a.K)) {
+            static bool done[kMaxDevices] = {};
+            constexpr int lds = 4 * 2 * 4 * 4096;
+            LDM_TRY(allow_dynamic_lds((const void*)&gemm_few_kernel<T, BKC>, lds, done));
+            const long grid = (a.M + 31) / 32 * ((a.N + 31) / 32);
+            LDM_REQUIRE(grid < (1L << 31), "more output tiles than one launch holds");
+            gemm_few_kernel<T, BKC><<<(unsigned)grid, 256, lds, s>>>(a);
+            LDM_HIP(hipGetLastError());
+            return LDM_OK;
+        }
     const GemmPlan p = gemm_plan(sizeof(T), a.M, a.N, a.K, dma);
     LDM_REQUIRE(p.parts == 1 || ws, "this product needs a workspace");
     // rows too short for a piece, or an empty contraction, which has no row at all to read
