@@ -893,6 +893,10 @@ bool gemm_is_few(int es, long M, long N, long K) { return M <= 64 && (es == 4 ||
 template <typename T, bool AKC, bool BKC>
 int gemm(GemmArgs a, float* ws, hipStream_t s) {
     if (a.M == 0 || a.N == 0) return LDM_OK;
+    // the stride of a single row is never used, whatever it is
+    if (a.M == 1) a.ldc = a.ldr = a.ldp = 0;
+    if ((AKC ? a.M : a.K) == 1) a.lda = 0;
+    if ((BKC ? a.N : a.K) == 1) a.ldb = 0;
     constexpr long V = 16 / sizeof(T);
     const long alen = AKC ? a.K : a.M, blen = BKC ? a.K : a.N;          // elements of an operand's row
     auto aligned = [&](const void* p, long ld, long len) { return (size_t)p % 16 == 0 && ld % V == 0 && len % V == 0; };

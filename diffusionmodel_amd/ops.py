@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import operator
 import struct
 from typing import Optional, Sequence, Tuple
 
@@ -390,7 +391,10 @@ def _rope_plan(qs, sq, ks, sk, so, sok, ps, pp, P, sections, layout):
         Hk = ks[2]
     if D < 1 or Hq < 1 or (ks is not None and Hk < 1) or (D > 1 and not sq[3] == sk[3] == so[3] == sok[3] == 1):
         raise ValueError("q, k and their outputs need at least one head and contiguous head vectors")
-    sec = (P,) if sections is None else sections
+    try:
+        sec = (P,) if sections is None else tuple(operator.index(n) for n in sections)
+    except TypeError:
+        raise ValueError(f"sections must be whole numbers, got {sections}") from None
     if not 1 <= len(sec) <= 4 or min(sec) < 0 or sum(sec) != P or P < 1 or 2 * P > D:
         raise ValueError(f"sections {sec} must hold one to four counts that add up to inv_freq's {P} pairs, at most D / 2")
     if len(ps) == 2:
