@@ -44,7 +44,9 @@ __device__ __forceinline__ void ln_param(const float* p, int c, int C, float dfl
     }
 }
 
-// sums over the LPR lanes of a row, the same bits in every lane; LPR = 256: the whole workgroup, through `sm` (8 floats)
+// threads of a workgroup: rows of up to a wave share 256, longer ones have a workgroup each
+constexpr int ln_block(int lpr) { return lpr > 256 ? lpr : 256; }
+// sums over the LPR lanes of a row, the same bits in every lane; LPR > 64: the whole workgroup, through `sm` (16 floats)
 template <int LPR>
 __device__ __forceinline__ void ln_sum2(float& a, float& b, float* sm) {
     a = lanes_sum<LPR < 64 ? LPR : 64>(a);
@@ -58,6 +60,10 @@ __device__ __forceinline__ void ln_sum2(float& a, float& b, float* sm) {
         __syncthreads();
         a = (sm[0] + sm[2]) + (sm[4] + sm[6]);
         b = (sm[1] + sm[3]) + (sm[5] + sm[7]);
+        if constexpr (LPR > 256) {
+            a += (sm[8] + sm[10]) + (sm[12] + sm[14]);
+            b += (sm[9] + sm[11]) + (sm[13] + sm[15]);
+        }
     }
 }
 template <int LPR>
@@ -68,9 +74,9 @@ __device__ __forceinline__ float ln_sum(float a, float* sm) {
 }
 
 template <typename T, int NV, int LPR>
-__global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
-    constexpr int N = RowVec<T>::N, RPB = 256 / LPR;
-    __shared__ float sm[8];
+__global__ __launch_bounds__(ln_block(LPR)) void ln_fwd_kernel(LnFwdArgs a) {
+    constexpr int N = RowVec<T>::N, RPB = ln_block(LPR) / LPR;
+    __shared__ float sm[16];
     const int l = threadIdx.x % LPR;
     float w[NV][N], b[NV][N];
 #pragma unroll
@@ -101,12 +107,20 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
         const float mu = ln_sum<LPR>(s, sm) / n;
         float q = 0.f;
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+        for (int v = 0; v < NV; ++v) {
+            // (a condition per vector, not per element: those would be kept over the rows in more registers than there are)
+            const int left = a.C - (v * LPR + l) * N;
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                x[v][e] -= mu;
-                if ((v * LPR + l) * N + e < a.C) q += x[v][e] * x[v][e];
+            for (int e = 0; e < N; ++e) x[v][e] -= mu;
+            if (left >= N) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) q += x[v][e] * x[v][e];
+            } else if (left > 0) {
+                asm volatile("" ::: "memory");
+#pragma unroll
+                for (int e = 0; e < N - 1; ++e) q += e < left ? x[v][e] * x[v][e] : 0.f;
             }
+        }
         const float r = 1.0f / sqrtf(ln_sum<LPR>(q, sm) / n + a.eps);
         T* yr = (T*)a.y + row * a.ys;
 #pragma unroll
@@ -128,7 +142,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(LnFwdArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(LnFwdArgs a) {
     constexpr int N = RowVec<T>::N;
-    __shared__ float sm[8];
+    __shared__ float sm[16];
     const float n = (float)a.C;
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* xr = (const T*)a.x + row * a.xs;
@@ -169,10 +183,10 @@ __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(LnFwdArgs a) {
 // Backward.  Every workgroup walks over rows and keeps its columns' sums of dy xh and dy in registers; at the end its row
 // groups are joined through LDS in a fixed order and written as one partial row, which colsum_kernel adds up.
 template <typename T, int NV, int LPR>
-__global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
-    constexpr int N = RowVec<T>::N, RPB = 256 / LPR;
-    __shared__ float sm[8];
-    __shared__ float join[256 * N];
+__global__ __launch_bounds__(ln_block(LPR)) void ln_bwd_kernel(LnBwdArgs a) {
+    constexpr int N = RowVec<T>::N, BLOCK = ln_block(LPR), RPB = BLOCK / LPR;
+    __shared__ float sm[16];
+    __shared__ float join[BLOCK * N];
     const int l = threadIdx.x % LPR;
     float w[NV][N], aw[NV][N], ab[NV][N];
 #pragma unroll
@@ -184,7 +198,9 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
     const float inv = 1.0f / (float)a.C;
     const long step = (long)gridDim.x * RPB;
     long row = (long)blockIdx.x * RPB + threadIdx.x / LPR;
-    typename RowVec<T>::R nx[NV], nd[NV], na[NV];       // the next row is on its way while this one is reduced
+    // the next row is on its way while this one is reduced, where the registers allow it
+    constexpr bool AHEAD = LPR <= 256;
+    typename RowVec<T>::R nx[NV], nd[NV], na[NV];
     float nmu = 0.f, nr = 0.f;
     auto fetch = [&](long r) {
 #pragma unroll
@@ -197,8 +213,9 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
         nmu = a.mean[r];
         nr = a.rstd[r];
     };
-    if (row < a.rows) fetch(row);
+    if (AHEAD && row < a.rows) fetch(row);
     for (; row < a.rows; row += step) {
+        if (!AHEAD) fetch(row);
         float xh[NV][N], g[NV][N];
         typename RowVec<T>::R add[NV];
         const float mu = nmu, r = nr;
@@ -209,12 +226,12 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
             row_floats<T>(nd[v], g[v]);
             add[v] = na[v];
         }
-        if (row + step < a.rows) fetch(row + step);
+        if (AHEAD && row + step < a.rows) fetch(row + step);
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                if ((v * LPR + l) * N + e < a.C) xh[v][e] = (xh[v][e] - mu) * r;
+                xh[v][e] = (xh[v][e] - mu) * r;       // behind the last column dy is zero, and what it multiplies counts nothing
                 aw[v][e] += g[v][e] * xh[v][e];
                 ab[v][e] += g[v][e];
                 g[v][e] *= w[v][e];
@@ -249,7 +266,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
 #pragma unroll
             for (int e = 0; e < N; ++e) join[threadIdx.x * N + e] = k ? ab[v][e] : aw[v][e];
             __syncthreads();
-            for (int i = threadIdx.x; i < LPR * N; i += 256) {
+            for (int i = threadIdx.x; i < LPR * N; i += BLOCK) {
                 float s = 0.f;
 #pragma unroll
                 for (int j = 0; j < RPB; ++j) s += join[j * LPR * N + i];
@@ -263,7 +280,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(LnBwdArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void ln_bwd_wide_dx_kernel(LnBwdArgs a) {
     constexpr int N = RowVec<T>::N;
-    __shared__ float sm[8];
+    __shared__ float sm[16];
     const float inv = 1.0f / (float)a.C;
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* xr = (const T*)a.x + row * a.xs;
@@ -353,20 +370,24 @@ LnShape ln_shape(long C, int es) {
     if (nvec <= 32) return {32, 1};
     if (nvec <= 64) return {64, 1};
     if (nvec <= 128) return {64, 2};
-    if (nvec <= 256) return {64, 4};
+    if (nvec <= 192) return {64, 3};
+    if (nvec <= 256) return {256, 1};
     if (nvec <= 512) return {256, 2};
-    if (nvec <= 1024) return {256, 4};
-    if (nvec <= 2048) return {256, 8};
+    if (nvec <= 768) return {256, 3};
+    if (nvec <= 1024) return {512, 2};
+    if (nvec <= 2048) return {512, 4};      // eight vectors of 256 lanes do not fit the backward pass's registers
     return {0, 0};
 }
 constexpr int kLnMaxGroups = 1024;      // workgroups that walk over the rows: four per CU
 
-// workgroups of the backward pass = rows of its partial sums
+// workgroups of the backward pass = rows of its partial sums, which are written and read again: fewer for long rows
+// (8192 rows of 8192 bf16: 105.9 us with 1024, 88.0 with 256)
 long ln_bwd_groups(int es, long rows, long C) {
     const LnShape sh = ln_shape(C, es);
     if (sh.lpr == 0) return rows < 64 ? rows : 64;
-    const long rpb = 256 / sh.lpr, n = (rows + rpb - 1) / rpb;
-    return n < kLnMaxGroups ? n : kLnMaxGroups;
+    const long rpb = ln_block(sh.lpr) / sh.lpr, n = (rows + rpb - 1) / rpb;
+    const long most = sh.lpr == 512 ? kLnMaxGroups / 4 : sh.lpr == 256 ? kLnMaxGroups / 2 : kLnMaxGroups;
+    return n < most ? n : most;
 }
 
 #define LN_DISPATCH(KERNEL, T, sh, grid, s, a)                                                        \
@@ -376,10 +397,12 @@ long ln_bwd_groups(int es, long rows, long C) {
         else if (sh.lpr == 32) KERNEL<T, 1, 32><<<grid, 256, 0, s>>>(a);                              \
         else if (sh.lpr == 64 && sh.nv == 1) KERNEL<T, 1, 64><<<grid, 256, 0, s>>>(a);                \
         else if (sh.lpr == 64 && sh.nv == 2) KERNEL<T, 2, 64><<<grid, 256, 0, s>>>(a);                \
-        else if (sh.lpr == 64) KERNEL<T, 4, 64><<<grid, 256, 0, s>>>(a);                              \
-        else if (sh.nv == 2) KERNEL<T, 2, 256><<<grid, 256, 0, s>>>(a);                               \
-        else if (sh.nv == 4) KERNEL<T, 4, 256><<<grid, 256, 0, s>>>(a);                               \
-        else KERNEL<T, 8, 256><<<grid, 256, 0, s>>>(a);                                               \
+        else if (sh.lpr == 64) KERNEL<T, 3, 64><<<grid, 256, 0, s>>>(a);                              \
+        else if (sh.lpr == 256 && sh.nv == 1) KERNEL<T, 1, 256><<<grid, 256, 0, s>>>(a);              \
+        else if (sh.lpr == 256 && sh.nv == 2) KERNEL<T, 2, 256><<<grid, 256, 0, s>>>(a);              \
+        else if (sh.lpr == 256) KERNEL<T, 3, 256><<<grid, 256, 0, s>>>(a);                            \
+        else if (sh.nv == 2) KERNEL<T, 2, 512><<<grid, 512, 0, s>>>(a);                               \
+        else KERNEL<T, 4, 512><<<grid, 512, 0, s>>>(a);                                               \
     } while (0)
 
 template <typename T>
@@ -388,7 +411,7 @@ int ln_fwd(const LnFwdArgs& a, hipStream_t s) {
     if (sh.lpr == 0) {
         ln_fwd_wide_kernel<T><<<(unsigned)(a.rows < 2048 ? a.rows : 2048), 256, 0, s>>>(a);
     } else {
-        const long rpb = 256 / sh.lpr, n = (a.rows + rpb - 1) / rpb;
+        const long rpb = ln_block(sh.lpr) / sh.lpr, n = (a.rows + rpb - 1) / rpb;
         const unsigned grid = (unsigned)(n < 2 * kLnMaxGroups ? n : 2 * kLnMaxGroups);
         LN_DISPATCH(ln_fwd_kernel, T, sh, grid, s, a);
     }

@@ -29,12 +29,14 @@ template <> struct RowVec<__bf16> {
 template <typename T>
 __device__ __forceinline__ typename RowVec<T>::R row_load(const T* p, int n) {
     constexpr int N = RowVec<T>::N;
-    typename RowVec<T>::R v;
+    typename RowVec<T>::R v = {};
     if (n >= N) {
         v = *(const typename RowVec<T>::V*)p;
-    } else {
+    } else if (n > 0) {
+        asm volatile("" ::: "memory");          // a branch of its own: lanes behind the end would walk through it as well
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = e < n ? p[e] : (T)0.f;
+        for (int e = 0; e < N - 1; ++e)
+            if (e < n) v[e] = p[e];
     }
     return v;
 }
@@ -55,9 +57,10 @@ __device__ __forceinline__ void row_store(T* p, int n, const float* o, bool thro
     if (n >= N) {
         if (through) store_through(p, v);
         else *(typename RowVec<T>::V*)p = v;
-    } else {
+    } else if (n > 0) {
+        asm volatile("" ::: "memory");
 #pragma unroll
-        for (int e = 0; e < N; ++e)
+        for (int e = 0; e < N - 1; ++e)
             if (e < n) p[e] = v[e];
     }
 }
