@@ -5,6 +5,8 @@
 // LPR lanes (a part of a wave, a wave, or a workgroup), so the mean, the centred sum of squares and the output come from
 // one read.  Statistics and all sums are f32; the variance is the sum of squares around the mean that was just found
 // (E[x^2] - mu^2 would lose it for rows far from zero).
+// Measured (a large copy: 5.0 TB/s): forward 65536 x 1024 bf16 42 us = 6.4 TB/s, partly from the memory-side cache, 20011 x
+// 1031 f32 33 us = 5.0 TB/s; backward 65536 x 1024 bf16 with `add` 105 us = 5.1 TB/s and 5 us for the partial rows.
 // Rows need no alignment: 16-byte vector accesses at element alignment, which this target's global memory serves.
 #include "blocks.h"
 #include "vec.h"

@@ -29,7 +29,7 @@ __device__ __forceinline__ float lin_act(float v, int act) {
     if (act == LIN_SILU) return v * __builtin_amdgcn_rcpf(1.0f + lin_exp(-v));
     if (act == LIN_RELU) return v < 0.f ? 0.f : v;
     if (act == LIN_GELU) {
-        // v Phi(v) = max(v, 0) - |v| q on either side of zero; q is 0 long before |v| = 64, and 0 * infinity is avoided
+        // v Phi(v) = max(v, 0) - |v| q on either side of zero; q is 0 long before |v| = 64, so infinities give the limits
         float e;
         const float q = lin_tail(v, e);
         return __builtin_fmaf(-__builtin_amdgcn_fmed3f(__builtin_fabsf(v), 0.f, 64.f), q,
@@ -65,6 +65,10 @@ __device__ __forceinline__ float lin_dact(float z, int act) {
 // for the next step's data, meets the other waves, and multiplies the second half while it reads the next step's first
 // fragments and asks for the step NS later.  One barrier per step; nothing in front of a product is read later than one
 // half step before it.
+//
+// Bound by the matrix cores (256 tile, long contractions: 65536 x 4096 x 1024 bf16 in 440 us = 1.25 PFLOP/s, the rate this
+// chip's clock holds under such load; a step alone runs at 1.4), by the epilogue's stores and arithmetic for short ones
+// (16384 x 256 x 1024 with GELU and the value before it: 27 us, of them 7 products), by LDS reads for the 64 tile.
 //
 // A wave of the 256 tile has its SIMD for itself and sends an instruction every four cycles or so, 256 in the time of half
 // a step's products: what is not a product has to fit between them.  (Walking over several tiles with the requests
@@ -207,8 +211,8 @@ constexpr int gemm_stages(int F, bool dma) { return F == 2 && dma ? 4 : 2; }
 constexpr int gemm_lds(int F, bool dma) { return 2 * gemm_stages(F, dma) * F * 4096; }
 
 // DMA: both operands have 16-byte aligned rows whose length along the contiguous index is a multiple of a piece, and come
-// by direct loads into LDS.  Otherwise pieces are loaded at element alignment into registers, two steps ahead, and written
-// to LDS one step before they are read; a piece that would leave its row is taken from the row's end and moved into
+// by direct loads into LDS.  Otherwise pieces are loaded at element alignment into registers, one (64 tile: two) steps ahead,
+// and written to LDS one step before they are read; a piece that would leave its row is taken from the row's end and moved into
 // place, so the loads need no branches (which would make the compiler wait for all of them).  That takes rows of at
 // least one piece.
 template <typename T, bool AKC, bool BKC, int F, bool DMA>
@@ -218,7 +222,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
     constexpr int ES = sizeof(T), V = 16 / ES, TILE = 32 * F, BK = OA::BK, NP = OA::NP, STAGE = OA::BYTES;
     constexpr int NS = gemm_stages(F, DMA);
     typedef typename RowVec<T>::R R;
-    constexpr int SETS = !DMA && F == 2 ? 2 : 1;          // register sets (more do not fit a tile of 128)
+    constexpr int SETS = !DMA && F == 2 ? 2 : 1;          // register sets in the step loop (two do not fit a tile of 128)
     extern __shared__ __attribute__((aligned(1024))) char smem[];       // [A: NS stages][B: NS stages], then the epilogue's
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
@@ -280,8 +284,8 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
             }
         }
     };
-    u32x4 ra[SETS][DMA ? 1 : NP], rb[SETS][DMA ? 1 : NP];
-    int rk[SETS] = {};                    // kleft of the steps in the register sets
+    u32x4 ra[2][DMA ? 1 : NP], rb[2][DMA ? 1 : NP];
+    int rk[2] = {};                       // kleft of the steps in the register sets
     // asks for piece Q of both operands (register set S); behind the last step: zeros, no memory access (DMA), or the
     // first elements of the matrix, which are not used
     auto request = [&](auto Q, auto S) __attribute__((always_inline)) {
@@ -304,26 +308,21 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         bp += bstep;
         narrow();
     };
-    // this wave's pieces of register set S are written to stage `st`
-    auto write = [&](auto S, int st) __attribute__((always_inline)) {
-        char* la = smem + st * STAGE + (wave * NP * 64 + lane) * 16;
-        // pieces that were taken from the end of their row, and those behind the end of k
+    // piece Q of register set S is written to stage `st`
+    auto put = [&](auto Q, auto S, int st) __attribute__((always_inline)) {
+        constexpr int q = Q;
+        // taken from the end of its row, or behind the end of k
         if (rk[S] < BK || (!AKC && arows < TILE) || (!BKC && brows < TILE)) {
-            gemm_for<0, NP>([&](auto Q) __attribute__((always_inline)) {
-                constexpr int q = Q;
-                const int xa = OA::element(wave, q, lane), xb = OB::element(wave, q, lane);
-                const int da = xa - ((AKC ? rk[S] : arows) - V), db = xb - ((BKC ? rk[S] : brows) - V);
-                if (da > 0) ra[S][q] = gemm_drop<T>(ra[S][q], da < V ? da : V - 1);
-                if (db > 0) rb[S][q] = gemm_drop<T>(rb[S][q], db < V ? db : V - 1);
-                if ((AKC ? xa : rowa + q * OA::ROWS) >= rk[S]) ra[S][q] = u32x4{0u, 0u, 0u, 0u};
-                if ((BKC ? xb : rowb + q * OB::ROWS) >= rk[S]) rb[S][q] = u32x4{0u, 0u, 0u, 0u};
-            });
+            const int xa = OA::element(wave, q, lane), xb = OB::element(wave, q, lane);
+            const int da = xa - ((AKC ? rk[S] : arows) - V), db = xb - ((BKC ? rk[S] : brows) - V);
+            if (da > 0) ra[S][q] = gemm_drop<T>(ra[S][q], da < V ? da : V - 1);
+            if (db > 0) rb[S][q] = gemm_drop<T>(rb[S][q], db < V ? db : V - 1);
+            if ((AKC ? xa : rowa + q * OA::ROWS) >= rk[S]) ra[S][q] = u32x4{0u, 0u, 0u, 0u};
+            if ((BKC ? xb : rowb + q * OB::ROWS) >= rk[S]) rb[S][q] = u32x4{0u, 0u, 0u, 0u};
         }
-        gemm_for<0, NP>([&](auto Q) __attribute__((always_inline)) {
-            *(u32x4*)(la + Q * 1024) = ra[S][Q];
-            *(u32x4*)(la + NS * STAGE + Q * 1024) = rb[S][Q];
-        });
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        char* la = smem + st * STAGE + ((wave * NP + q) * 64 + lane) * 16;
+        *(u32x4*)la = ra[S][q];
+        *(u32x4*)(la + NS * STAGE) = rb[S][q];
     };
 
     f32x4 acc[F][F];       // [row fragment][column fragment]
@@ -349,7 +348,10 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         constexpr int h = H, r = 1 - h;
         gemm_for<0, F>([&](auto I) __attribute__((always_inline)) {
             constexpr int i = I;
-            if constexpr (h == 1 && i < NP) request(I, S);
+            if constexpr (h == 1 && i < NP) {
+                if constexpr (!DMA) put(I, S, 1 - stage);       // the step after the next, where the last one was
+                request(I, S);
+            }
             OA::template read<i, r>(fa[r][i], aa[r] + stage * STAGE);
             OB::template read<i, r>(fb[r][i], bb[r] + stage * STAGE);
             gemm_for<0, F>([&](auto J) __attribute__((always_inline)) {
@@ -516,11 +518,14 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         for (int t = 0; t < NS; ++t) ask(c0);
         gemm_all_but<(NS - 1) * 2 * NP>();
     } else {
-        // sets hold the steps 1, 2 (of two) or the step 1 when the loop starts
+        // the steps 0 and 1 go to LDS; when the loop starts the sets hold the step 2, or 2 and 3
+        ask(c0);
+        ask(c1);
+        gemm_for<0, NP>([&](auto Q) __attribute__((always_inline)) { put(Q, c0, 0); });
+        gemm_for<0, NP>([&](auto Q) __attribute__((always_inline)) { put(Q, c1, 1); });
         ask(c0);
         if constexpr (SETS == 2) ask(c1);
-        write(c0, 0);
-        ask(c0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -533,13 +538,14 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         OB::template read<I, 0>(fb[0][I], bb[0]);
     });
     landed(c0);
-    // a step; S: the register set that holds the next one
+    // a step; S: the register set that holds the one after the next
     auto step = [&](auto S) __attribute__((always_inline)) {
         multiply(c0, S);
         landed(c1);
         const int next = stage + 1 == NS ? 0 : stage + 1;
-        if constexpr (DMA) gemm_all_but<(NS - 2) * 2 * NP>();       // the later steps that were asked for
-        else write(S, next);
+        // the next step is in LDS: the later ones that were asked for may be on their way (what this wave wrote itself is there
+        // since landed())
+        if constexpr (DMA) gemm_all_but<(NS - 2) * 2 * NP>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         stage = next;
@@ -551,15 +557,15 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
         for (int t = 0; t < nt; ++t) step(c0);
     } else {
         for (int t = 0; t < nt; t += 2) {
-            step(c1);
             step(c0);
+            step(c1);
         }
     }
     // nothing is on its way into LDS any more, and the last products' results may be read
     gemm_all_but<0>();
     if constexpr (F == 8) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
     __syncthreads();
-    if (a.res && !a.part) finish(std::integral_constant<int, F == 8 ? 1 : 2>{}, std::true_type{});
+    if (a.res && !a.part) finish(std::integral_constant<int, F == 8 || !DMA ? 1 : 2>{}, std::true_type{});
     else finish(std::integral_constant<int, 2>{}, std::false_type{});
 }
 
@@ -842,9 +848,9 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long lddy, 
 // Tile and split of one product: the pair with the least estimated time.  The estimate is what the kernels measured (us):
 // a workgroup costs `fixed` (first loads, epilogue) and per step of the contraction `busy` where several share a CU and hide
 // each other's waits, `lone` where one has a CU for itself; a split adds a launch and the traffic of its f32 parts.
-//   bf16, 16384 x 1024 outputs of K = 1024:  tiles of 256: 38.3 us, 128: 40.5, 64: 69.0      (K = 256: 21.2, 21.2, 38.0)
-//   bf16,  1024 x 1024 outputs of K = 2048:  128: 23.3 us, in two parts 19.7; 64: 12.1, in two parts 17.4
-//   bf16,   256 x 1024 outputs of K = 16384: 128: 152.6 us whole, 30.9 in sixteen parts; 64: 66.1 whole, 24.4 in four
+//   bf16, 16384 x 1024 outputs of K = 1024:  tiles of 256: 36.2 us, 128: 38.7, 64: 69.7      (K = 256: 17.3, 17.8, 35.0)
+//   bf16,  1024 x 1024 outputs of K = 2048:  128: 25.7 us, in two parts 19.8; 64: 11.3, in two parts 18.2
+//   bf16,   256 x 1024 outputs of K = 16384: 128: 142.5 us whole, 25.7 in sixteen parts; 64: 55.6 whole, 22.0 in four
 // f32 steps are bound by their matrix instructions, a sixteenth of bf16's rate; operands staged through registers cost
 // about twice the direct loads' step.
 struct GemmPlan { int F, parts, kper; };

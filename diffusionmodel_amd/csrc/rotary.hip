@@ -3,6 +3,8 @@
 // Elements behind the rotated pairs pass through.  Queries and keys, which share positions, go through one launch.
 // Bound by HBM: one read and one write per element.  A thread holds the angles of one 16-byte vector's pairs in registers
 // and applies them to a group of heads of one token, so the trigonometry is paid once per group.
+// 2 x 8192 tokens, 20 heads of 128 f32: 69 us = 4.9 TB/s (a large copy: 5.0); 64 x 256 tokens, 8 heads of 64 bf16 out of a
+// fused projection: 9.4 us, of which the first loads, the angles and the launch are about half.
 // Angles: the product of a position (below 2^29) and an f32 frequency is exact in f64; it is reduced to a fraction of a
 // turn in f64 and only that fraction goes through f32 sine and cosine, so far positions lose nothing.
 #include "blocks.h"

@@ -444,7 +444,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     of an [N, K] weight) in bf16 or f32, bias N values used in f32, res [..., N] in x's type, added before the activation
     like a convolution's; act None, 'silu', 'relu' or 'gelu' (the exact one).  Products accumulate in f32.
     Returns the output in x's type, or (output, z) with save_pre: z, the value before the activation, is what
-    linear_backward needs with one.  `out` may be res itself."""
+    linear_backward needs with one.  `out` may be res itself.  Rows of a matrix may lie up to 2^21 elements apart."""
     dev, K, N = _check_linear(x, weight, act)
     M, ldx = _rows("x", x)
     order, ldw = _weight_order(weight)

@@ -202,7 +202,7 @@ const char* ldm_last_kernel(void);
 /* Layer norm, rotary positions and the linear layer, each with its backward pass: what a block of tokens needs around the
  * attention.  `dtype` is the element type of the tensors (LDM_F32 / LDM_BF16); statistics, biases, norm parameters and
  * their gradients are f32, sums are f32 whatever the type.  Strides are in elements and tensors need no alignment beyond
- * their element's.  Workspaces belong to one call at a time: calls that may overlap take different ones.  Nothing is
+ * their element's; the rows of ldm_linear's matrices may lie up to 2^21 elements apart.  Workspaces belong to one call at a time: calls that may overlap take different ones.  Nothing is
  * allocated, nothing synchronises; every call can be captured into a graph.  Sums are taken in a fixed order: the same
  * call gives the same bits. */
 /* y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis of x [rows, C] (biased variance); weight / bias [C]
