@@ -29,7 +29,7 @@ struct LnBwdArgs {
     const char *dy, *x, *add;
     char* dx;
     const float *mean, *rstd, *w;
-    float* part;       // [2][gridDim.x][C] partial sums of dw and db, or null
+    float *part_w, *part_b;       // [gridDim.x][C] partial sums of dw and db, or null
     long dys, xs, as, dxs;
     long rows;
     int C;
@@ -258,12 +258,12 @@ __global__ __launch_bounds__(ln_block(LPR)) void ln_bwd_kernel(LnBwdArgs a) {
             row_store<T>(or_ + (v * LPR + l) * N, a.C - (v * LPR + l) * N, o);
         }
     }
-    if (!a.part) return;
+    if (!a.part_w) return;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            float* dst = a.part + ((long)k * gridDim.x + blockIdx.x) * a.C;
+            float* dst = (k ? a.part_b : a.part_w) + (long)blockIdx.x * a.C;
             __syncthreads();
 #pragma unroll
             for (int e = 0; e < N; ++e) join[threadIdx.x * N + e] = k ? ab[v][e] : aw[v][e];
@@ -337,8 +337,8 @@ __global__ __launch_bounds__(256) void ln_bwd_wide_dw_kernel(LnBwdArgs a) {
 #pragma unroll
     for (int e = 0; e < N; ++e)
         if (c + e < a.C) {
-            a.part[(long)blockIdx.x * a.C + c + e] = aw[e];
-            a.part[((long)gridDim.x + blockIdx.x) * a.C + c + e] = ab[e];
+            a.part_w[(long)blockIdx.x * a.C + c + e] = aw[e];
+            a.part_b[(long)blockIdx.x * a.C + c + e] = ab[e];
         }
 }
 
@@ -386,8 +386,9 @@ constexpr int kLnMaxGroups = 1024;      // workgroups that walk over the rows: f
 // (8192 rows of 8192 bf16: 105.9 us with 1024, 88.0 with 256)
 long ln_bwd_groups(int es, long rows, long C) {
     const LnShape sh = ln_shape(C, es);
-    if (sh.lpr == 0) return rows < 64 ? rows : 64;
+    if (sh.lpr == 0) return rows <= 4 ? rows > 0 : rows < 64 ? rows : 64;
     const long rpb = ln_block(sh.lpr) / sh.lpr, n = (rows + rpb - 1) / rpb;
+    if (n <= 4) return n > 0;             // no second launch
     const long most = sh.lpr == 512 ? kLnMaxGroups / 4 : sh.lpr == 256 ? kLnMaxGroups / 2 : kLnMaxGroups;
     return n < most ? n : most;
 }
@@ -428,7 +429,7 @@ int ln_bwd(const LnBwdArgs& a, hipStream_t s) {
     if (sh.lpr == 0) {
         ln_bwd_wide_dx_kernel<T><<<(unsigned)(a.rows < 2048 ? a.rows : 2048), 256, 0, s>>>(a);
         LDM_HIP(hipGetLastError());
-        if (a.part) {
+        if (a.part_w) {
             const unsigned cb = (unsigned)((a.C + 256 * RowVec<T>::N - 1) / (256 * RowVec<T>::N));
             ln_bwd_wide_dw_kernel<T><<<dim3(G, cb), 256, 0, s>>>(a);
         }
@@ -461,11 +462,13 @@ long ln_ws_floats(int dtype, long rows, long C) {
 int launch_layer_norm_backward(int dtype, const void* dy, long dys, const void* x, long xs, const void* add, long as,
                                const float* mean, const float* rstd, const float* w, void* dx, long dxs, float* dw,
                                float* db, float* ws, long rows, int C, hipStream_t s) {
-    LnBwdArgs a{(const char*)dy, (const char*)x, (const char*)add, (char*)dx, mean, rstd, w, dw ? ws : nullptr,
-                dys, xs, as, dxs, rows, C};
+    const long G = ln_bwd_groups(dtype == LDM_BF16 ? 2 : 4, rows, C);
+    const bool direct = G == 1;           // the one partial row is the result
+    LnBwdArgs a{(const char*)dy, (const char*)x, (const char*)add, (char*)dx, mean, rstd, w, direct ? dw : dw ? ws : nullptr,
+                direct ? db : dw ? ws + G * C : nullptr, dys, xs, as, dxs, rows, C};
     if (rows > 0) LDM_TRY(dtype == LDM_BF16 ? ln_bwd<__bf16>(a, s) : ln_bwd<float>(a, s));
-    if (!dw) return LDM_OK;
-    return launch_colsum(ws, (int)ln_bwd_groups(dtype == LDM_BF16 ? 2 : 4, rows, C), C, 2, dw, db, s);
+    if (!dw || direct) return LDM_OK;
+    return launch_colsum(ws, (int)G, C, 2, dw, db, s);
 }
 
 }  // namespace ldm

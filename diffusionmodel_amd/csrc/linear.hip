@@ -953,8 +953,8 @@ int gemm_by_order(const GemmArgs& a, bool akc, bool bkc, float* ws, hipStream_t 
     return akc ? (bkc ? gemm<T, true, true>(a, ws, s) : gemm<T, true, false>(a, ws, s)) : gemm<T, false, false>(a, ws, s);
 }
 
-// threads per row of the dz kernel, workgroups along the rows (at least four rows a thread where there are that many) and
-// along the columns
+// threads per row of the dz kernel, workgroups along the rows (at least four rows a thread where there are that many; one,
+// whose sums need no second launch, up to sixteen) and along the columns
 struct DzShape { int ct; long groups, blocks; };
 DzShape dz_shape(int es, long M, long N) {
     const long nvec = (N * es + 15) / 16;
@@ -962,8 +962,9 @@ DzShape dz_shape(int es, long M, long N) {
     d.ct = 1;
     while (d.ct < 256 && d.ct < nvec) d.ct *= 2;
     d.blocks = (nvec + d.ct - 1) / d.ct;
+    if (M == 0) return {d.ct, 0, d.blocks};
     const long rows = (M + 256 / d.ct - 1) / (256 / d.ct);
-    d.groups = (rows + 3) / 4;
+    d.groups = rows <= 16 ? 1 : (rows + 3) / 4;
     const long most = d.blocks < 1024 ? 1024 / d.blocks : 1;
     if (d.groups > most) d.groups = most;
     return d;
@@ -992,12 +993,13 @@ static int dz_launch(const void* dy, long lddy, const void* pre, long ldp, void*
                      long N, int act, hipStream_t s) {
     const DzShape d = dz_shape(sizeof(T), M, N);
     LDM_REQUIRE(d.blocks <= 65535, "too many columns for one launch");
+    if (d.groups == 1 && M > 0) ws = db;
     if (M > 0 && (act != LIN_NONE || db)) {
         linear_dz_kernel<T><<<dim3((unsigned)d.groups, (unsigned)d.blocks), 256, 0, s>>>(
             (const T*)dy, lddy, (const T*)pre, ldp, (T*)dz, lddz, db ? ws : nullptr, M, N, act, d.ct);
         LDM_HIP(hipGetLastError());
     }
-    if (!db) return LDM_OK;
+    if (!db || ws == db) return LDM_OK;
     return launch_colsum(ws, (int)d.groups, (int)N, 1, db, nullptr, s);
 }
 int launch_linear_dz(int dtype, const void* dy, long lddy, const void* pre, long ldp, void* dz, long lddz, float* db, float* ws,
