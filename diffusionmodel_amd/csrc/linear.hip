@@ -854,12 +854,17 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long lddy, 
 // f32 steps are bound by their matrix instructions, a sixteenth of bf16's rate; operands staged through registers cost
 // about twice the direct loads' step.
 struct GemmPlan { int F, parts, kper; };
+struct GemmCost { int F; double fixed, busy, lone; };
+constexpr GemmCost kBf16Direct[3] = {{8, 11.0, 1.5, 1.5}, {4, 2.5, 0.45, 0.60}, {2, 1.7, 0.17, 0.25}};
+constexpr GemmCost kBf16Staged[2] = {{4, 3.4, 0.80, 1.20}, {2, 1.7, 0.34, 0.50}};
+constexpr GemmCost kF32[2] = {{4, 4.0, 1.90, 2.0}, {2, 1.8, 0.50, 0.55}};
+// `extra`: what a tile's epilogue adds
+double gemm_us(const GemmCost& c, long M, long N, long parts, long kper, double extra) {
+    const long t = 32 * c.F, per_cu = (((M + t - 1) / t) * ((N + t - 1) / t) * parts + 255) / 256;
+    return per_cu <= 1 ? c.fixed + kper * c.lone + extra : per_cu * (c.fixed + kper * c.busy + extra);
+}
 GemmPlan gemm_plan(int es, long M, long N, long K, bool dma) {
-    struct Cost { int F; double fixed, busy, lone; };
-    static const Cost bf16_dma[3] = {{8, 11.0, 1.5, 1.5}, {4, 3.4, 0.45, 0.60}, {2, 1.7, 0.17, 0.25}};
-    static const Cost bf16_reg[2] = {{4, 3.4, 0.80, 1.20}, {2, 1.7, 0.34, 0.50}};
-    static const Cost f32[2] = {{4, 4.0, 1.90, 2.0}, {2, 1.8, 0.50, 0.55}};
-    const Cost* costs = es == 4 ? f32 : dma ? bf16_dma : bf16_reg;
+    const GemmCost* costs = es == 4 ? kF32 : dma ? kBf16Direct : kBf16Staged;
     const int n = es == 2 && dma ? 3 : 2;
     const long bk = 128 / es, steps = K > 0 ? (K + bk - 1) / bk : 1;
     GemmPlan best = {2, 1, (int)steps};
@@ -868,8 +873,7 @@ GemmPlan gemm_plan(int es, long M, long N, long K, bool dma) {
         const long t = 32 * costs[i].F, tiles = ((M + t - 1) / t) * ((N + t - 1) / t);
         for (long want = 1; want <= 64 && want <= steps; ++want) {
             const long kper = (steps + want - 1) / want, parts = (steps + kper - 1) / kper;
-            const long per_cu = (tiles * parts + 255) / 256;
-            double us = per_cu <= 1 ? costs[i].fixed + kper * costs[i].lone : per_cu * (costs[i].fixed + kper * costs[i].busy);
+            double us = gemm_us(costs[i], M, N, parts, kper, 0.0);
             if (parts > 1) us += 4.0 + (double)M * N * (8.0 * parts + es) / 7e6;
             if (us < least) {
                 least = us;
@@ -879,6 +883,29 @@ GemmPlan gemm_plan(int es, long M, long N, long K, bool dma) {
         }
     }
     return best;
+}
+// The tile of a whole bf16 product with an epilogue: a workgroup of the 256 tile has its CU for itself and nothing to
+// multiply meanwhile; two of the 128 tile hide one's epilogue behind the other's products, as long as what they write stays
+// in the caches.  us per tile of (256, 128, 64), outputs written through / larger ones:
+//   GELU 8.0, 1.1, 0.15   SiLU 3.0, 0.45, 0.05   residual 7.0, 1.2, 0.3 / 10, 2.2, 0.5   z kept 2.5, 0.3, 0.05 / 5.2, 2.3, 0.5
+//   16384 x 256 x 1024: GELU and z kept 27.7 us with the 256 tile, 23.6 with 128; 65536 x 256 x 1024: 109.6, 118.3, GELU
+//   alone 92.9, 78.0; residual 105.1, 100.1
+int gemm_tile_with_epilogue(const GemmArgs& a, int steps) {
+    static constexpr double gelu[3] = {8.0, 1.1, 0.15}, silu[3] = {3.0, 0.45, 0.05};
+    static constexpr double res[2][3] = {{7.0, 1.2, 0.3}, {10.0, 2.2, 0.5}}, pre[2][3] = {{2.5, 0.3, 0.05}, {5.2, 2.3, 0.5}};
+    const int large = !a.through;
+    int F = 8;
+    double least = 1e30;
+    for (int i = 0; i < 3; ++i) {
+        const double extra = (a.act == LIN_GELU ? gelu[i] : a.act == LIN_SILU ? silu[i] : 0.0) + (a.res ? res[large][i] : 0.0) +
+                             (a.pre ? pre[large][i] : 0.0);
+        const double us = gemm_us(kBf16Direct[i], a.M, a.N, 1, steps, extra);
+        if (us < least) {
+            least = us;
+            F = kBf16Direct[i].F;
+        }
+    }
+    return F;
 }
 long gemm_part_floats(const GemmPlan& p, long M, long N) { return p.parts > 1 ? p.parts * M * ((N + 7) & ~7L) : 0; }
 
@@ -922,16 +949,17 @@ int gemm(GemmArgs a, float* ws, hipStream_t s) {
             LDM_HIP(hipGetLastError());
             return LDM_OK;
         }
-    const GemmPlan p = gemm_plan(sizeof(T), a.M, a.N, a.K, dma);
+    // bf16: a lane's eight columns are one access, and a row's lanes cover whole lines
+    a.through = sizeof(T) == 2 && a.M * a.N * (a.pre ? 4 : 2) <= kThroughBytes && a.N % 64 == 0 && a.ldc % 64 == 0 &&
+                (size_t)a.C % 128 == 0 && (!a.pre || (a.ldp % 64 == 0 && (size_t)a.pre % 128 == 0));
+    GemmPlan p = gemm_plan(sizeof(T), a.M, a.N, a.K, dma);
+    if (sizeof(T) == 2 && dma && p.parts == 1 && (a.act != LIN_NONE || a.res || a.pre)) p.F = gemm_tile_with_epilogue(a, p.kper);
     LDM_REQUIRE(p.parts == 1 || ws, "this product needs a workspace");
     // rows too short for a piece, or an empty contraction, which has no row at all to read
     const bool any = a.K == 0 || alen < V || blen < V;
     const long t = any ? GT : 32 * p.F, tiles = ((a.M + t - 1) / t) * ((a.N + t - 1) / t) * p.parts;
     LDM_REQUIRE(tiles < (1L << 31), "more output tiles than one launch holds");
     a.kper = p.kper;
-    // bf16: a lane's eight columns are one access, and a row's lanes cover whole lines
-    a.through = sizeof(T) == 2 && a.M * a.N * (a.pre ? 4 : 2) <= kThroughBytes && a.N % 64 == 0 && a.ldc % 64 == 0 &&
-                (size_t)a.C % 128 == 0 && (!a.pre || (a.ldp % 64 == 0 && (size_t)a.pre % 128 == 0));
     a.part = p.parts > 1 ? ws : nullptr;
     if (any) {
         gemm_any_kernel<T, AKC, BKC><<<(unsigned)tiles, 256, 0, s>>>(a);
