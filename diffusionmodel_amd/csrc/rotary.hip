@@ -37,8 +37,10 @@ __device__ __forceinline__ void turn_sincos(double turns, float& sn, float& cs) 
     cs = ((k + 1) & 2) ? -b : b;
 }
 
+constexpr int kRopeMost = 320;        // threads of a workgroup whose head takes one chunk more than 256
+
 template <typename T, bool INTER>
-__global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
+__global__ __launch_bounds__(kRopeMost) void rope_kernel(RopeArgs a) {
     constexpr int N = RowVec<T>::N;
     const int local = threadIdx.x / a.nchunk, chunk = threadIdx.x - local * a.nchunk;
     // the head groups of the same tokens follow each other, so that a token's heads are read at about the same time
@@ -154,13 +156,16 @@ int launch_rope(int dtype, int interleaved, RopeArgs a, hipStream_t s) {
     if (a.tokens == 0) return LDM_OK;
     a.nrot = interleaved ? ((2 * a.P + N - 1) / N + 1) / 2 : (a.P + N - 1) / N;      // two vectors a thread
     a.nchunk = a.nrot + (a.D - 2 * a.P + 2 * N - 1) / (2 * N);
-    a.tpb = 256 / a.nchunk;
+    // a head of 2048 f32 elements whose rotated pairs end inside a vector has 257 chunks
+    const int threads = a.nchunk > 256 ? kRopeMost : 256;
+    LDM_REQUIRE(a.nchunk <= threads, "a head is longer than a workgroup");
+    a.tpb = threads / a.nchunk;
     // a group of heads per workgroup, all of them where the tokens alone give eight workgroups per CU: the angles are taken
     // once for a group.  2 x 8192 tokens, 20 heads of 128 in f32: 76.8 us in two groups of ten, 80.4 in one, 78.1 in four
     // (and 100.6 with a workgroup per head); one token, 8 heads of 64: 5.2 us in four groups, 7.4 in one
     const int heads = a.H[0] + a.H[1], es = dtype == LDM_BF16 ? 2 : 4;
     const long blocks = (a.tokens + a.tpb - 1) / a.tpb;
-        long groups = 2048 / blocks;
+    long groups = 2048 / blocks;
     groups = groups < 1 ? 1 : groups > (heads + 1) / 2 ? (heads + 1) / 2 : groups;
     a.hpg = (int)((heads + groups - 1) / groups);
     a.groups = (unsigned)((heads + a.hpg - 1) / a.hpg);
@@ -168,14 +173,14 @@ int launch_rope(int dtype, int interleaved, RopeArgs a, hipStream_t s) {
     a.through = a.tokens * heads * a.D * es <= kThroughBytes && (interleaved ? 2 : 1) * a.P * es % 64 == 0 && a.D * es % 64 == 0;
     for (int w = 0; w < 2 && a.H[w]; ++w)
         a.through = a.through && ((size_t)a.out[w] | (size_t)(a.osb[w] * es) | (size_t)(a.osn[w] * es) | (size_t)(a.osh[w] * es)) % 64 == 0;
-    LDM_REQUIRE(blocks * a.groups < (1L << 31), "too many tokens and heads for one launch");
+    LDM_REQUIRE(blocks * a.groups * threads < (1L << 32), "too many tokens and heads for one launch");
     const unsigned grid = (unsigned)(blocks * a.groups);
     if (dtype == LDM_BF16) {
-        if (interleaved) rope_kernel<__bf16, true><<<grid, 256, 0, s>>>(a);
-        else rope_kernel<__bf16, false><<<grid, 256, 0, s>>>(a);
+        if (interleaved) rope_kernel<__bf16, true><<<grid, threads, 0, s>>>(a);
+        else rope_kernel<__bf16, false><<<grid, threads, 0, s>>>(a);
     } else {
-        if (interleaved) rope_kernel<float, true><<<grid, 256, 0, s>>>(a);
-        else rope_kernel<float, false><<<grid, 256, 0, s>>>(a);
+        if (interleaved) rope_kernel<float, true><<<grid, threads, 0, s>>>(a);
+        else rope_kernel<float, false><<<grid, threads, 0, s>>>(a);
     }
     LDM_HIP(hipGetLastError());
     return LDM_OK;

@@ -655,3 +655,18 @@ def test_refusals(ops):
     with torch.no_grad():
         ops.layer_norm(x.clone().requires_grad_())                            # nothing is recorded, nothing is lost
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("P", [1, 5, 509, 1021])
+def test_rope_longest_heads(ops, P, dtype, layout):
+    dt, N, H, D = DT[dtype], 3, 2, 2048
+    print("rope", layout, dtype, P, flush=True)
+    q = _rn(P, 1, N, H, D).to(dt)
+    inv = ops.rope_frequencies((P,), device="cuda")
+    pos = torch.tensor([[7, 0, 1000]], device="cuda")
+    got = ops.rope(q, None, pos, inv, layout=layout)
+    ref, size = _rope_ref(q, pos[None], inv, (P,), layout, 1.0)
+    _rope_within(got, ref, size, dt, "q")
+    assert torch.equal(got[..., 2 * P:], q[..., 2 * P:])
