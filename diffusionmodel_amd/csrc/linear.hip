@@ -923,6 +923,8 @@ int gemm_launch(const GemmArgs& a, unsigned grid, hipStream_t s) {
 // 20.0 / 13.8; f32 2048 x 256: 13.0 / 21.5, 4096 x 4096: 24.3 / 27.4
 bool gemm_is_few(int es, long M, long N, long K) { return M <= 64 && (es == 4 || K * N <= (1L << 23)); }
 
+constexpr long kMostTiles = 1L << 24;      // a launch holds less than 2^32 threads
+
 template <typename T, bool AKC, bool BKC>
 int gemm(GemmArgs a, float* ws, hipStream_t s) {
     if (a.M == 0 || a.N == 0) return LDM_OK;
@@ -944,7 +946,7 @@ int gemm(GemmArgs a, float* ws, hipStream_t s) {
             constexpr int lds = 4 * 2 * 4 * 4096;
             LDM_TRY(allow_dynamic_lds((const void*)&gemm_few_kernel<T, BKC>, lds, done));
             const long grid = (a.M + 31) / 32 * ((a.N + 31) / 32);
-            LDM_REQUIRE(grid < (1L << 31), "more output tiles than one launch holds");
+            LDM_REQUIRE(grid < kMostTiles, "more output tiles than one launch holds");
             gemm_few_kernel<T, BKC><<<(unsigned)grid, 256, lds, s>>>(a);
             LDM_HIP(hipGetLastError());
             return LDM_OK;
@@ -958,7 +960,8 @@ int gemm(GemmArgs a, float* ws, hipStream_t s) {
     // rows too short for a piece, or an empty contraction, which has no row at all to read
     const bool any = a.K == 0 || alen < V || blen < V;
     const long t = any ? GT : 32 * p.F, tiles = ((a.M + t - 1) / t) * ((a.N + t - 1) / t) * p.parts;
-    LDM_REQUIRE(tiles < (1L << 31), "more output tiles than one launch holds");
+    LDM_REQUIRE(tiles < kMostTiles, "more output tiles than one launch holds");
+    LDM_REQUIRE(a.K / p.parts < (1L << 30), "a contraction longer than 2^30");
     a.kper = p.kper;
     a.part = p.parts > 1 ? ws : nullptr;
     if (any) {

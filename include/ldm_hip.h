@@ -202,9 +202,10 @@ const char* ldm_last_kernel(void);
 /* Layer norm, rotary positions and the linear layer, each with its backward pass: what a block of tokens needs around the
  * attention.  `dtype` is the element type of the tensors (LDM_F32 / LDM_BF16); statistics, biases, norm parameters and
  * their gradients are f32, sums are f32 whatever the type.  Strides are in elements and tensors need no alignment beyond
- * their element's; the rows of ldm_linear's matrices may lie up to 2^21 elements apart.  Workspaces belong to one call at a time: calls that may overlap take different ones.  Nothing is
- * allocated, nothing synchronises; every call can be captured into a graph.  Sums are taken in a fixed order: the same
- * call gives the same bits. */
+ * their element's; the rows of ldm_linear's matrices may lie up to 2^21 elements apart.  An output overlaps no input
+ * unless its function says so.  Workspaces belong to one call at a time: calls that may overlap take different ones.
+ * Nothing is allocated, nothing synchronises; every call can be captured into a graph.  Sums are taken in a fixed order:
+ * the same call gives the same bits. */
 /* y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis of x [rows, C] (biased variance); weight / bias [C]
  * or NULL.  mean_dev / rstd_dev [rows] f32, optional: what the backward pass needs.  y may be x (same stride). */
 int ldm_layer_norm(int dtype, const void* x_dev, long x_stride, const float* weight_dev, const float* bias_dev, float eps,

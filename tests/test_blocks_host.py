@@ -138,3 +138,13 @@ def test_host_tensors_are_refused():
               lambda: ops.rope(torch.zeros(1, 2, 1, 8), None, torch.zeros(1, 2, dtype=torch.int32), torch.ones(4))):
         with pytest.raises(ValueError):
             f()
+
+
+def test_launches_beyond_the_grid_are_refused(lib):
+    import struct
+    assert lib.ldm_linear(BF, P, 1, P, 1, 0, None, None, 0, 0, P, 1, None, 1, 1 << 36, 1, 1, P, None) == 1
+    assert lib.ldm_linear(F32, P, 16, P, 1 << 29, 0, None, None, 0, 0, P, 1 << 29, None, 1, 4, 16, 1 << 29, P, None) == 1
+    assert lib.ldm_linear_backward(F32, P, 1, P, 1, P, 1, 0, None, 0, 0, None, 0, None, 0, P, 1, None, P, 1 << 39, 1, 1,
+                                   None) == 1
+    assert lib.ldm_rope(F32, P, None, P, None, struct.pack("12l", *([2048] * 12)), 32768, 65535, 1, 0, 2048, P, 0,
+                        struct.pack("3l", 0, 4, 1), P, struct.pack("i", 1024), 1, 0, 0, None) == 1

@@ -670,3 +670,43 @@ def test_rope_longest_heads(ops, P, dtype, layout):
     ref, size = _rope_ref(q, pos[None], inv, (P,), layout, 1.0)
     _rope_within(got, ref, size, dt, "q")
     assert torch.equal(got[..., 2 * P:], q[..., 2 * P:])
+
+
+def test_rope_past_32_bit_offsets(ops):
+    N, H, D = 2 ** 31 // 1024 + 5, 16, 64
+    q = torch.zeros(1, N, H, D, dtype=torch.bfloat16, device="cuda")
+    tail = _rn(2, 1, 7, H, D).to(torch.bfloat16)
+    q[:, -7:] = tail
+    inv = ops.rope_frequencies((32,), device="cuda")
+    pos = torch.arange(N, device="cuda", dtype=torch.int32)[None]
+    want = ops.rope(tail, None, pos[:, -7:], inv)
+    got = ops.rope(q, None, pos, inv)
+    assert torch.equal(got[:, -7:], want) and not bool(got[:, :-7].any())
+    ops.rope(q, None, pos, inv, out=q)
+    assert torch.equal(q, got)
+
+
+@pytest.mark.parametrize("K", [1024, 1021])
+def test_linear_past_32_bit_offsets(ops, K):
+    """Rows, outputs and a contraction whose offsets pass 32 bits: all but the last rows are zero."""
+    M, N = 2 ** 31 // K + 300, 1024
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    tail = _rn(3, 9, K).to(torch.bfloat16)
+    x[-9:] = tail
+    w = _rn(4, K, N).to(torch.bfloat16)
+    print("linear", M, K, N, flush=True)
+
+    def within(got, a, b, what):
+        a, b = a.double().cpu(), b.double().cpu()
+        ref, size = a @ b, a.abs() @ b.abs()
+        _within(got.cpu(), ref, HALF[got.dtype] * ref.abs() + a.shape[-1] * E32 * size, what)
+    y = ops.linear(x, w, res=x if K == N else None)
+    within(y[-9:], torch.cat([tail, tail], 1) if K == N else tail,
+           torch.cat([w, torch.eye(K, dtype=w.dtype, device="cuda")]) if K == N else w, "y")
+    assert not bool(y[:-9].any())
+    gx, gw, gb, _ = ops.linear_backward(y, x, w)
+    t = y[-9:].clone()
+    within(gx[-9:], t, w.t(), "dx")
+    assert not bool(gx[:-9].any())
+    within(gw, tail.t(), t, "dw")
+    within(gb[None], torch.ones(1, 9, dtype=t.dtype), t, "db")
