@@ -4,8 +4,6 @@
 
 namespace ldm {
 
-// out[k][c] = sum over the G rows g of part[k][g][c], k < nsums <= 2, in a fixed order
-int launch_colsum(const float* part, int G, int C, int nsums, float* out0, float* out1, hipStream_t s);
 int launch_layer_norm(int dtype, const void* x, long xs, const float* w, const float* b, float eps, void* y, long ys,
                       float* mean, float* rstd, long rows, int C, hipStream_t s);
 long ln_ws_floats(int dtype, long rows, long C);
@@ -51,11 +49,22 @@ struct GemmArgs {
     int kper;                      // set by launch_gemm: steps of the contraction per part
     bool through;                  // set by launch_gemm: outputs are written through the L2
 };
+// the join of a split contraction that the caller launches later; blocks = 0: none
+struct GemmJoin {
+    GemmArgs a;
+    int parts;
+    unsigned blocks;
+};
 long gemm_ws_floats(int dtype, long M, long N, long K);
-int launch_gemm(int dtype, const GemmArgs& a, bool akc, bool bkc, float* ws, hipStream_t s);
-// dz = dy act'(pre) (not written without an activation: dz is dy) and db = column sums of dz (db null: not taken)
+// later null: the product is complete; otherwise a join may be left there, and ws holds its parts until then
+int launch_gemm(int dtype, const GemmArgs& a, bool akc, bool bkc, float* ws, GemmJoin* later, hipStream_t s);
+// dz = dy act'(pre) (not written without an activation: dz is dy) and, in ws [*groups][N], what adds up to db = column sums
+// of dz; *groups = -1: db is complete, or null and not taken
 long linear_dz_ws_floats(int dtype, long M, long N);
 int launch_linear_dz(int dtype, const void* dy, long lddy, const void* pre, long ldp, void* dz, long lddz, float* db, float* ws,
-                     long M, long N, int act, hipStream_t s);
+                     long M, long N, int act, int* groups, hipStream_t s);
+// what the products and the dz kernel left, in one launch
+int launch_linear_finish(int dtype, const GemmJoin& x, const GemmJoin& w, const float* part, int groups, long N, float* db,
+                         hipStream_t s);
 
 }  // namespace ldm

@@ -442,12 +442,6 @@ int ln_bwd(const LnBwdArgs& a, hipStream_t s) {
 
 }  // namespace
 
-int launch_colsum(const float* part, int G, int C, int nsums, float* out0, float* out1, hipStream_t s) {
-    colsum_kernel<<<dim3((unsigned)((C + 31) / 32), (unsigned)nsums), 1024, 0, s>>>(part, G, C, out0, out1);
-    LDM_HIP(hipGetLastError());
-    return LDM_OK;
-}
-
 int launch_layer_norm(int dtype, const void* x, long xs, const float* w, const float* b, float eps, void* y, long ys,
                       float* mean, float* rstd, long rows, int C, hipStream_t s) {
     if (rows == 0) return LDM_OK;
@@ -468,7 +462,9 @@ int launch_layer_norm_backward(int dtype, const void* dy, long dys, const void* 
                 direct ? db : dw ? ws + G * C : nullptr, dys, xs, as, dxs, rows, C};
     if (rows > 0) LDM_TRY(dtype == LDM_BF16 ? ln_bwd<__bf16>(a, s) : ln_bwd<float>(a, s));
     if (!dw || direct) return LDM_OK;
-    return launch_colsum(ws, (int)G, C, 2, dw, db, s);
+    colsum_kernel<<<dim3((unsigned)((C + 31) / 32), 2), 1024, 0, s>>>(ws, (int)G, C, dw, db);
+    LDM_HIP(hipGetLastError());
+    return LDM_OK;
 }
 
 }  // namespace ldm

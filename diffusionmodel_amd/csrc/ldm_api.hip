@@ -1538,16 +1538,14 @@ int ldm_linear(int dtype, const void* x, long ldx, const void* w, long ldw, int 
     a.bias = bias; a.res = res; a.ldr = ldres;
     a.pre = pre; a.ldp = ldpre; a.C = out; a.ldc = ldo;
     a.M = M; a.N = N; a.K = K; a.act = act;
-    return launch_gemm(dtype, a, true, w_order == 1, ws, (hipStream_t)stream);
+    return launch_gemm(dtype, a, true, w_order == 1, ws, nullptr, (hipStream_t)stream);
 }
+// the backward pass's workspace: the parts of dz's column sums, then those of dx and of dw
+static long linear_ws_sums(int dtype, long M, long N) { return (linear_dz_ws_floats(dtype, M, N) + 7) & ~7L; }
 long ldm_linear_backward_ws_floats(int dtype, long M, long K, long N, int w_order) {
     if (check_linear(dtype, M, K, N, w_order, 0) != LDM_OK) return -1;
-    // one after the other: the column sums of dz, dx, dw
-    long n = linear_dz_ws_floats(dtype, M, N);
-    const long nx = gemm_ws_floats(dtype, M, K, N);
-    const long nw = w_order == 0 ? gemm_ws_floats(dtype, K, N, M) : gemm_ws_floats(dtype, N, K, M);
-    n = nx > n ? nx : n;
-    return nw > n ? nw : n;
+    return linear_ws_sums(dtype, M, N) + gemm_ws_floats(dtype, M, K, N) +
+           (w_order == 0 ? gemm_ws_floats(dtype, K, N, M) : gemm_ws_floats(dtype, N, K, M));
 }
 int ldm_linear_backward(int dtype, const void* dy, long lddy, const void* x, long ldx, const void* w, long ldw, int w_order,
                         const void* pre, long ldpre, int act, void* dz, long lddz, void* dx, long lddx, void* dw, long lddw,
@@ -1561,22 +1559,26 @@ int ldm_linear_backward(int dtype, const void* dy, long lddy, const void* x, lon
     LDM_REQUIRE(!dw || (w_order == 0 ? (K == 1 || lddw >= N) : (N == 1 || lddw >= K)), "rows of dw overlap");
     LDM_REQUIRE(!db || ws || M == 0, "dbias needs a workspace");
     hipStream_t st = (hipStream_t)stream;
-    LDM_TRY(launch_linear_dz(dtype, dy, lddy, pre, ldpre, dz, lddz, db, ws, M, N, act, st));
+    int groups;
+    GemmJoin jx = {}, jw = {};
+    LDM_TRY(launch_linear_dz(dtype, dy, lddy, pre, ldpre, dz, lddz, db, ws, M, N, act, &groups, st));
     if (act == LIN_NONE) { dz = (void*)dy; lddz = lddy; }
+    float* wsx = ws ? ws + linear_ws_sums(dtype, M, N) : nullptr;
+    float* wsw = ws ? wsx + gemm_ws_floats(dtype, M, K, N) : nullptr;
     if (dx) {
         GemmArgs a = {};
         a.A = dz; a.lda = lddz; a.B = w; a.ldb = ldw; a.C = dx; a.ldc = lddx;
         a.M = M; a.N = K; a.K = N;
-        LDM_TRY(launch_gemm(dtype, a, true, w_order == 0, ws, st));
+        LDM_TRY(launch_gemm(dtype, a, true, w_order == 0, wsx, &jx, st));
     }
     if (dw) {
         GemmArgs a = {};
         a.C = dw; a.ldc = lddw; a.K = M;
         if (w_order == 0) { a.A = x; a.lda = ldx; a.M = K; a.B = dz; a.ldb = lddz; a.N = N; }
         else { a.A = dz; a.lda = lddz; a.M = N; a.B = x; a.ldb = ldx; a.N = K; }
-        LDM_TRY(launch_gemm(dtype, a, false, false, ws, st));
+        LDM_TRY(launch_gemm(dtype, a, false, false, wsw, &jw, st));
     }
-    return LDM_OK;
+    return launch_linear_finish(dtype, jx, jw, ws, groups, N, db, st);
 }
 
 int ldm_resblock_forward(ldm_module* m, const float* x, const float* t_emb, float* out, int B, int H, int W, void* stream) {

@@ -710,3 +710,30 @@ def test_linear_past_32_bit_offsets(ops, K):
     assert not bool(gx[:-9].any())
     within(gw, tail.t(), t, "dw")
     within(gb[None], torch.ones(1, 9, dtype=t.dtype), t, "db")
+
+
+@pytest.mark.parametrize("dtype,M,K,N", [("fp32", 1000, 321, 643), ("bf16", 700, 1536, 600), ("fp32", 12, 40, 24)])
+def test_linear_backward_gradients_do_not_depend_on_each_other(ops, dtype, M, K, N):
+    """Each subset of the gradients, eager and captured, gives the bits that all of them together give."""
+    dt = DT[dtype]
+    x, w, dy = _rn(1, M, K).to(dt), (_rn(2, K, N) / K ** 0.5).to(dt), _rn(3, M, N).to(dt)
+    pre = ops.linear(x, w, act="silu", save_pre=True)[1]
+    want = ops.linear_backward(dy, x, w, pre, "silu")
+    graphs = []
+    for mask in range(8):
+        on = dict(dx=bool(mask & 1), dweight=bool(mask & 2), dbias=bool(mask & 4))
+        got = ops.linear_backward(dy, x, w, pre, "silu", **on)
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            captured = ops.linear_backward(dy, x, w, pre, "silu", **on)
+        graphs.append((mask, g, captured, got))
+    for _ in range(2):
+        for mask, g, captured, got in graphs:
+            g.replay()
+            torch.cuda.synchronize()
+            for i, ref in enumerate(want):
+                if i < 3 and not mask >> i & 1:
+                    assert got[i] is None and captured[i] is None
+                else:
+                    assert torch.equal(got[i], ref) and torch.equal(captured[i], ref), (mask, i)
