@@ -68,7 +68,8 @@ __device__ __forceinline__ float lin_dact(float z, int act) {
 //
 // Bound by the matrix cores (256 tile, long contractions: 65536 x 4096 x 1024 bf16 in 440 us = 1.25 PFLOP/s, the rate this
 // chip's clock holds under such load; a step alone runs at 1.4), by the epilogue's stores and arithmetic for short ones
-// (16384 x 256 x 1024 with GELU and the value before it: 27 us, of them 7 products), by LDS reads for the 64 tile.
+// (16384 x 256 x 1024 with GELU and the value before it: 24 us with 128 tiles, 28 with 256, of which the
+// products are 7), by LDS reads for the 64 tile.
 //
 // A wave of the 256 tile has its SIMD for itself and sends an instruction every four cycles or so, 256 in the time of half
 // a step's products: what is not a product has to fit between them.  (Walking over several tiles with the requests
