@@ -230,16 +230,25 @@ __global__ __launch_bounds__(ln_block(LPR)) void ln_bwd_kernel(LnBwdArgs a) {
         }
         if (AHEAD && row + step < a.rows) fetch(row + step);
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+        for (int v = 0; v < NV; ++v) {
+            const int left = a.C - (v * LPR + l) * N;
+#pragma unroll
+            for (int e = 0; e < N; ++e) xh[v][e] = (xh[v][e] - mu) * r;
+            // behind the last column dy is zero; so that zero times it is, xh must not be an overflow of -mu r
+            if (left < N) {
+                asm volatile("" ::: "memory");
+#pragma unroll
+                for (int e = 0; e < N; ++e) xh[v][e] = e < left ? xh[v][e] : 0.f;
+            }
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                xh[v][e] = (xh[v][e] - mu) * r;       // behind the last column dy is zero, and what it multiplies counts nothing
                 aw[v][e] += g[v][e] * xh[v][e];
                 ab[v][e] += g[v][e];
                 g[v][e] *= w[v][e];
                 s1 += g[v][e];
                 s2 += g[v][e] * xh[v][e];
             }
+        }
         ln_sum2<LPR>(s1, s2, sm);
         s1 *= inv;
         s2 *= inv;

@@ -737,3 +737,20 @@ def test_linear_backward_gradients_do_not_depend_on_each_other(ops, dtype, M, K,
                     assert got[i] is None and captured[i] is None
                 else:
                     assert torch.equal(got[i], ref) and torch.equal(captured[i], ref), (mask, i)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("C", [7, 9, 30])
+def test_layer_norm_backward_of_large_constant_rows(ops, C, dtype):
+    """xh is zero, and mean rstd, which no gradient contains, is past the largest f32: dx = rstd (dy - mean(dy))."""
+    dt = DT[dtype]
+    x = torch.full((3, C), 2.0 ** 121, device="cuda").to(dt)
+    dy = _rn(C, 3, C).to(dt)
+    y, mean, rstd = ops.layer_norm(x, stats=True)
+    assert bool((y == 0).all()) and bool((mean == 2.0 ** 121).all())
+    dx, dw, db = ops.layer_norm_backward(dy, x, mean, rstd, None, param_grads=True)
+    d = dy.double()
+    ref = rstd.double()[:, None] * (d - d.mean(-1, keepdim=True))
+    size = rstd.double()[:, None] * (d.abs() + d.abs().mean(-1, keepdim=True))
+    _within(dx, ref, HALF[dt] * ref.abs() + _adds(C) * E32 * size, "dx")
+    assert bool((dw == 0).all())
