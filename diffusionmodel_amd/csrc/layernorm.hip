@@ -3,10 +3,11 @@
 //   dx = r (g - mean(g) - xh mean(g xh)) + add,   xh = (x - mu) r, g = dy w;   dw = sum_rows dy xh, db = sum_rows dy
 // Both passes are bound by HBM: one read of each input and one write of the output.  A row lives in the registers of its
 // LPR lanes (a part of a wave, a wave, or a workgroup), so the mean, the centred sum of squares and the output come from
-// one read.  Statistics and all sums are f32; the variance is the sum of squares around the mean that was just found
-// (E[x^2] - mu^2 would lose it for rows far from zero).
-// Measured (a large copy: 5.0 TB/s): forward 65536 x 1024 bf16 42 us = 6.4 TB/s, partly from the memory-side cache, 20011 x
-// 1031 f32 33 us = 5.0 TB/s; backward 65536 x 1024 bf16 with `add` 105 us = 5.1 TB/s and 5 us for the partial rows.
+// one read.  Statistics and sums are f32 (the mean of rows that are read again: f64); the mean is corrected by the mean of
+// what is left around it, and the variance is the sum of squares around it (E[x^2] - mu^2 would lose it for rows far from
+// zero).
+// Measured (a large copy: 5.0 TB/s): forward 65536 x 1024 bf16 44 us = 6.1 TB/s, partly from the memory-side cache, 20011 x
+// 1031 f32 32 us = 5.2 TB/s; backward 65536 x 1024 bf16 with `add` 105 us = 5.1 TB/s and 5 us for the partial rows.
 // Rows need no alignment: 16-byte vector accesses at element alignment, which this target's global memory serves.
 #include "blocks.h"
 #include "vec.h"
@@ -75,8 +76,20 @@ __device__ __forceinline__ float ln_sum(float a, float* sm) {
     return a;
 }
 
+// sum over a workgroup of 256, the same bits in every lane
+__device__ __forceinline__ double ln_sum64(double a, double* sm) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) a += __shfl_xor(a, d);
+    __syncthreads();                     // the previous sum has been read
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = a;
+    __syncthreads();
+    return (sm[0] + sm[1]) + (sm[2] + sm[3]);
+}
+
+// (the two vectors of a wave's bf16 row take two registers more than six waves on a SIMD have: 65536 x 1024 45.3 us with five
+// waves, 44.1 with six)
 template <typename T, int NV, int LPR>
-__global__ __launch_bounds__(ln_block(LPR)) void ln_fwd_kernel(LnFwdArgs a) {
+__global__ __launch_bounds__(ln_block(LPR), sizeof(T) == 2 && NV == 2 && LPR == 64 ? 6 : 1) void ln_fwd_kernel(LnFwdArgs a) {
     constexpr int N = RowVec<T>::N, RPB = ln_block(LPR) / LPR;
     __shared__ float sm[16];
     const int l = threadIdx.x % LPR;
@@ -86,7 +99,7 @@ __global__ __launch_bounds__(ln_block(LPR)) void ln_fwd_kernel(LnFwdArgs a) {
         ln_param<N>(a.w, (v * LPR + l) * N, a.C, 1.f, w[v]);
         ln_param<N>(a.b, (v * LPR + l) * N, a.C, 0.f, b[v]);
     }
-    const float n = (float)a.C;      // divided by, not multiplied with 1 / C: the mean of a constant row is exact
+    const float n = (float)a.C, inv = 1.0f / n;
     const long step = (long)gridDim.x * RPB;
     long row = (long)blockIdx.x * RPB + threadIdx.x / LPR;
     typename RowVec<T>::R next[NV];  // the next row is on its way while this one is reduced
@@ -106,30 +119,60 @@ __global__ __launch_bounds__(ln_block(LPR)) void ln_fwd_kernel(LnFwdArgs a) {
             for (int e = 0; e < N; ++e) s += x[v][e];
         }
         if (row + step < a.rows) fetch(row + step);
-        const float mu = ln_sum<LPR>(s, sm) / n;
-        float q = 0.f;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            // (a condition per vector, not per element: those would be kept over the rows in more registers than there are)
-            const int left = a.C - (v * LPR + l) * N;
-#pragma unroll
-            for (int e = 0; e < N; ++e) x[v][e] -= mu;
-            if (left >= N) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) q += x[v][e] * x[v][e];
-            } else if (left > 0) {
-                asm volatile("" ::: "memory");
-#pragma unroll
-                for (int e = 0; e < N - 1; ++e) q += e < left ? x[v][e] * x[v][e] : 0.f;
-            }
+        // The first mean m0 is off by the rounding of its sum, which rows far from zero would see as a shift and as variance.
+        // What is left around it is small, so its mean m1 corrects m0 to the last bit: the variance is the mean square
+        // around m0 less m1^2, in one reduction.
+        float m0 = ln_sum<LPR>(s, sm);
+        {
+#pragma clang fp contract(off)
+            m0 *= inv;                   // rounded before it is used: m1 belongs to this value
         }
-        const float r = 1.0f / sqrtf(ln_sum<LPR>(q, sm) / n + a.eps);
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[v][e] -= m0;
+        // sums of x - c and its square (a condition per vector, not per element: those would be kept over the rows in more
+        // registers than there are)
+        auto around = [&](float c, float& s, float& q) {
+            s = q = 0.f;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int left = a.C - (v * LPR + l) * N;
+                auto add = [&](int e) {
+                    const float d = x[v][e] - c;
+                    s += d;
+                    q += d * d;
+                };
+                if (left >= N) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) add(e);
+                } else if (left > 0) {
+                    asm volatile("" ::: "memory");
+#pragma unroll
+                    for (int e = 0; e < N - 1; ++e)
+                        if (e < left) add(e);
+                }
+            }
+            ln_sum2<LPR>(s, q, sm);
+        };
+        float q;
+        around(0.f, s, q);
+        const float m1 = s / n;                            // (divided by: the mean of a constant row is exact)
+        float var = q * inv - m1 * m1;
+        // (rows of nearly one value, where that difference would cancel, and squares past the largest f32: once more)
+        const bool again = m1 != 0.f && !(m1 * m1 < 0.0625f * inv * q);
+        if (__any(again)) {
+            around(m1, s, q);
+            if (again) var = q * inv;
+        }
+        const float mu = m1 == m1 ? m0 + m1 : m0;          // (a row with an infinity has an infinite mean)
+        const float r = 1.0f / sqrtf(var + a.eps);
         T* yr = (T*)a.y + row * a.ys;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             float o[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) o[e] = x[v][e] * r * w[v][e] + b[v][e];
+            for (int e = 0; e < N; ++e) o[e] = (x[v][e] - m1) * r * w[v][e] + b[v][e];
             row_store<T>(yr + (v * LPR + l) * N, a.C - (v * LPR + l) * N, o);
         }
         if (l == 0) {
@@ -145,24 +188,26 @@ template <typename T>
 __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(LnFwdArgs a) {
     constexpr int N = RowVec<T>::N;
     __shared__ float sm[16];
+    __shared__ double sm64[4];
     const float n = (float)a.C;
     for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* xr = (const T*)a.x + row * a.xs;
-        float s = 0.f;
+        double s = 0.0;          // (in f64 and not corrected afterwards, which would read the row once more)
         for (int c = threadIdx.x * N; c < a.C; c += 256 * N) {
             float x[N];
             row_floats<T>(row_load<T>(xr + c, a.C - c), x);
 #pragma unroll
             for (int e = 0; e < N; ++e) s += x[e];
         }
-        const float mu = ln_sum<256>(s, sm) / n;
+        const double mean = ln_sum64(s, sm64) / a.C;
+        const float mu = (float)mean, m1 = (float)(mean - mu);
         float q = 0.f;
         for (int c = threadIdx.x * N; c < a.C; c += 256 * N) {
             float x[N];
             row_floats<T>(row_load<T>(xr + c, a.C - c), x);
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                if (c + e < a.C) q += (x[e] - mu) * (x[e] - mu);
+                if (c + e < a.C) q += ((x[e] - mu) - m1) * ((x[e] - mu) - m1);
         }
         const float r = 1.0f / sqrtf(ln_sum<256>(q, sm) / n + a.eps);
         T* yr = (T*)a.y + row * a.ys;
@@ -172,7 +217,7 @@ __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(LnFwdArgs a) {
             ln_param<N>(a.w, c, a.C, 1.f, w);
             ln_param<N>(a.b, c, a.C, 0.f, b);
 #pragma unroll
-            for (int e = 0; e < N; ++e) x[e] = (x[e] - mu) * r * w[e] + b[e];
+            for (int e = 0; e < N; ++e) x[e] = ((x[e] - mu) - m1) * r * w[e] + b[e];
             row_store<T>(yr + c, a.C - c, x);
         }
         if (threadIdx.x == 0) {

@@ -754,3 +754,42 @@ def test_layer_norm_backward_of_large_constant_rows(ops, C, dtype):
     size = rstd.double()[:, None] * (d.abs() + d.abs().mean(-1, keepdim=True))
     _within(dx, ref, HALF[dt] * ref.abs() + _adds(C) * E32 * size, "dx")
     assert bool((dw == 0).all())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,C,value,spread", [(4, 551, 18223.738, 0.0), (7, 100, 1080.3, 0.0), (300, 255, 777.7, 0.0),
+                                                 (5, 1531, 9.1e5, 0.0), (3, 2052, 1e30, 0.0), (5, 6000, 3.3e4, 0.0),
+                                                 (2, 20011, 1.23e4, 0.0), (33, 551, 1e4, 1.0), (9, 3001, -3e5, 2.0),
+                                                 (2, 17001, 5e4, 0.5), (70, 64, 1e6, 4.0)])
+def test_layer_norm_of_rows_far_from_zero(ops, rows, C, value, spread, dtype):
+    """Rows whose mean is large against their deviation (none at all: constant rows give the bias)."""
+    dt = DT[dtype]
+    x = (value + spread * _rn(C, rows, C)).to(dt)
+    w, b = 1.0 + 0.2 * _rn(1, C), 0.3 * _rn(2, C)
+    y, mean, rstd = ops.layer_norm(x, w, b, stats=True)
+    ref, mu, r, xh = _ln_ref(x, w, b, 1e-5)
+    # The sums around a first mean, itself off by n E32 |mu|, add numbers of at most |x - mu| + n E32 |mu| (each difference is
+    # exact or rounded once), so the centre is off by n + 2 times E32 of that, as is a constant row's remainder; the mean is
+    # rounded to f32.
+    n = _adds(C)
+    xc = (x.double() - mu).abs()
+    around = xc.mean(-1, keepdim=True) + n * E32 * mu.abs()
+    off = (n + 2) * E32 * around + E32 * xc
+    assert spread == 0.0 or float((off * r).max()) < 0.05
+    rel = (n + 8) * E32 + (off * r).amax(-1, keepdim=True) ** 2
+    tol = HALF[dt] * ref.abs() + w.double().abs() * (off * r + xh.abs() * rel) + 2 * E32 * (ref.abs() + b.double().abs())
+    _within(y, ref, tol, "y")
+    _within(mean, mu[:, 0], 2 * E32 * mu[:, 0].abs() + off.amax(-1), "mean")
+    _within(rstd, r[:, 0], r[:, 0] * 2 * rel[:, 0], "rstd")
+    if spread == 0.0:
+        # the first mean is off by j steps of f32, j C far below 2^24: the remainder, its sum and its mean are exact
+        assert torch.equal(mean, x[:, 0].float()) and torch.equal(y, b.to(dt).expand(rows, C))
+
+
+def test_layer_norm_mean_of_rows_with_infinities(ops):
+    for C in (100, 6000, 17001):
+        x = _rn(C, 4, C)
+        x[1, C // 2], x[2, 3] = float("inf"), float("-inf")
+        y, mean, rstd = ops.layer_norm(x, stats=True)
+        assert float(mean[1]) == float("inf") and float(mean[2]) == float("-inf")
+        assert bool(torch.isnan(y[1:3]).all()) and bool(torch.isfinite(y[[0, 3]]).all())
