@@ -10,42 +10,96 @@ namespace ldm {
 
 namespace {
 
-// exp and the reciprocal by the hardware's instructions (one step of f32 each)
-__device__ __forceinline__ float lin_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
-// q = (1 - erf(|z| / sqrt 2)) / 2 and e = exp(-z^2 / 2): Abramowitz and Stegun 7.1.26, erfc(x) = t poly(t) exp(-x^2) with
-// t = 1 / (1 + 0.3275911 x), off by at most 1.5e-7.  A tile's epilogue has few cycles for this: 9 instructions, where the
-// library's erff would cost as much as a tile of 256 products.
-__device__ __forceinline__ float lin_tail(float z, float& e) {
-    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.23164189f, __builtin_fabsf(z), 1.0f));      // 0.3275911 / sqrt 2
-    float p = __builtin_fmaf(t, 0.5307027145f, -0.7265760135f);                                         // halved
-    p = __builtin_fmaf(t, p, 0.7107068705f);
-    p = __builtin_fmaf(t, p, -0.142248368f);
-    p = __builtin_fmaf(t, p, 0.127414796f);
-    const float u = z * 0.84932180028801905f;                                                           // sqrt(log2(e) / 2)
-    e = __builtin_amdgcn_exp2f(-u * u);
-    return t * p * e;
+// The activations, for outputs of type T.  f32 outputs are within 9 half steps of the value (above 2^-119): exponents are
+// taken in two parts and reciprocals get a step of Newton's.  For bf16 outputs 2^-11 of the value (GELU: down to -9) is enough, and a tile's
+// epilogue has few cycles: the hardware's exp2 and reciprocal as they are, a shorter polynomial.
+//
+// 1 / d, d >= 1
+template <typename T> __device__ __forceinline__ float lin_rcp(float d) {
+    const float t = __builtin_amdgcn_rcpf(d);
+    return sizeof(T) == 2 ? t : __builtin_fmaf(__builtin_fmaf(-d, t, 1.0f), t, t);
 }
-__device__ __forceinline__ float lin_act(float v, int act) {
-    if (act == LIN_SILU) return v * __builtin_amdgcn_rcpf(1.0f + lin_exp(-v));
+// exp(-y), y = hi + lo >= 0 with lo far below hi: exp2 of the rounded product, times 1 + what the rounding left
+__device__ __forceinline__ float lin_exp_neg(float hi, float lo) {
+    constexpr float c = -1.44269504088896341f, cl = (float)(-1.44269504088896341 - (double)c);
+    const float y = hi * c;
+    const float r = __builtin_fmaf(hi, cl, __builtin_fmaf(lo, c, __builtin_fmaf(hi, c, -y)));
+    const float e = __builtin_amdgcn_exp2f(y);
+    return __builtin_fmaf(e * r, 0.69314718055994531f, e);
+}
+// |z|, at most `most`; NaN stays NaN
+__device__ __forceinline__ float lin_abs(float z, float most) {
+    const float a = __builtin_fabsf(z);
+    return a > most ? most : a;
+}
+// q = (1 - erf(|z| / sqrt 2)) / 2 and e = exp(-z^2 / 2): q = t poly(t) e with t = 1 / (1 + p |z|), the form of Abramowitz and
+// Stegun 7.1.26 with coefficients fitted here (least largest error, by reweighted least squares).  f32: nine terms, off by
+// 3.2e-8 of q (4096 x 256 x 1024 with GELU: 27.4 us; five terms off by 1.5e-7 and no corrections: 25.8; without GELU: 24.2).
+// bf16: six terms, off by at most 2.5e-8 and, up to |z| = 9, by 2.1e-4 of q, in 12 instructions; the library's erff would cost
+// as much as a tile of 256 products.
+template <typename T> __device__ __forceinline__ float lin_tail(float z, float& e) {
+    if constexpr (sizeof(T) == 2) {
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.28f, __builtin_fabsf(z), 1.0f));
+        float p = __builtin_fmaf(t, -0.10303881f, 0.37849629f);
+        p = __builtin_fmaf(t, p, -0.21841556f);
+        p = __builtin_fmaf(t, p, 0.25384381f);
+        p = __builtin_fmaf(t, p, 0.07356371f);
+        p = __builtin_fmaf(t, p, 0.11555059f);
+        const float u = z * 0.84932180028801905f;                                                       // sqrt(log2(e) / 2)
+        e = __builtin_amdgcn_exp2f(-u * u);
+        return t * p * e;
+    } else {
+        const float a = lin_abs(z, 64.f), t = lin_rcp<T>(__builtin_fmaf(0.35f, a, 1.0f));
+        float p = __builtin_fmaf(t, -0.029108857736f, 0.143787875772f);
+        p = __builtin_fmaf(t, p, -0.255326569080f);
+        p = __builtin_fmaf(t, p, 0.158721208572f);
+        p = __builtin_fmaf(t, p, -0.022790208459f);
+        p = __builtin_fmaf(t, p, 0.105368971825f);
+        p = __builtin_fmaf(t, p, 0.119869142771f);
+        p = __builtin_fmaf(t, p, 0.139856696129f);
+        p = __builtin_fmaf(t, p, 0.139621704817f);
+        const float h = 0.5f * a, hi = h * a;
+        e = lin_exp_neg(hi, __builtin_fmaf(h, a, -hi));
+        return t * p * e;
+    }
+}
+// s = 1 / (1 + exp(-z)) and 1 - s
+template <typename T> __device__ __forceinline__ float lin_sigmoid(float z, float& rest) {
+    if constexpr (sizeof(T) == 2) {
+        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+        rest = 1.0f - s;
+        return s;
+    } else {
+        const float e = lin_exp_neg(lin_abs(z, 128.f), 0.f), r = lin_rcp<T>(1.0f + e), er = e * r;
+        rest = z < 0.f ? r : er;
+        return z < 0.f ? er : r;
+    }
+}
+template <typename T> __device__ __forceinline__ float lin_act(float v, int act) {
+    if (act == LIN_SILU) {
+        float rest;
+        return v * lin_sigmoid<T>(v, rest);
+    }
     if (act == LIN_RELU) return v < 0.f ? 0.f : v;
     if (act == LIN_GELU) {
         // v Phi(v) = max(v, 0) - |v| q on either side of zero; q is 0 long before |v| = 64, so infinities give the limits
         float e;
-        const float q = lin_tail(v, e);
+        const float q = lin_tail<T>(v, e);
         return __builtin_fmaf(-__builtin_amdgcn_fmed3f(__builtin_fabsf(v), 0.f, 64.f), q,
                               __builtin_amdgcn_fmed3f(v, 0.f, __builtin_inff()));
     }
     return v;
 }
-__device__ __forceinline__ float lin_dact(float z, int act) {
+template <typename T> __device__ __forceinline__ float lin_dact(float z, int act) {
     if (act == LIN_SILU) {
-        const float s = __builtin_amdgcn_rcpf(1.0f + lin_exp(-z));
-        return s * (1.0f + z * (1.0f - s));
+        float rest;
+        const float s = lin_sigmoid<T>(z, rest);
+        return __builtin_fmaf(s * z, rest, s);
     }
     if (act == LIN_RELU) return z > 0.f ? 1.f : 0.f;
     if (act == LIN_GELU) {
         float e;
-        const float q = lin_tail(z, e);
+        const float q = lin_tail<T>(z, e);
         return __builtin_fmaf(z * 0.39894228040143268f, e, z < 0.f ? q : 1.0f - q);
     }
     return 1.f;
@@ -75,7 +129,9 @@ __device__ __forceinline__ float lin_dact(float z, int act) {
 // a step's products: what is not a product has to fit between them.  (Walking over several tiles with the requests
 // running ahead over a tile's end was measured: its bookkeeping made the step longer than the first loads it hid,
 // 497 us against 459 for 65536 x 4096 x 1024.)
-// Fragment reads that the compiler does not wait for: GemmFrag::landed() behind an explicit wait makes the values usable.
+// Fragment reads that the compiler does not wait for: GemmFrag::landed() behind an explicit wait makes the values usable.  The
+// compiler may not touch such a register in between: tests/test_lds_reads.py looks for that in the built code, and for the
+// distances that gemm_mfma_in_place() needs.
 template <typename T, bool KC> struct GemmFrag;
 template <typename T> struct GemmFrag<T, true> {
     u32x4 v;
@@ -167,7 +223,7 @@ __device__ __forceinline__ void gemm_finish(const GemmArgs& a, long m, long n, c
             float x = v[e];
             if (a.res) x += (float)((const T*)a.res)[m * a.ldr + n + e];
             if (a.pre) ((T*)a.pre)[m * a.ldp + n + e] = (T)x;
-            ((T*)a.C)[m * a.ldc + n + e] = (T)lin_act(x, a.act);
+            ((T*)a.C)[m * a.ldc + n + e] = (T)lin_act<T>(x, a.act);
         }
 }
 __device__ __forceinline__ void gemm_bias(const GemmArgs& a, long n, float (&b)[8]) {
@@ -483,7 +539,7 @@ __global__ __launch_bounds__(256, F == 8 ? 1 : 2) void gemm_kernel(GemmArgs a) {
 #pragma unroll
                 for (int p = 0; p < G * P; ++p)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[p][e] = lin_act(v[p][e], A);
+                    for (int e = 0; e < 8; ++e) v[p][e] = lin_act<T>(v[p][e], A);
             };
             if (a.act == LIN_SILU) activate(std::integral_constant<int, LIN_SILU>{});
             else if (a.act == LIN_RELU) activate(std::integral_constant<int, LIN_RELU>{});
@@ -677,7 +733,7 @@ __global__ __launch_bounds__(256) void gemm_few_kernel(GemmArgs a) {
         if (e < left) {
             if (a.res) v[e] += (float)((const T*)a.res)[m * a.ldr + n + e];
             if (a.pre) ((T*)a.pre)[m * a.ldp + n + e] = (T)v[e];
-            ((T*)a.C)[m * a.ldc + n + e] = (T)lin_act(v[e], a.act);
+            ((T*)a.C)[m * a.ldc + n + e] = (T)lin_act<T>(v[e], a.act);
         }
 }
 
@@ -752,7 +808,7 @@ __global__ __launch_bounds__(256) void gemm_any_kernel(GemmArgs a) {
                 if (a.bias) v += a.bias[n];
                 if (a.res) v += (float)((const T*)a.res)[m * a.ldr + n];
                 if (a.pre) ((T*)a.pre)[m * a.ldp + n] = (T)v;
-                ((T*)a.C)[m * a.ldc + n] = (T)lin_act(v, a.act);
+                ((T*)a.C)[m * a.ldc + n] = (T)lin_act<T>(v, a.act);
             }
     }
 }
@@ -789,7 +845,7 @@ __device__ __forceinline__ void gemm_join(const GemmArgs& a, int parts, long i) 
         }
         if (a.pre) row_store<T>((T*)a.pre + m * a.ldp + n + h, left - h, v + h);
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[h + e] = lin_act(v[h + e], a.act);
+        for (int e = 0; e < V; ++e) v[h + e] = lin_act<T>(v[h + e], a.act);
         row_store<T>((T*)a.C + m * a.ldc + n + h, left - h, v + h);
     }
 }
@@ -858,7 +914,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long lddy, 
                 float p[V];
                 row_floats<T>(vp[u], p);
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[e] *= lin_dact(p[e], act);
+                for (int e = 0; e < V; ++e) v[e] *= lin_dact<T>(p[e], act);
                 row_store<T>(dz + r * lddz + n, r < M ? left : 0, v);
             }
             if (r < M) {

@@ -442,7 +442,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            res: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, save_pre: bool = False):
     """act(x @ weight + bias + res) (ldm_linear): x [..., K] and weight [K, N] (burn's Linear layout, or a transposed view
     of an [N, K] weight) in bf16 or f32, bias N values used in f32, res [..., N] in x's type, added before the activation
-    like a convolution's; act None, 'silu', 'relu' or 'gelu' (the exact one).  Products accumulate in f32.
+    like a convolution's; act None, 'silu', 'relu' or 'gelu' (z Phi(z), not the tanh form).  Products accumulate in f32.
+    Activations before the last rounding: within 9 half steps of f32 of their value; in bf16 within 2^-11 (GELU: down to z = -9).
     Returns the output in x's type, or (output, z) with save_pre: z, the value before the activation, is what
     linear_backward needs with one.  `out` may be res itself.  Rows of a matrix may lie up to 2^21 elements apart."""
     dev, K, N = _check_linear(x, weight, act)

@@ -381,6 +381,45 @@ def test_linear_backward(ops, M, K, N, dtype, order):
         assert part[0] is None and part[2] is None and torch.equal(part[1], dw)
 
 
+def _tail_points(act, dt):
+    """Arguments over which the activation falls from its value at zero to far below it, and its positive side."""
+    lo, hi = (-80.0, 80.0) if act == "silu" else (-12.5, 12.5) if dt == torch.float32 else (-9.0, 9.0)
+    z = torch.cat([torch.linspace(lo, hi, 8 * 640 - 640), 0.01 * torch.randn(640, generator=torch.Generator().manual_seed(1))])
+    return z.cuda().to(dt)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("C", [64, 20, 3])
+def test_activations_relative_to_their_value(ops, C, act, dtype):
+    """The negative tails, where the value is far below the argument: the identity as weight, so that z is exact."""
+    dt = DT[dtype]
+    z = _tail_points(act, dt)
+    x = z[:z.numel() // C * C].view(-1, C)
+    eye = torch.eye(C, dtype=dt, device="cuda")
+    zd = x.double()
+    phi, d_phi = 0.5 * torch.erfc(-zd / math.sqrt(2)), torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi)
+    s, rest = torch.sigmoid(zd), torch.sigmoid(-zd)
+    ref = zd * phi if act == "gelu" else zd * s
+    grad = phi + zd * d_phi if act == "gelu" else s + zd * s * rest
+    size = phi + zd.abs() * d_phi if act == "gelu" else s + zd.abs() * s * rest
+    # f32: the fit of the normal distribution's tail is off by E32 / 2, its nine steps by 2, its argument by 3, the exponential
+    # by 3, two products by 2; a sigmoid's exponential 3, sum, reciprocal and products 5.  bf16: 2^-11 of the value, or what
+    # |z| times the tail's 2.5e-8 and a few steps are, if that is less
+    if dt == torch.float32:
+        rel, least = 12 * E32, 12 * E32 * ref.abs()
+    else:
+        rel = 2.0 ** -11
+        least = torch.minimum(rel * ref.abs(), 8 * E32 * zd.abs()) if act == "gelu" else (1.5 * zd.abs() + 8) * E32 * ref.abs()
+    tiny = 2.0 ** -119                                              # exponentials below the least normal number are zero
+    for M in (1, 60, x.shape[0]):                                   # few rows, one tile, many
+        got, pre = ops.linear(x[:M], eye, act=act, save_pre=True)
+        assert torch.equal(pre, x[:M])
+        _within(got, ref[:M], (HALF[dt] * ref.abs() + least + tiny)[:M], ("value", M))
+    _, _, _, dz = ops.linear_backward(torch.ones_like(x), x, eye, pre=x, act=act, dx=False, dweight=False)
+    _within(dz, grad, HALF[dt] * grad.abs() + (12 * E32 if dt == torch.float32 else rel) * size + tiny, "gradient")
+
+
 def test_linear_gradient_against_differences(ops):
     M, K, N = 12, 40, 56
     x, w, b, r, c = _rn(1, M, K), _rn(2, K, N) * K ** -0.5, _rn(3, N), _rn(4, M, N), _rn(5, M, N)
