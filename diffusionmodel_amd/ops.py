@@ -12,6 +12,7 @@ import struct
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -147,19 +148,30 @@ def _data(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _check_bits(name: str, t: torch.Tensor) -> None:
+    """The library reads a tensor's memory: what torch keeps beside it would be lost without a word."""
+    if t.is_neg():
+        raise ValueError(f"{name} is a negated view whose memory holds the opposite values: call resolve_neg() on it first")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a forward-mode tangent, which this operator does not propagate: unpack it first")
+
+
 def _check(name: str, t, dev: int = -1, dtypes=_TD) -> int:
     """A device tensor of one of `dtypes`, on device `dev` (-1: any), that needs no gradient.  Returns its device."""
-    if isinstance(t, torch.Tensor) and t.dtype in dtypes and not t.requires_grad:
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and not t.requires_grad and not t.is_neg() \
+            and forward_ad._current_level < 0:
         d = t.get_device()
         if d >= 0 and (dev < 0 or d == dev):
             return d
+    if isinstance(t, torch.Tensor):
+        _check_bits(name, t)
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a device tensor")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} is {t.dtype}, expected one of {tuple(str(d) for d in dtypes)}")
     if dev >= 0 and t.get_device() != dev:
         raise ValueError(f"{name} is on device {t.get_device()}, expected {dev}")
-    if torch.is_grad_enabled():
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which this operator does not record: call it under "
                          "torch.no_grad() and use the operator's backward function")
     return t.get_device()

@@ -148,3 +148,23 @@ def test_launches_beyond_the_grid_are_refused(lib):
                                    None) == 1
     assert lib.ldm_rope(F32, P, None, P, None, struct.pack("12l", *([2048] * 12)), 32768, 65535, 1, 0, 2048, P, 0,
                         struct.pack("3l", 0, 4, 1), P, struct.pack("i", 1024), 1, 0, 0, None) == 1
+
+
+def test_what_torch_keeps_beside_the_memory_is_refused():
+    """Forward-mode tangents and negated views have a data pointer like any tensor; the values would be misread."""
+    from torch.autograd import forward_ad
+    from diffusionmodel_amd import ops
+    x = torch.randn(4, 8)
+    ops._check_bits("x", x)
+    with pytest.raises(ValueError, match="resolve_neg"):
+        ops._check_bits("x", torch._neg_view(x))
+    ops._check_bits("x", torch._neg_view(x).resolve_neg())
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        ops._check_bits("x", x)
+        for t in (dual, dual[1:], dual.view(-1)):
+            with pytest.raises(ValueError, match="tangent"):
+                ops._check_bits("x", t)
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                ops._check("x", t)
+        ops._check_bits("x", forward_ad.unpack_dual(dual).primal)

@@ -832,3 +832,27 @@ def test_layer_norm_mean_of_rows_with_infinities(ops):
         y, mean, rstd = ops.layer_norm(x, stats=True)
         assert float(mean[1]) == float("inf") and float(mean[2]) == float("-inf")
         assert bool(torch.isnan(y[1:3]).all()) and bool(torch.isfinite(y[[0, 3]]).all())
+
+
+def test_tangents_and_negated_views_are_refused(ops):
+    from torch.autograd import forward_ad
+    x, w, q = _rn(1, 6, 32), _rn(2, 32, 16), _rn(3, 1, 2, 1, 8)
+    _, m, r = ops.layer_norm(x, stats=True)
+    inv, pos = ops.rope_frequencies((4,), device="cuda"), torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    calls = {"layer_norm": (lambda *t: ops.layer_norm(*t), (x, x[0], x[1])),
+             "layer_norm_backward": (lambda *t: ops.layer_norm_backward(*t, param_grads=True), (x, x, m, r, x[0], x)),
+             "rope": (lambda q, k, p, f: ops.rope(q, k, p, f), (q, q.clone(), pos.float(), inv)),
+             "linear": (lambda x, w, b, res: ops.linear(x, w, b, res=res), (x, w, w[0], x[:, :16].contiguous())),
+             "linear_backward": (lambda dy, x, w, p: ops.linear_backward(dy, x, w, pre=p, act="silu"),
+                                 (x[:, :16], x, w, x[:, 16:]))}
+    with forward_ad.dual_level():
+        for name, (f, args) in calls.items():
+            f(*args)
+            for i, t in enumerate(args):
+                for bad in (forward_ad.make_dual(t, torch.ones_like(t)), torch._neg_view(t)):
+                    with torch.no_grad(), pytest.raises(ValueError):
+                        f(*args[:i], bad, *args[i + 1:])
+                        print("not refused:", name, i, flush=True)
+    out = torch._neg_view(torch.empty_like(x))
+    with pytest.raises(ValueError):
+        ops.layer_norm(x, out=out)
