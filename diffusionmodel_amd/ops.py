@@ -377,10 +377,16 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, in
         _check_out("out[0]", oq, q.shape, q, (k, positions, inv_freq), same=q)
         if k is not None:
             _check_out("out[1]", ok, k.shape, q, (q, oq, positions, inv_freq), same=k)
+    if sections is not None:
+        # (as whole numbers before the plans are searched, where 4.0 or a tensor would find what 4 left)
+        try:
+            sections = tuple(map(operator.index, sections))
+        except TypeError:
+            raise ValueError(f"sections must be whole numbers, got {sections}") from None
     strides, dims, pos_strides, sec, axes = _rope_plan(
         q.shape, q.stride(), None if k is None else k.shape, None if k is None else k.stride(), oq.stride(),
         None if k is None else ok.stride(), positions.shape, positions.stride(), inv_freq.numel(),
-        sections if sections is None else tuple(sections), layout)
+        sections, layout)
     if q.numel():
         _call(_lib.load().ldm_rope, dev, _TD[q.dtype], q.data_ptr(), _data(k), oq.data_ptr(), _data(ok), strides, *dims,
               positions.data_ptr(), _POS_TYPES[positions.dtype], pos_strides, inv_freq.data_ptr(), sec, axes,
@@ -403,10 +409,7 @@ def _rope_plan(qs, sq, ks, sk, so, sok, ps, pp, P, sections, layout):
         Hk = ks[2]
     if D < 1 or Hq < 1 or (ks is not None and Hk < 1) or (D > 1 and not sq[3] == sk[3] == so[3] == sok[3] == 1):
         raise ValueError("q, k and their outputs need at least one head and contiguous head vectors")
-    try:
-        sec = (P,) if sections is None else tuple(operator.index(n) for n in sections)
-    except TypeError:
-        raise ValueError(f"sections must be whole numbers, got {sections}") from None
+    sec = (P,) if sections is None else sections
     if not 1 <= len(sec) <= 4 or min(sec) < 0 or sum(sec) != P or P < 1 or 2 * P > D:
         raise ValueError(f"sections {sec} must hold one to four counts that add up to inv_freq's {P} pairs, at most D / 2")
     if len(ps) == 2:

@@ -856,3 +856,17 @@ def test_tangents_and_negated_views_are_refused(ops):
     out = torch._neg_view(torch.empty_like(x))
     with pytest.raises(ValueError):
         ops.layer_norm(x, out=out)
+
+
+def test_rope_sections_are_whole_numbers_whatever_was_called_before(ops):
+    q = _rn(1, 2, 5, 4, 16)
+    inv, pos = ops.rope_frequencies((4, 4), device="cuda"), torch.arange(10, device="cuda").view(2, 5)
+    want = ops.rope(q, None, pos, inv, sections=(4, 4))
+    for bad in ((4.0, 4.0), [4, 4.0], (torch.tensor(4.0), 4), 8, ("4", "4")):
+        with pytest.raises(ValueError):
+            ops.rope(q, None, pos, inv, sections=bad)
+            print("not refused:", bad, flush=True)
+    changing = [torch.tensor(4), torch.tensor(4)]                   # read at each call
+    assert torch.equal(ops.rope(q, None, pos, inv, sections=changing), want)
+    changing[0].fill_(2), changing[1].fill_(6)
+    assert torch.equal(ops.rope(q, None, pos, inv, sections=changing), ops.rope(q, None, pos, inv, sections=(2, 6)))
