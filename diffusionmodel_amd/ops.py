@@ -270,6 +270,13 @@ def _call(fn, dev: int, *args) -> None:
         _lib.check(rc)
 
 
+def _columns(t: torch.Tensor) -> int:
+    """Elements of t's last axis; the library's norms take up to 2^24 (and a larger count would not survive its 32 bits)."""
+    if t.dim() < 1 or not 1 <= t.size(-1) <= 1 << 24:
+        raise ValueError("x must have a last axis of 1 to 2^24 elements")
+    return t.size(-1)
+
+
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5, out: Optional[torch.Tensor] = None, stats: bool = False):
     """y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis of x [..., C] (bf16 or f32, last axis
@@ -278,11 +285,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     `out` may be x itself."""
     dev = _check("x", x)
     shape = x.shape
-    if not shape or shape[-1] < 1:
-        raise ValueError("x must have a last axis of at least one element")
+    Cc = _columns(x)
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    Cc = shape[-1]
     rows, xs = _rows("x", x)
     w, b = _params("weight", weight, Cc, dev), _params("bias", bias, Cc, dev)
     if out is None:
@@ -307,8 +312,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     mean and rstd are the forward pass's statistics; `add` (x's shape and type) is added to dx, the gradient that
     reaches x by the residual branch.  param_grads=False (the default without a weight) leaves dweight and dbias None."""
     dev = _check("x", x)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("x must have a last axis of at least one element")
+    Cc = _columns(x)
     for name, t in (("dy", dy), ("add", add)):
         if t is not None or name == "dy":
             _check(name, t, dev, (x.dtype,))
@@ -318,7 +322,6 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
         _check(name, t, dev, _F32)
         if t.shape != x.shape[:-1] or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous with shape {tuple(x.shape[:-1])}")
-    Cc = x.shape[-1]
     rows, xs = _rows("x", x)
     dys = _rows("dy", dy)[1]
     adds = 0 if add is None else _rows("add", add)[1]
@@ -407,6 +410,8 @@ def _rope_plan(qs, sq, ks, sk, so, sok, ps, pp, P, sections, layout):
         if len(ks) != 4 or ks[0] != B or ks[1] != N or ks[3] != D:
             raise ValueError(f"k must be [{B}, {N}, heads, {D}], has shape {tuple(ks)}")
         Hk = ks[2]
+    if max(B, N, Hq, Hk, D) >= 1 << 31:
+        raise ValueError("B, N, heads and D must be below 2^31")
     if D < 1 or Hq < 1 or (ks is not None and Hk < 1) or (D > 1 and not sq[3] == sk[3] == so[3] == sok[3] == 1):
         raise ValueError("q, k and their outputs need at least one head and contiguous head vectors")
     sec = (P,) if sections is None else sections

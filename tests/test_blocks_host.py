@@ -168,3 +168,22 @@ def test_what_torch_keeps_beside_the_memory_is_refused():
             with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
                 ops._check("x", t)
         ops._check_bits("x", forward_ad.unpack_dual(dual).primal)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """The C ABI's int arguments would take the low 32 bits: 2^32 + 8 columns would be 8."""
+    from diffusionmodel_amd import ops
+    for n in (2 ** 32 + 8, 2 ** 31, 2 ** 24 + 1, 0):
+        with pytest.raises(ValueError, match="last axis"):
+            ops._columns(torch.empty(1, n, device="meta"))
+    with pytest.raises(ValueError, match="last axis"):
+        ops._columns(torch.empty((), device="meta"))
+    assert ops._columns(torch.empty(3, 1 << 24, device="meta")) == 1 << 24
+
+    def plan(B, N, H, D):
+        st = (N * H * D, H * D, D, 1)
+        return ops._rope_plan((B, N, H, D), st, None, None, st, None, (1, N), (N, 1), 4, (4,), "half")
+    assert plan(2, 3, 4, 8)[1] == (2, 3, 4, 0, 8)
+    for dims in ((2 ** 32 + 1, 1, 1, 8), (1, 2 ** 32 + 5, 1, 8), (1, 1, 2 ** 32 + 1, 8), (1, 1, 1, 2 ** 32 + 8), (1, 2 ** 31, 1, 8)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            plan(*dims)
