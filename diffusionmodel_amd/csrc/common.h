@@ -155,6 +155,8 @@ int launch_tapconv(const PackedConv& pc, const ConvCall& cc, hipStream_t stream)
 // Name of the kernel the calling thread's last launch_tapconv / launch_upfuse started, spelled as a profiler lists it
 // ("void ldm::tapconv_kernel<unsigned short, 16, 64, 4, 2, 1, 3, 9, 2, 3, 9>(ldm::TapConvArgs)"); "" before the first.
 const char* tapconv_last_kernel();
+// The same for the matrix products of linear.hip, by their template arguments: a name that stays for the process.
+void set_last_kernel(const char* name);
 
 // ---------------------------------------------------------------------------------------------
 // Attention core: softmax(q k^T / sqrt(C)) v over the tokens of one image, single head.

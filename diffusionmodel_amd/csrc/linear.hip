@@ -4,6 +4,7 @@
 // contraction (KC) or along its other index.
 #include "blocks.h"
 #include "vec.h"
+#include <cstdio>
 #include <type_traits>
 
 namespace ldm {
@@ -999,10 +1000,37 @@ int gemm_tile_with_epilogue(const GemmArgs& a, int steps) {
 }
 long gemm_part_floats(const GemmPlan& p, long M, long N) { return p.parts > 1 ? p.parts * M * ((N + 7) & ~7L) : 0; }
 
+// what ldm_last_kernel() says of a product
+#define GEMM_BOOL(b) ((b) ? "true" : "false")
+#define GEMM_TYPE(T) (sizeof(T) == 2 ? "bf16" : "f32")
+template <typename T, bool AKC, bool BKC, int F, bool DMA>
+const char* gemm_name() {
+    static char name[64];
+    static const int n = snprintf(name, sizeof name, "gemm_kernel<%s, %s, %s, %d, %s>", GEMM_TYPE(T), GEMM_BOOL(AKC), GEMM_BOOL(BKC), F,
+                                  GEMM_BOOL(DMA));
+    (void)n;
+    return name;
+}
+template <typename T, bool BKC>
+const char* gemm_few_name() {
+    static char name[64];
+    static const int n = snprintf(name, sizeof name, "gemm_few_kernel<%s, %s>", GEMM_TYPE(T), GEMM_BOOL(BKC));
+    (void)n;
+    return name;
+}
+template <typename T, bool AKC, bool BKC>
+const char* gemm_any_name() {
+    static char name[64];
+    static const int n = snprintf(name, sizeof name, "gemm_any_kernel<%s, %s, %s>", GEMM_TYPE(T), GEMM_BOOL(AKC), GEMM_BOOL(BKC));
+    (void)n;
+    return name;
+}
+
 template <typename T, bool AKC, bool BKC, int F, bool DMA>
 int gemm_launch(const GemmArgs& a, unsigned grid, hipStream_t s) {
     static bool done[kMaxDevices] = {};
     LDM_TRY(allow_dynamic_lds((const void*)&gemm_kernel<T, AKC, BKC, F, DMA>, gemm_lds(F, DMA), done));
+    set_last_kernel(gemm_name<T, AKC, BKC, F, DMA>());
     gemm_kernel<T, AKC, BKC, F, DMA><<<grid, 256, gemm_lds(F, DMA), s>>>(a);
     LDM_HIP(hipGetLastError());
     return LDM_OK;
@@ -1037,6 +1065,7 @@ int gemm(GemmArgs a, float* ws, GemmJoin* later, hipStream_t s) {
             LDM_TRY(allow_dynamic_lds((const void*)&gemm_few_kernel<T, BKC>, lds, done));
             const long grid = (a.M + 31) / 32 * ((a.N + 31) / 32);
             LDM_REQUIRE(grid < kMostTiles, "more output tiles than one launch holds");
+            set_last_kernel(gemm_few_name<T, BKC>());
             gemm_few_kernel<T, BKC><<<(unsigned)grid, 256, lds, s>>>(a);
             LDM_HIP(hipGetLastError());
             return LDM_OK;
@@ -1055,6 +1084,7 @@ int gemm(GemmArgs a, float* ws, GemmJoin* later, hipStream_t s) {
     a.kper = p.kper;
     a.part = p.parts > 1 ? ws : nullptr;
     if (any) {
+        set_last_kernel(gemm_any_name<T, AKC, BKC>());
         gemm_any_kernel<T, AKC, BKC><<<(unsigned)tiles, 256, 0, s>>>(a);
         LDM_HIP(hipGetLastError());
     } else if (!dma && p.F == 2) LDM_TRY((gemm_launch<T, AKC, BKC, 2, false>(a, (unsigned)tiles, s)));

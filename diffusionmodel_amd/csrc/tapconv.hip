@@ -2351,6 +2351,7 @@ __global__ __launch_bounds__(64 * NWV) void skinny3x3_kernel(const TapConvArgs a
 // ---------------------------------------------------------------------------------------------
 static thread_local const char* g_last_kernel = "";
 const char* tapconv_last_kernel() { return g_last_kernel; }
+void set_last_kernel(const char* name) { g_last_kernel = name; }
 
 template <typename T> static const char* type_name() { return sizeof(T) == 2 ? "unsigned short" : "float"; }
 

@@ -195,7 +195,9 @@ void ldm_conv_destroy(ldm_conv* c);
 /* Diagnostics (no counterpart in the reference): the name of the convolution kernel that the calling thread's last
  * ldm_conv_forward (or any other convolution launch of the library) started, spelled as rocprofv3 lists it, e.g.
  * "void ldm::tapconv_kernel<unsigned short, 16, 64, 4, 2, 1, 3, 9, 2, 3, 9>(ldm::TapConvArgs)".  bench.py uses it to
- * pick the hardware-counter record that belongs to the kernel it timed. */
+ * pick the hardware-counter record that belongs to the kernel it timed.  After ldm_linear and ldm_linear_backward it names the
+ * kernel of their last product by its template arguments: "gemm_kernel<bf16, rows of A along k, columns of B along k, F, direct>"
+ * (true or false, tiles of 32 F squared), "gemm_few_kernel<bf16, columns of B along k>" or "gemm_any_kernel<...>". */
 const char* ldm_last_kernel(void);
 
 /* ---- operators of transformer blocks over latent tokens (no counterpart in the reference) ---- */

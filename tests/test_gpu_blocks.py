@@ -870,3 +870,66 @@ def test_rope_sections_are_whole_numbers_whatever_was_called_before(ops):
     assert torch.equal(ops.rope(q, None, pos, inv, sections=changing), want)
     changing[0].fill_(2), changing[1].fill_(6)
     assert torch.equal(ops.rope(q, None, pos, inv, sections=changing), ops.rope(q, None, pos, inv, sections=(2, 6)))
+
+
+# ---- the largest tile ---------------------------------------------------------------------------------------------------
+def _last_kernel():
+    from diffusionmodel_amd import _lib
+    return _lib.load().ldm_last_kernel().decode()
+
+
+@pytest.mark.parametrize("M,K,N,order", [(4093, 1032, 4077, "nk"), (4093, 1032, 4072, "kn"), (4085, 4104, 4088, "nk"),
+                                         (4081, 4104, 4096, "kn")])
+def test_linear_on_the_largest_tile(ops, M, K, N, order):
+    """Dense rows in every fragment, ragged rows and columns, bias, residual, activations and z; the tile is asserted, so that
+    another choice of tiles cannot take these cases elsewhere."""
+    dt = torch.bfloat16
+    x, w = _rn(M + K, M, K).to(dt), _weights(N, K, N, dt, order)
+    b, res = 0.5 * _rn(1, N), _rn(2, M, N).to(dt)
+    z0 = x.double() @ w.double()
+    size = x.double().abs() @ w.double().abs()
+    print("linear", order, M, K, N, flush=True)
+    for bias, r, act, save in ((None, None, None, False), (b, None, "gelu", True), (b, res, "silu", True), (None, res, "relu", False),
+                               (b, res, None, False), (b, None, "relu", True), (b, None, "silu", False), (b, res, "gelu", True)):
+        got = ops.linear(x, w, bias, act=act, res=r, save_pre=save)
+        assert _last_kernel() == f"gemm_kernel<bf16, true, {'true' if order == 'nk' else 'false'}, 8, true>", (act, r is None)
+        out, pre = got if save else (got, None)
+        z = z0 + (0 if bias is None else bias.double()) + (0 if r is None else r.double())
+        tz = (K + 8) * E32 * (size + (0 if bias is None else bias.double().abs()) + (0 if r is None else r.double().abs()))
+        if save:
+            _within(pre, z, HALF[dt] * z.abs() + tz, ("pre", act))
+        ref = _act_ref(z, act)
+        _within(out, ref, HALF[dt] * ref.abs() + 1.13 * tz + 8 * E32 * z.abs(), ("out", act))
+    # in place on the residual stream, and rows that are slices
+    stream = res.clone()
+    ops.linear(x, w, b, act="silu", res=stream, out=stream)
+    assert torch.equal(stream, ops.linear(x, w, b, act="silu", res=res))
+    big = torch.full((M, N + 16), 9.0, dtype=dt, device="cuda")
+    ops.linear(x, w, b, act="silu", res=res, out=big[:, 8:8 + N])
+    assert torch.equal(big[:, 8:8 + N], stream) and bool((big[:, :8] == 9).all()) and bool((big[:, 8 + N:] == 9).all())
+
+
+# (rows, K, N): gradients on the largest tile of the input and, with a short or with a long contraction (in parts), the weight
+@pytest.mark.parametrize("order", ["kn", "nk"])
+@pytest.mark.parametrize("M,K,N,of_x", [(4093, 4080, 1032, True), (1032, 4080, 4088, False), (9001, 2040, 2056, False)])
+def test_linear_backward_on_the_largest_tile(ops, M, K, N, of_x, order):
+    dt = torch.bfloat16
+    x, w = _rn(M + K, M, K).to(dt), _weights(N, K, N, dt, order)
+    dy, pre = _rn(5, M, N).to(dt), _rn(6, M, N).to(dt)
+    print("linear_backward", order, M, K, N, flush=True)
+    for act in (None, "gelu"):
+        gx, gw, gb, dz = ops.linear_backward(dy, x, w, pre=pre if act else None, act=act, dx=of_x, dweight=not of_x)
+        kernel = f"gemm_kernel<bf16, true, {'true' if order == 'kn' else 'false'}, 8, true>" if of_x \
+            else "gemm_kernel<bf16, false, false, 8, true>"
+        assert _last_kernel() == kernel
+        rz = dy.double() * _dact_ref(pre.double(), act)
+        ez = 16 * E32 * dy.double().abs() * (1 + pre.double().abs()) if act else torch.zeros_like(rz)
+        if act:
+            _within(dz, rz, HALF[dt] * rz.abs() + ez, ("dz", act))
+        d = dz.double()                            # the products' operand, as it is
+        if of_x:
+            ref, sz, n = d @ w.double().t(), d.abs() @ w.double().abs().t(), N
+        else:
+            ref, sz, n = x.double().t() @ d, x.double().abs().t() @ d.abs(), M
+        _within(gx if of_x else gw, ref, HALF[dt] * ref.abs() + (n + 8) * E32 * sz, ("gradient", act))
+        _within(gb, rz.sum(0), ez.sum(0) + (M + 8) * E32 * rz.abs().sum(0), ("db", act))
