@@ -3,11 +3,12 @@
 //   dx = r (g - mean(g) - xh mean(g xh)) + add,   xh = (x - mu) r, g = dy w;   dw = sum_rows dy xh, db = sum_rows dy
 // Both passes are bound by HBM: one read of each input and one write of the output.  A row lives in the registers of its
 // LPR lanes (a part of a wave, a wave, or a workgroup), so the mean, the centred sum of squares and the output come from
-// one read.  Statistics and sums are f32 (the mean of rows that are read again: f64); the mean is corrected by the mean of
-// what is left around it, and the variance is the sum of squares around it (E[x^2] - mu^2 would lose it for rows far from
-// zero).
-// Measured (a large copy: 5.0 TB/s): forward 65536 x 1024 bf16 44 us = 6.1 TB/s, partly from the memory-side cache, 20011 x
-// 1031 f32 32 us = 5.2 TB/s; backward 65536 x 1024 bf16 with `add` 105 us = 5.1 TB/s and 5 us for the partial rows.
+// one read.  Statistics and sums are f32 (the mean of rows that are read again: f64).  The variance is the sum of squares
+// around the mean that was just found (E[x^2] - mu^2 would lose it for rows far from zero), and that mean is corrected where it
+// is more than two deviations from zero.
+// Measured (a large copy: 5.0 TB/s): forward 65536 x 1024 bf16 44 us = 6.1 TB/s, partly from the memory-side cache (46 where
+// every row is far from zero), 20011 x 1031 f32 30.5 us = 5.4 TB/s (38); backward 65536 x 1024 bf16 with `add` 105 us = 5.1 TB/s
+// and 5 us for the partial rows.
 // Rows need no alignment: 16-byte vector accesses at element alignment, which this target's global memory serves.
 #include "blocks.h"
 #include "vec.h"
@@ -86,10 +87,8 @@ __device__ __forceinline__ double ln_sum64(double a, double* sm) {
     return (sm[0] + sm[1]) + (sm[2] + sm[3]);
 }
 
-// (the two vectors of a wave's bf16 row take two registers more than six waves on a SIMD have: 65536 x 1024 45.3 us with five
-// waves, 44.1 with six)
 template <typename T, int NV, int LPR>
-__global__ __launch_bounds__(ln_block(LPR), sizeof(T) == 2 && NV == 2 && LPR == 64 ? 6 : 1) void ln_fwd_kernel(LnFwdArgs a) {
+__global__ __launch_bounds__(ln_block(LPR)) void ln_fwd_kernel(LnFwdArgs a) {
     constexpr int N = RowVec<T>::N, RPB = ln_block(LPR) / LPR;
     __shared__ float sm[16];
     const int l = threadIdx.x % LPR;
@@ -119,64 +118,61 @@ __global__ __launch_bounds__(ln_block(LPR), sizeof(T) == 2 && NV == 2 && LPR == 
             for (int e = 0; e < N; ++e) s += x[v][e];
         }
         if (row + step < a.rows) fetch(row + step);
-        // The first mean m0 is off by the rounding of its sum, which rows far from zero would see as a shift and as variance.
-        // What is left around it is small, so its mean m1 corrects m0 to the last bit: the variance is the mean square
-        // around m0 less m1^2, in one reduction.
-        float m0 = ln_sum<LPR>(s, sm);
+        const float sum = ln_sum<LPR>(s, sm);
+        float m0;
         {
 #pragma clang fp contract(off)
-            m0 *= inv;                   // rounded before it is used: m1 belongs to this value
+            m0 = sum * inv;              // rounded before it is used: m1 belongs to this value
         }
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int e = 0; e < N; ++e) x[v][e] -= m0;
-        // sums of x - c and its square (a condition per vector, not per element: those would be kept over the rows in more
-        // registers than there are)
-        auto around = [&](float c, float& s, float& q) {
-            s = q = 0.f;
+        // sum of f(x) over the row (a condition per vector, not per element: those would be kept over the rows in more registers
+        // than there are)
+        auto over_row = [&](auto f) {
+            float t = 0.f;
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 const int left = a.C - (v * LPR + l) * N;
-                auto add = [&](int e) {
-                    const float d = x[v][e] - c;
-                    s += d;
-                    q += d * d;
-                };
                 if (left >= N) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) add(e);
+                    for (int e = 0; e < N; ++e) t += f(x[v][e]);
                 } else if (left > 0) {
                     asm volatile("" ::: "memory");
 #pragma unroll
-                    for (int e = 0; e < N - 1; ++e)
-                        if (e < left) add(e);
+                    for (int e = 0; e < N - 1; ++e) t += e < left ? f(x[v][e]) : 0.f;
                 }
             }
-            ln_sum2<LPR>(s, q, sm);
+            return ln_sum<LPR>(t, sm);
         };
-        float q;
-        around(0.f, s, q);
-        const float m1 = s / n;                            // (divided by: the mean of a constant row is exact)
-        float var = q * inv - m1 * m1;
-        // (rows of nearly one value, where that difference would cancel, and squares past the largest f32: once more)
-        const bool again = m1 != 0.f && !(m1 * m1 < 0.0625f * inv * q);
-        if (__any(again)) {
-            around(m1, s, q);
-            if (again) var = q * inv;
+        auto square = [](float d) { return d * d; };
+        float q = over_row(square), m1 = 0.f;
+        // m0 is off by the rounding of its sum, which rows far from zero would see as a shift and as variance.  What is left
+        // around m0 is small there and exact, so its mean m1 corrects m0 to the last bit.  (Within two deviations of zero the
+        // differences' own rounding would be the larger error.)
+        const bool near = m0 * m0 <= 4.f * inv * q && q < __builtin_inff();
+        if (__any(!near)) {
+            m1 = over_row([](float d) { return d; }) / n;       // (divided by: the mean of a constant row is exact)
+            if (near) m1 = 0.f;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int e = 0; e < N; ++e) x[v][e] -= m1;
+            q = over_row(square);
         }
-        const float mu = m1 == m1 ? m0 + m1 : m0;          // (a row with an infinity has an infinite mean)
-        const float r = 1.0f / sqrtf(var + a.eps);
+        const float r = 1.0f / sqrtf(q * inv + a.eps);
         T* yr = (T*)a.y + row * a.ys;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             float o[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) o[e] = (x[v][e] - m1) * r * w[v][e] + b[v][e];
+            for (int e = 0; e < N; ++e) o[e] = x[v][e] * r * w[v][e] + b[v][e];
             row_store<T>(yr + (v * LPR + l) * N, a.C - (v * LPR + l) * N, o);
         }
         if (l == 0) {
-            if (a.mean) a.mean[row] = mu;
+            // (a row with an infinity has an infinite mean)
+            if (a.mean) a.mean[row] = near ? sum / n : m1 == m1 ? m0 + m1 : m0;
             if (a.rstd) a.rstd[row] = r;
         }
     }

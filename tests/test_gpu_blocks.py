@@ -933,3 +933,16 @@ def test_linear_backward_on_the_largest_tile(ops, M, K, N, of_x, order):
             ref, sz, n = x.double().t() @ d, x.double().abs().t() @ d.abs(), M
         _within(gx if of_x else gw, ref, HALF[dt] * ref.abs() + (n + 8) * E32 * sz, ("gradient", act))
         _within(gb, rz.sum(0), ez.sum(0) + (M + 8) * E32 * rz.abs().sum(0), ("db", act))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("C", [3, 64, 250, 1031, 2500, 6000, 17001])
+def test_layer_norm_mean_of_exact_sums(ops, C, dtype):
+    """Rows of small whole numbers around zero: every partial sum is exact, and so is the mean but for the division."""
+    x = torch.randint(-9, 10, (40, C), generator=torch.Generator().manual_seed(C)).cuda().to(DT[dtype])
+    _, mean, rstd = ops.layer_norm(x, stats=True)
+    mu = x.double().mean(-1)
+    _within(mean, mu, E32 * mu.abs(), "mean")
+    var = ((x.double() - mu[:, None]) ** 2).mean(-1)
+    r = 1.0 / torch.sqrt(var + 1e-5)
+    _within(rstd, r, r * (_adds(C) + 8) * E32, "rstd")
