@@ -12,8 +12,8 @@ namespace ldm {
 namespace {
 
 // The activations, for outputs of type T.  f32 outputs are within 9 half steps of the value (above 2^-119): exponents are
-// taken in two parts and reciprocals get a step of Newton's.  For bf16 outputs 2^-11 of the value (GELU: down to -9) is enough, and a tile's
-// epilogue has few cycles: the hardware's exp2 and reciprocal as they are, a shorter polynomial.
+// taken in two parts and reciprocals get a step of Newton's.  For bf16 outputs 2^-11 of the value (GELU: down to -9) is enough,
+// and a tile's epilogue has few cycles: the hardware's exp2 and reciprocal as they are, a shorter polynomial.
 //
 // 1 / d, d >= 1
 template <typename T> __device__ __forceinline__ float lin_rcp(float d) {
@@ -121,7 +121,7 @@ template <typename T> __device__ __forceinline__ float lin_dact(float z, int act
 // fragments and asks for the step NS later.  One barrier per step; nothing in front of a product is read later than one
 // half step before it.
 //
-// Bound by the matrix cores (256 tile, long contractions: 65536 x 4096 x 1024 bf16 in 440 us = 1.25 PFLOP/s, the rate this
+// Bound by the matrix cores (256 tile, long contractions: 65536 x 4096 x 1024 bf16 in 443 us = 1.24 PFLOP/s, the rate this
 // chip's clock holds under such load; a step alone runs at 1.4), by the epilogue's stores and arithmetic for short ones
 // (16384 x 256 x 1024 with GELU and the value before it: 24 us with 128 tiles, 28 with 256, of which the
 // products are 7), by LDS reads for the 64 tile.
@@ -857,7 +857,7 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a, int parts) {
 
 // What the backward pass leaves for its end, in one launch (each costs some 4 us): the joins of dx and dw, and the bias
 // gradient's sums over the dz kernel's workgroups, 16 threads per column, in a fixed order.
-// 1001 x 321 -> 643 f32: 47.1 us with three launches, 39.8 with one; 16384 x 1024 -> 4096 bf16: 330 and 332
+// 1001 x 321 -> 643 f32: 47.1 us with three launches, 39.8 with one; 16384 x 1024 -> 4096 bf16: the same within 1 %
 template <typename T>
 __global__ __launch_bounds__(256) void linear_finish_kernel(GemmArgs x, int xparts, unsigned xblocks, GemmArgs w, int wparts,
                                                             unsigned sblocks, const float* part, int G, long N, float* db) {
@@ -885,9 +885,12 @@ __global__ __launch_bounds__(256) void linear_finish_kernel(GemmArgs x, int xpar
     }
 }
 
-// dz = dy act'(pre), and the column sums of dz over this workgroup's rows (part [gridDim.x][N]).  One pass over dy and pre
-// and one write, bound by HBM: a thread keeps eight (f32: four) columns, `ct` threads cover a row's part, 256 / ct rows go
-// at once, and each thread asks for four rows before it uses the first.
+// dz = dy act'(pre), and the column sums of dz over this workgroup's rows (part [gridDim.x][N]).  dz is rounded to the element
+// type: bf16 is what the matrix cores multiply, and dz is the caller's gradient of `res`.  The products of a bf16 call are then
+// off by 0.0023 in norm, where the rounding of their own outputs alone gives 0.0017; two bf16 parts of dz would double both
+// products' time.  The column sums take it unrounded.
+// One pass over dy and pre and one write, bound by HBM: a thread keeps eight (f32: four) columns, `ct` threads cover a row's
+// part, 256 / ct rows go at once, and each thread asks for four rows before it uses the first.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long lddy, const T* pre, long ldp, T* dz, long lddz,
                                                         float* part, long M, long N, int act, int ct) {
@@ -1038,7 +1041,8 @@ int gemm_launch(const GemmArgs& a, unsigned grid, hipStream_t s) {
 
 // products for gemm_few_kernel: up to 64 rows, and in bf16 at most 16 MB of weights, whose rows it reads in pieces of 64
 // bytes (us, against the 64 tile; [K, N] weights): 4 rows bf16 2048 x 256: 5.6 / 12.9, 1024 x 1024: 6.0 / 6.7, 4096 x 4096:
-// 20.0 / 13.8; f32 2048 x 256: 13.0 / 21.5, 4096 x 4096: 24.3 / 27.4
+// 20.0 / 12.0; f32 2048 x 256: 13.0 / 21.5, 4096 x 4096: 23.2 / 27.4.  The rule does not look at the length of the contraction,
+// which only its four waves share: 32 x 262144 x 32 takes 284 us.
 bool gemm_is_few(int es, long M, long N, long K) { return M <= 64 && (es == 4 || K * N <= (1L << 23)); }
 
 constexpr long kMostTiles = 1L << 24;      // a launch holds less than 2^32 threads

@@ -4,7 +4,7 @@
 // Bound by HBM: one read and one write per element.  A thread holds the angles of one 16-byte vector's pairs in registers
 // and applies them to a group of heads of one token, so the trigonometry is paid once per group.
 // 2 x 8192 tokens, 20 heads of 128 f32: 69 us = 4.9 TB/s (a large copy: 5.0); 64 x 256 tokens, 8 heads of 64 bf16 out of a
-// fused projection: 9.4 us, of which the first loads, the angles and the launch are about half.
+// fused projection: 9.1 us, of which the first loads, the angles and the launch are about half.
 // Angles: the product of a position (below 2^29) and an f32 frequency is exact in f64; it is reduced to a fraction of a
 // turn in f64 and only that fraction goes through f32 sine and cosine, so far positions lose nothing.
 #include "blocks.h"
@@ -161,8 +161,9 @@ int launch_rope(int dtype, int interleaved, RopeArgs a, hipStream_t s) {
     LDM_REQUIRE(a.nchunk <= threads, "a head is longer than a workgroup");
     a.tpb = threads / a.nchunk;
     // a group of heads per workgroup, all of them where the tokens alone give eight workgroups per CU: the angles are taken
-    // once for a group.  2 x 8192 tokens, 20 heads of 128 in f32: 76.8 us in two groups of ten, 80.4 in one, 78.1 in four
-    // (and 100.6 with a workgroup per head); one token, 8 heads of 64: 5.2 us in four groups, 7.4 in one
+    // once for a group.  2 x 8192 tokens, 20 heads of 128 in f32: 69.6 us in two groups of ten, 72.8 in one, 70.6 in four, 93
+    // with a workgroup per head; 64 x 256 tokens, 8 heads of 64 in bf16: 9.1 in four groups, 9.5 in one, 12.5 per head; one
+    // token, 8 heads of 64: 4.7 in four, 7.6 in one
     const int heads = a.H[0] + a.H[1], es = dtype == LDM_BF16 ? 2 : 4;
     const long blocks = (a.tokens + a.tpb - 1) / a.tpb;
     long groups = 2048 / blocks;
